@@ -358,6 +358,7 @@ int ur_channel_shuffle(const void* x, void* y, int dtype, long long rows, int c,
 #define UR_ACT_LEAKYRELU 3
 #define UR_ACT_GELU 4
 #define UR_ACT_HSWISH 5
+#define UR_ACT_SILU 6 /* ur_gn_act_* only */
 int ur_act_fwd(const void* x, void* y, int dtype, long long count, int act, float slope, ur_stream_t s);
 int ur_act_bwd(const void* dy, const void* x, void* dx, int dtype, long long count, int act, float slope,
                ur_stream_t s);
@@ -447,6 +448,23 @@ int ur_confusion_matrix(const void* logits, int dtype, const int64_t* target, lo
  * loss: device scalar of the batch (NULL: none). */
 int ur_seg_metrics_accumulate(const unsigned long long* cm, int classes, const float* loss, double* acc7, ur_stream_t s);
 
+/* ---------------------------------------------------------------- GroupNorm + activation
+ * No counterpart in the reference, whose networks normalise per batch (S/C:95): the normalisation to use with few images
+ * per GPU.  One image's `hw` pixels x the c / groups channels of a group share a mean and a variance;
+ *   pre = (x - mean) / sqrt(var + eps) * gamma + beta (+ residual),  y = act(pre)
+ * x, residual, y and dy are NHWC with pixel pitches *_ld (0 = dense), dx and dres dense.  gamma / beta may be NULL (1 / 0).
+ * act: UR_ACT_*, slope for UR_ACT_LEAKYRELU.  stats: double[n][groups][2] = {mean, 1 / sqrt(var + eps)}, written by the
+ * forward and read by the backward pass.  Backward: any of dx, dres, dgamma, dbeta may be NULL (dres needs residual and dx).
+ * Sums are in a fixed order: the same call gives the same bits.  Workspace bytes: ur_gn_*_workspace (0: bad sizes). */
+size_t ur_gn_fwd_workspace(int dtype, int n, long long hw, int c, int groups);
+size_t ur_gn_bwd_workspace(int dtype, int n, long long hw, int c, int groups);
+int ur_gn_act_fwd(const void* x, int x_ld, const void* residual, int res_ld, const float* gamma, const float* beta, void* y,
+                  int y_ld, double* stats, int dtype, int n, long long hw, int c, int groups, float eps, int act, float slope,
+                  void* workspace, size_t ws_bytes, ur_stream_t s);
+int ur_gn_act_bwd(const void* dy, int dy_ld, const void* x, int x_ld, const void* residual, int res_ld, const float* gamma,
+                  const float* beta, const double* stats, void* dx, void* dres, float* dgamma, float* dbeta, int dtype, int n,
+                  long long hw, int c, int groups, int act, float slope, void* workspace, size_t ws_bytes, ur_stream_t s);
+
 /* ---------------------------------------------------------------- optimisers (multi-tensor)
  * optim.Adam(lr) (train_UResNetAblitionStudy.py:203) and optim.SGD(lr) (CNN-CIFAR10.py:130).
  * ptrs: device array of ntensors*{4|2} pointers (param, grad, exp_avg, exp_avg_sq | param, grad);
@@ -463,6 +481,39 @@ int ur_adam_multi_dev(const void* const* ptrs, const long long* sizes, int ntens
                       float beta1, float beta2, float eps, float weight_decay, float grad_scale, ur_stream_t s);
 int ur_sgd_multi(const void* const* ptrs, const long long* sizes, int ntensors, long long max_size, float lr,
                  float weight_decay, float grad_scale, ur_stream_t s);
+
+/* AdamW (decoupled weight decay) and gradient clipping by the global norm; no counterpart in the reference, which trains
+ * with Adam and without clipping.  The tensors are listed in HOST memory and travel as kernel arguments: no staging
+ * buffer, every call can be captured in a graph.
+ *   1. ur_param_table writes the list as a table in device memory (ur_param_table_bytes), counts the chunks of work into
+ *      *nchunks (host) and, where `steps` (int32 counts in device memory) is given, adds 1 to steps[slot] of every tensor
+ *      and stores the bias corrections of the new count.  Every slot at most once per call.
+ *   2. ur_grad_sqnorm (optional) writes *nparts (host; at most ur_grad_sqnorm_max_parts()) partial sums of the squared
+ *      gradients.  Several lists (parameter groups) can share one norm: give each its place in one array.
+ *   3. ur_adamw_multi makes the step.  nparts > 0: gradients are scaled by min(1, max_norm / (norm + 1e-6)), norm over all
+ *      `nparts` sums, and out_norm (may be NULL) gets the norm before clipping.  grad_scale multiplies every gradient first.
+ *      Moments lie in buffers of blocks of 256 elements, a tensor's first one at `block`: state_bits 32: fp32;
+ *      8: e4m3 codes of m and of sqrt(v) and an fp32 scale per block.
+ *   or ur_grad_clip scales the gradients in place.
+ * Parameters and gradients are dense fp32; tensors of a list must not overlap. */
+typedef struct {
+    void* param;      /* may be NULL for ur_grad_sqnorm / ur_grad_clip */
+    void* grad;
+    long long n;      /* elements */
+    long long block;  /* first block of 256 elements in the state buffers */
+    long long slot;   /* index into steps */
+} ur_param;
+size_t ur_param_table_bytes(int ntensors);
+int ur_param_table(const ur_param* list, int ntensors, void* table, size_t table_bytes, int* steps, double lr, double beta1,
+                   double beta2, long long* nchunks, ur_stream_t s);
+int ur_grad_sqnorm_max_parts(void);
+int ur_grad_sqnorm(const void* table, int ntensors, long long nchunks, double* parts, int* nparts, ur_stream_t s);
+int ur_grad_clip(const void* table, int ntensors, long long nchunks, const double* parts, int nparts, float max_norm,
+                 float* out_norm, ur_stream_t s);
+int ur_adamw_multi(const void* table, int ntensors, long long nchunks, int state_bits, void* exp_avg, void* exp_avg_sq,
+                   float* exp_avg_scale, float* exp_avg_sq_scale, double lr, double beta1, double beta2, double eps,
+                   double weight_decay, const double* parts, int nparts, float max_norm, float grad_scale, float* out_norm,
+                   ur_stream_t s);
 
 #ifdef __cplusplus
 }

@@ -12,7 +12,7 @@ HEADER_PATH = os.path.join(os.path.dirname(_HERE), "include", "uresnet_hip.h")
 
 UR_F32, UR_BF16 = 0, 1
 PACK_FWD, PACK_DGRAD, PACK_CONVT_FWD, PACK_CONVT_DGRAD = 0, 1, 2, 3
-ACT_NONE, ACT_RELU, ACT_RELU6, ACT_LEAKYRELU, ACT_GELU, ACT_HSWISH = range(6)
+ACT_NONE, ACT_RELU, ACT_RELU6, ACT_LEAKYRELU, ACT_GELU, ACT_HSWISH, ACT_SILU = range(7)
 
 
 class ConvDesc(C.Structure):
@@ -24,7 +24,7 @@ class UResNetHipError(RuntimeError):
     pass
 
 
-_vp, _i, _ll, _f, _sz = C.c_void_p, C.c_int, C.c_longlong, C.c_float, C.c_size_t
+_vp, _i, _ll, _f, _sz, _d = C.c_void_p, C.c_int, C.c_longlong, C.c_float, C.c_size_t, C.c_double
 _dp = C.POINTER(ConvDesc)
 
 # name -> (restype, argtypes); every symbol the header declares
@@ -142,9 +142,19 @@ SIGNATURES = {
     "ur_sigmoid_mask": (_i, [_vp, _i, _ll, _vp, _vp]),
     "ur_confusion_matrix": (_i, [_vp, _i, _vp, _ll, _i, _i, _ll, _vp, _vp]),
     "ur_seg_metrics_accumulate": (_i, [_vp, _i, _vp, _vp, _vp]),
+    "ur_gn_fwd_workspace": (_sz, [_i, _i, _ll, _i, _i]),
+    "ur_gn_bwd_workspace": (_sz, [_i, _i, _ll, _i, _i]),
+    "ur_gn_act_fwd": (_i, [_vp, _i, _vp, _i, _vp, _vp, _vp, _i, _vp, _i, _i, _ll, _i, _i, _f, _i, _f, _vp, _sz, _vp]),
+    "ur_gn_act_bwd": (_i, [_vp, _i, _vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _ll, _i, _i, _i, _f, _vp, _sz, _vp]),
     "ur_adam_multi": (_i, [_vp, _vp, _i, _ll, _f, _f, _f, _f, _f, _i, _f, _vp]),
     "ur_adam_multi_dev": (_i, [_vp, _vp, _i, _ll, _f, _f, _f, _f, _f, _f, _vp]),
     "ur_sgd_multi": (_i, [_vp, _vp, _i, _ll, _f, _f, _f, _vp]),
+    "ur_param_table_bytes": (_sz, [_i]),
+    "ur_param_table": (_i, [_vp, _i, _vp, _sz, _vp, _d, _d, _d, _vp, _vp]),
+    "ur_grad_sqnorm_max_parts": (_i, []),
+    "ur_grad_sqnorm": (_i, [_vp, _i, _ll, _vp, _vp, _vp]),
+    "ur_grad_clip": (_i, [_vp, _i, _ll, _vp, _i, _f, _vp, _vp]),
+    "ur_adamw_multi": (_i, [_vp, _i, _ll, _i, _vp, _vp, _vp, _vp, _d, _d, _d, _d, _d, _vp, _i, _f, _f, _vp, _vp]),
 }
 
 _lib = None

@@ -1,0 +1,384 @@
+// AdamW over many tensors at once, with the moments in 32 or in 8 bits, and gradient clipping by the global norm.
+//
+//   factor = grad_scale * min(1, max_norm / (norm + 1e-6)),  norm = grad_scale * sqrt(sum over all tensors of grad^2)
+//   g = factor * grad;  m += (g - m) (1 - b1);  v = b2 v + (1 - b2) g^2
+//   p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//
+// Bound by HBM: 28 bytes per element with 32-bit moments, 16 + 1/16 with 8-bit ones, 4 more where the norm is taken (the
+// gradients are read twice, the second time partly from the last-level cache).
+//
+// Work list.  The host hands over the tensors by value (ur_param rows, as kernel arguments); param_table_kernel writes them
+// as a table in the caller's workspace, advances the step counts and derives the bias corrections.  No staging buffer and
+// no copy from the host: a captured graph replays the whole step.  The other kernels walk chunks of 2048 elements of all
+// tensors in one launch and find a chunk's tensor in the sorted list of first chunks, 64 entries per look.
+//
+// 8-bit moments.  m and r = sqrt(v) are stored as e4m3 codes (3 mantissa bits, exponents over 2^17) with one fp32 scale per
+// 256 elements that maps the block's largest value to the largest code, 448.  m is rounded to the nearest code: it moves by
+// a tenth of itself per step, more than half a code step (3 to 6 %).  r moves by at most 0.05 % per step when the gradients
+// get smaller, so nearest rounding would pin it for good; it is rounded up with the probability of its fraction instead,
+// so that its expectation follows the recurrence.  The 20 random bits per element come from a hash of the element's place
+// in the state and the step count: the same step gives the same bits, and nothing is kept between calls.  The step itself
+// uses m and v before they are rounded.
+#include "ur_common.h"
+
+namespace {
+
+constexpr int NT = 256;
+constexpr int BLOCK = 256;                   // elements per scale
+constexpr int CHUNK = 2048;                  // elements per unit of work: two 16-byte accesses per thread and tensor
+constexpr int BATCH = 80;                    // rows per table launch: kernel arguments stay under 4 KB
+constexpr int MAX_PARTS = 1024;              // partial sums of the norm
+constexpr float TOP = 448.f;
+
+typedef __attribute__((ext_vector_type(4))) float fvec4_t;
+typedef __attribute__((ext_vector_type(2))) float fvec2_t;
+
+struct Row {
+    float* p;
+    float* g;
+    long long n;
+    long long block;                         // first block of 256 elements in the state buffers
+    float step_size, bc2_sqrt;               // lr / (1 - b1^t), sqrt(1 - b2^t)
+    unsigned step;
+    unsigned pad;
+};
+
+struct ListRow {
+    void* p;
+    void* g;
+    long long n, block;
+    int slot, first;
+};
+struct ListBatch {
+    int count, at;
+    ListRow r[BATCH];
+};
+
+// table: Row[ntensors], then int first[ntensors] (first chunk of every tensor)
+__device__ __forceinline__ const int* firsts(const Row* rows, int ntensors) { return reinterpret_cast<const int*>(rows + ntensors); }
+
+__global__ __launch_bounds__(128) void param_table_kernel(ListBatch b, Row* __restrict__ rows, int ntensors, int* __restrict__ steps,
+                                                          double lr, double beta1, double beta2) {
+    const int i = threadIdx.x;
+    if (i >= b.count) return;
+    const ListRow l = b.r[i];
+    Row w;
+    w.p = (float*)l.p;
+    w.g = (float*)l.g;
+    w.n = l.n;
+    w.block = l.block;
+    w.step_size = 0.f;
+    w.bc2_sqrt = 1.f;
+    w.step = 0;
+    w.pad = 0;
+    if (steps) {
+        const int t = steps[l.slot] + 1;
+        steps[l.slot] = t;
+        w.step = (unsigned)t;
+        w.step_size = (float)(lr / (1.0 - pow(beta1, (double)t)));
+        w.bc2_sqrt = (float)sqrt(1.0 - pow(beta2, (double)t));
+    }
+    rows[b.at + i] = w;
+    reinterpret_cast<int*>(rows + ntensors)[b.at + i] = l.first;
+}
+
+// the tensor that a chunk belongs to: the last entry of the sorted list that is not above it (a whole wave looks)
+__device__ __forceinline__ int find_tensor(const int* __restrict__ first, int ntensors, int chunk) {
+    const int lane = threadIdx.x & 63;
+    int lo = 0, len = ntensors;
+    while (len > 1) {
+        const int step = (len + 63) >> 6, at = lane * step;
+        const bool below = at < len && first[lo + at] <= chunk;
+        const int hits = __popcll(__ballot(below));                          // entries are sorted: a prefix of the lanes
+        lo += (hits - 1) * step;
+        len = min(step, len - (hits - 1) * step);
+    }
+    return __builtin_amdgcn_readfirstlane(lo);
+}
+
+__device__ __forceinline__ double wave_sum(double v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    return v;
+}
+// sum over a workgroup of NT threads, in every thread
+__device__ __forceinline__ double group_sum(double v) {
+    __shared__ double red[NT / 64];
+    v = wave_sum(v);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return (red[0] + red[1]) + (red[2] + red[3]);
+}
+
+__device__ __forceinline__ bool aligned16(const void* a, const void* b) { return (((uintptr_t)a | (uintptr_t)b) & 15) == 0; }
+
+// squares summed in 64 bits (two fp64 instructions per element against the four bytes it is read by)
+__global__ __launch_bounds__(NT) void grad_sqnorm_kernel(const Row* __restrict__ rows, int ntensors, int nchunks, double* __restrict__ parts) {
+    const int* first = firsts(rows, ntensors);
+    double s = 0.0;
+    for (int c = blockIdx.x; c < nchunks; c += gridDim.x) {
+        const int t = find_tensor(first, ntensors, c);
+        const long long base = (long long)(c - first[t]) * CHUNK, n = rows[t].n;
+        const float* g = rows[t].g;
+        const bool vec = aligned16(g, g);
+#pragma unroll
+        for (int u = 0; u < CHUNK / (NT * 4); ++u) {
+            const long long e = base + u * (NT * 4) + threadIdx.x * 4;
+            if (vec && e + 4 <= n) {
+                const fvec4_t v = *reinterpret_cast<const fvec4_t*>(g + e);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s = fma((double)v[i], (double)v[i], s);
+            } else {
+                for (long long i = e; i < e + 4 && i < n; ++i) s = fma((double)g[i], (double)g[i], s);
+            }
+        }
+    }
+    s = group_sum(s);
+    if (threadIdx.x == 0) parts[blockIdx.x] = s;
+}
+
+// the factor every gradient is multiplied by; workgroup 0 writes the norm
+__device__ __forceinline__ float clip_factor(const double* __restrict__ parts, int nparts, float max_norm, float grad_scale,
+                                             float* __restrict__ out_norm) {
+    double s = 0.0;
+    for (int i = threadIdx.x; i < nparts; i += NT) s += parts[i];
+    const float norm = (float)(sqrt(group_sum(s)) * (double)fabsf(grad_scale));
+    if (out_norm && blockIdx.x == 0 && threadIdx.x == 0) *out_norm = norm;
+    float f = max_norm / (norm + 1e-6f);
+    if (f > 1.f) f = 1.f;                                                    // (a NaN norm stays one)
+    return f * grad_scale;
+}
+
+__global__ __launch_bounds__(NT) void grad_scale_kernel(const Row* __restrict__ rows, int ntensors, int nchunks,
+                                                        const double* __restrict__ parts, int nparts, float max_norm,
+                                                        float* __restrict__ out_norm) {
+    const float f = clip_factor(parts, nparts, max_norm, 1.f, out_norm);
+    if (f == 1.f) return;                                                    // within the limit: nothing to write
+    const int* first = firsts(rows, ntensors);
+    for (int c = blockIdx.x; c < nchunks; c += gridDim.x) {
+        const int t = find_tensor(first, ntensors, c);
+        const long long base = (long long)(c - first[t]) * CHUNK, n = rows[t].n;
+        float* g = rows[t].g;
+        const bool vec = aligned16(g, g);
+#pragma unroll
+        for (int u = 0; u < CHUNK / (NT * 4); ++u) {
+            const long long e = base + u * (NT * 4) + threadIdx.x * 4;
+            if (vec && e + 4 <= n) *reinterpret_cast<fvec4_t*>(g + e) = *reinterpret_cast<const fvec4_t*>(g + e) * f;
+            else for (long long i = e; i < e + 4 && i < n; ++i) g[i] *= f;
+        }
+    }
+}
+
+// ------------------------------------------------------------------ 8-bit codes
+// 20 pseudo-random bits for element `place` of the state at step `step`: a multiplicative hash of both
+__device__ __forceinline__ unsigned dither(unsigned place, unsigned step) {
+    unsigned h = place * 0x9E3779B9u + step * 0xA3D8F1B5u;
+    h = (h ^ (h >> 16)) * 0x45D9F3B5u;
+    h = (h ^ (h >> 15)) * 0x2C92774Du;
+    return (h ^ (h >> 16)) & 0xFFFFFu;
+}
+__device__ __forceinline__ bool is_finite(float v) { return (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u; }
+
+__device__ __forceinline__ fvec4_t decode4(unsigned q) {
+    const fvec2_t a = __builtin_amdgcn_cvt_pk_f32_fp8((int)q, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)q, true);
+    fvec4_t v = {a[0], a[1], b[0], b[1]};
+    return v;
+}
+// nearest codes of values within [-448, 448]
+__device__ __forceinline__ unsigned encode4(fvec4_t y) {
+    int q = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+    return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], q, true);
+}
+// y in [0, 448]: the code below plus one with the probability of the fraction.  Normal codes drop 20 mantissa bits, so
+// adding the dither there carries into the code; below 2^-6 the codes are multiples of 2^-9.
+__device__ __forceinline__ unsigned encode_up(float y, unsigned d) {
+    if (y < 0.015625f) return ((unsigned)(y * 536870912.f) + d) >> 20;       // y * 2^9 * 2^20
+    return ((__float_as_uint(y) + d) >> 20) - ((127 - 7) << 3);
+}
+constexpr unsigned CODE_NAN = 0x7f;
+
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+    return v;
+}
+
+struct Hyper {
+    float b1c, b2, b2c, eps, keep;           // 1 - b1, b2, 1 - b2, eps, 1 - lr * wd
+};
+
+// Every operation rounded by itself: the codes of an 8-bit state are then a function of the inputs alone, and not of which
+// products the compiler contracts (a value next to a border between two codes would go another way).
+__device__ __forceinline__ void adamw_one(float& p, float g, float& m, float& v, float& root, const Hyper& h, float step_size, float bc2_sqrt) {
+#pragma clang fp contract(off)
+    m = m + (g - m) * h.b1c;
+    v = v * h.b2 + (h.b2c * g) * g;
+    root = sqrtf(v);
+    p = p * h.keep - step_size * (m / (root / bc2_sqrt + h.eps));
+}
+
+// BITS 32: m, v fp32.  BITS 8: m, v are codes (the root of the second moment) with one scale per block of 256; a wave owns a
+// block, four elements per lane.
+template <int BITS>
+__global__ __launch_bounds__(NT) void adamw_kernel(const Row* __restrict__ rows, int ntensors, int nchunks, void* __restrict__ m_,
+                                                   void* __restrict__ v_, float* __restrict__ ms, float* __restrict__ vs, Hyper h,
+                                                   const double* __restrict__ parts, int nparts, float max_norm, float grad_scale,
+                                                   float* __restrict__ out_norm) {
+    float factor = grad_scale;
+    if (nparts) factor = clip_factor(parts, nparts, max_norm, grad_scale, out_norm);
+    const int* first = firsts(rows, ntensors);
+    for (int c = blockIdx.x; c < nchunks; c += gridDim.x) {
+        const int t = find_tensor(first, ntensors, c);
+        const Row row = rows[t];
+        const long long base = (long long)(c - first[t]) * CHUNK, n = row.n;
+        const bool vec = aligned16(row.p, row.g);
+        constexpr int U = CHUNK / (NT * 4);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const long long e = base + u * (NT * 4) + threadIdx.x * 4;
+            const long long wave0 = base + u * (NT * 4) + (threadIdx.x & ~63) * 4;      // first element of the wave's block
+            if (wave0 >= n) break;
+            fvec4_t p = {0.f, 0.f, 0.f, 0.f}, g = p, m, v, root;
+            const bool full = vec && e + 4 <= n;
+            if (full) {
+                p = *reinterpret_cast<const fvec4_t*>(row.p + e);
+                g = *reinterpret_cast<const fvec4_t*>(row.g + e);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) if (e + i < n) { p[i] = row.p[e + i]; g[i] = row.g[e + i]; }
+            }
+            const long long at = row.block * BLOCK + e;                      // the state is padded to whole blocks
+            const long long blk = row.block + wave0 / BLOCK;
+            if constexpr (BITS == 32) {
+                m = reinterpret_cast<const fvec4_t*>(m_)[at >> 2];
+                v = reinterpret_cast<const fvec4_t*>(v_)[at >> 2];
+            } else {
+                m = decode4(reinterpret_cast<const unsigned*>(m_)[at >> 2]) * ms[blk];
+                v = decode4(reinterpret_cast<const unsigned*>(v_)[at >> 2]) * vs[blk];
+                v = v * v;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float pi = p[i], mi = m[i], vi = v[i], ri;
+                adamw_one(pi, g[i] * factor, mi, vi, ri, h, row.step_size, row.bc2_sqrt);
+                p[i] = pi; m[i] = mi; v[i] = vi; root[i] = ri;
+            }
+            if (full) *reinterpret_cast<fvec4_t*>(row.p + e) = p;
+            else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) if (e + i < n) row.p[e + i] = p[i];
+            }
+            if constexpr (BITS == 32) {
+                reinterpret_cast<fvec4_t*>(m_)[at >> 2] = m;
+                reinterpret_cast<fvec4_t*>(v_)[at >> 2] = v;
+            } else {
+                // scales from the finite values; an infinite or NaN value becomes the NaN code and stays alone
+                float am = 0.f, ar = 0.f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (is_finite(m[i])) am = fmaxf(am, fabsf(m[i]));
+                    if (is_finite(root[i])) ar = fmaxf(ar, root[i]);
+                }
+                am = fmaxf(wave_max(am), 0x1p-100f);                          // keeps 448 / am finite
+                ar = fmaxf(wave_max(ar), 0x1p-100f);
+                const float im = 1.f / am * TOP, ir = 1.f / ar * TOP;
+                fvec4_t y;
+                unsigned qr = 0, bad = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    y[i] = fminf(fmaxf(m[i] * im, -TOP), TOP);
+                    unsigned cr = encode_up(fminf(root[i] * ir, TOP), dither((unsigned)(at + i), row.step));
+                    if (!is_finite(root[i])) cr = CODE_NAN;
+                    if (!is_finite(m[i])) bad |= CODE_NAN << (8 * i);
+                    qr |= cr << (8 * i);
+                }
+                reinterpret_cast<unsigned*>(m_)[at >> 2] = encode4(y) | bad;
+                reinterpret_cast<unsigned*>(v_)[at >> 2] = qr;
+                if ((threadIdx.x & 63) == 0) { ms[blk] = am * (1.f / TOP); vs[blk] = ar * (1.f / TOP); }
+            }
+        }
+    }
+}
+
+// chunks of all tensors; -1: a bad row
+long long count_chunks(const ur_param* list, int ntensors) {
+    long long chunks = 0;
+    for (int i = 0; i < ntensors; ++i) {
+        if (!list[i].grad || list[i].n <= 0 || list[i].n > (1LL << 40) || list[i].block < 0 || list[i].slot < 0 || list[i].slot > 0x7fffffffLL) return -1;
+        chunks += (list[i].n + CHUNK - 1) / CHUNK;
+    }
+    return chunks;
+}
+
+int norm_parts(long long chunks) { return (int)(chunks < MAX_PARTS ? chunks : MAX_PARTS); }
+
+}  // namespace
+
+extern "C" {
+
+size_t ur_param_table_bytes(int ntensors) { return ntensors <= 0 ? 0 : (size_t)ntensors * (sizeof(Row) + sizeof(int)); }
+int ur_grad_sqnorm_max_parts(void) { return MAX_PARTS; }
+
+int ur_param_table(const ur_param* list, int ntensors, void* table, size_t table_bytes, int* steps, double lr, double beta1, double beta2,
+                   long long* nchunks, ur_stream_t s) {
+    UR_REQUIRE(list && ntensors > 0 && table && nchunks, "param_table: bad arguments");
+    UR_REQUIRE(table_bytes >= ur_param_table_bytes(ntensors), "param_table: table too small");
+    const long long chunks = count_chunks(list, ntensors);
+    UR_REQUIRE(chunks > 0 && chunks <= 0x7fffffffLL, "param_table: a tensor without gradient or elements, or too many elements");
+    int first = 0;
+    for (int at = 0; at < ntensors; at += BATCH) {
+        ListBatch b;
+        b.count = ntensors - at < BATCH ? ntensors - at : BATCH;
+        b.at = at;
+        for (int i = 0; i < b.count; ++i) {
+            const ur_param& l = list[at + i];
+            b.r[i].p = l.param;
+            b.r[i].g = l.grad;
+            b.r[i].n = l.n;
+            b.r[i].block = l.block;
+            b.r[i].slot = (int)l.slot;
+            b.r[i].first = first;
+            first += (int)((l.n + CHUNK - 1) / CHUNK);
+        }
+        for (int i = b.count; i < BATCH; ++i) b.r[i] = b.r[0];
+        hipLaunchKernelGGL(param_table_kernel, dim3(1), dim3(128), 0, (hipStream_t)s, b, (Row*)table, ntensors, steps, lr, beta1, beta2);
+    }
+    *nchunks = chunks;
+    return ur_check_launch("param_table");
+}
+
+int ur_grad_sqnorm(const void* table, int ntensors, long long nchunks, double* parts, int* nparts, ur_stream_t s) {
+    UR_REQUIRE(table && ntensors > 0 && nchunks > 0 && nchunks <= 0x7fffffffLL && parts && nparts, "grad_sqnorm: bad arguments");
+    *nparts = norm_parts(nchunks);
+    hipLaunchKernelGGL(grad_sqnorm_kernel, dim3(*nparts), dim3(NT), 0, (hipStream_t)s, (const Row*)table, ntensors, (int)nchunks, parts);
+    return ur_check_launch("grad_sqnorm");
+}
+
+int ur_grad_clip(const void* table, int ntensors, long long nchunks, const double* parts, int nparts, float max_norm, float* out_norm,
+                 ur_stream_t s) {
+    UR_REQUIRE(table && ntensors > 0 && nchunks > 0 && nchunks <= 0x7fffffffLL && parts && nparts > 0, "grad_clip: bad arguments");
+    hipLaunchKernelGGL(grad_scale_kernel, dim3(norm_parts(nchunks)), dim3(NT), 0, (hipStream_t)s, (const Row*)table, ntensors, (int)nchunks,
+                       parts, nparts, max_norm, out_norm);
+    return ur_check_launch("grad_clip");
+}
+
+int ur_adamw_multi(const void* table, int ntensors, long long nchunks, int state_bits, void* exp_avg, void* exp_avg_sq, float* exp_avg_scale,
+                   float* exp_avg_sq_scale, double lr, double beta1, double beta2, double eps, double weight_decay, const double* parts,
+                   int nparts, float max_norm, float grad_scale, float* out_norm, ur_stream_t s) {
+    UR_REQUIRE(table && ntensors > 0 && nchunks > 0 && nchunks <= 0x7fffffffLL && exp_avg && exp_avg_sq, "adamw_multi: bad arguments");
+    UR_REQUIRE(state_bits == 32 || state_bits == 8, "adamw_multi: state_bits is 32 or 8 (got %d)", state_bits);
+    UR_REQUIRE(state_bits == 32 || (exp_avg_scale && exp_avg_sq_scale), "adamw_multi: 8-bit states without scales");
+    UR_REQUIRE((((uintptr_t)exp_avg | (uintptr_t)exp_avg_sq) & 15) == 0, "adamw_multi: the state buffers are not 16-byte aligned");
+    UR_REQUIRE(nparts == 0 || (nparts > 0 && parts), "adamw_multi: bad partial sums");
+    const Hyper h = {(float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)eps, (float)(1.0 - lr * weight_decay)};
+    const int grid = (int)(nchunks < 1024 ? nchunks : 1024);
+    if (state_bits == 32)
+        hipLaunchKernelGGL(adamw_kernel<32>, dim3(grid), dim3(NT), 0, (hipStream_t)s, (const Row*)table, ntensors, (int)nchunks, exp_avg,
+                           exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, h, parts, nparts, max_norm, grad_scale, out_norm);
+    else
+        hipLaunchKernelGGL(adamw_kernel<8>, dim3(grid), dim3(NT), 0, (hipStream_t)s, (const Row*)table, ntensors, (int)nchunks, exp_avg,
+                           exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, h, parts, nparts, max_norm, grad_scale, out_norm);
+    return ur_check_launch("adamw_multi");
+}
+
+}  // extern "C"

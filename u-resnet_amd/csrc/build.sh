@@ -9,7 +9,7 @@ HIPCC="${HIPCC:-/opt/rocm/bin/hipcc}"
 # packed fp32 instructions off: some of their forms have given wrong results on this hardware (the host pass does not know
 # the feature and says so; the warning is harmless)
 FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wall -Wno-unused-function -Xclang -target-feature -Xclang -packed-fp32-ops ${URESNET_EXTRA_FLAGS:-}"
-SRCS=(common conv_igemm convt_gemm conv1x1_pw conv1x1_pw_wgrad conv3x3_tile conv3x3_wide wgrad3x3_tile conv_wgrad conv_group bn spatial loss optim)
+SRCS=(common conv_igemm convt_gemm conv1x1_pw conv1x1_pw_wgrad conv3x3_tile conv3x3_wide wgrad3x3_tile conv_wgrad conv_group bn gnorm spatial loss optim adamw)
 pids=()
 for s in "${SRCS[@]}"; do
     src="$HERE/$s.hip"

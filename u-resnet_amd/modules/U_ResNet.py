@@ -48,7 +48,7 @@ class _TwoBranch(ResTrunk):
         with on_side():
             res = self._res_forward(x)
         n, _, h, w = x.shape
-        c_u, c_res = self.up4.conv[3].out_channels, self.out_conv[0].num_features - self.up4.conv[3].out_channels
+        c_u, c_res = self.up4.conv[3].out_channels, self.out_conv[2].in_channels - self.up4.conv[3].out_channels
         head_conv = self.out_conv[2]
         if (res.shape[2] * 2 == h and res.shape[3] * 2 == w and not has_hooks(self.out_conv, *self.out_conv)
                 and head_conv.stride == (1, 1) and head_conv.padding == (0, 0) and head_conv.groups == 1
@@ -59,7 +59,7 @@ class _TwoBranch(ResTrunk):
             # tensor are 128- and 32-byte runs at a 160-byte pitch: partial memory lines in every pass that touches them.)
             with on_side():
                 res_out = self.Upsample(res)
-            u_out = unet_branch_forward(self, x, out_stats=self.out_conv[0].training)   # (the head's BatchNorm comes next)
+            u_out = unet_branch_forward(self, x, out_stats=hnn.wants_stats(self.out_conv[0]))   # (the head's BatchNorm comes next)
             if fork is not None:
                 fork.join(res_out)
             z = ops.bn_relu_conv1x1_pair(ops.dense(u_out), ops.dense(res_out), self.out_conv[0], head_conv)

@@ -10,9 +10,11 @@ import torch
 
 from .. import _lib, ops
 from .. import nn as hnn
-from ..nn import act_dtype, conv_bn_act, has_hooks
+from ..nn import act_dtype, conv_bn_act, has_hooks, is_group_norm, wants_stats
 
 _ACT_CODES = {hnn.ReLU: _lib.ACT_RELU}
+_GN_ACT_CODES = {hnn.ReLU: _lib.ACT_RELU, hnn.ReLU6: _lib.ACT_RELU6, hnn.LeakyReLU: _lib.ACT_LEAKYRELU, hnn.GELU: _lib.ACT_GELU,
+                 hnn.Hardswish: _lib.ACT_HSWISH}          # a GroupNorm fuses these too (ops.gn_act)
 
 
 def channel_shuffle(x, groups):
@@ -43,6 +45,8 @@ def _cba(seq, x, i, out=None, pool=False, out_stats=False):
     channel window for the result (honoured on the fused path only; callers compare data_ptr()).  pool: the caller
     max-pools the result next, out_stats: the caller normalises it with another BatchNorm next (ops.bn_act)."""
     conv, bn, act = seq[i], seq[i + 1], seq[i + 2]
+    if is_group_norm(bn) and type(act) in _GN_ACT_CODES and getattr(act, 'approximate', 'none') == 'none':
+        return ops.gn_act(conv.raw(x)[0], bn, act=_GN_ACT_CODES[type(act)], slope=getattr(act, 'negative_slope', 0.0), out=out)
     if type(act) in _ACT_CODES:
         return conv_bn_act(x, conv, bn, _ACT_CODES[type(act)], out=out, pool=pool, out_stats=out_stats)
     return act(conv_bn_act(x, conv, bn, _lib.ACT_NONE))
@@ -59,7 +63,7 @@ def _cba_conv1x1(seq, x, i, pw, out=None):
     n, _, h, w = x.shape
     if n * h * w < 1 << 16 or x.dtype != torch.bfloat16:          # (below that the streaming backward-weight kernel is not used)
         return None
-    y, stats = conv.raw(x, want_stats=bn.training)
+    y, stats = conv.raw(x, want_stats=wants_stats(bn))
     z = ops.bn_relu_conv1x1(y, bn, pw, stats=stats, out=out)
     if z is None:                                                # not covered after all: finish the stage the usual way
         a = ops.bn_act(y, bn, stats=stats, act=_lib.ACT_RELU)
@@ -259,7 +263,7 @@ class BasicBlock(hnn.Module):
         if fuse_residual_grad and x.requires_grad and x.is_cuda and self.left[0].groups == 1:
             # the shortcut reads an alias of x handed out by the first convolution, whose backward-data kernel then
             # adds the shortcut's gradient in its epilogue
-            y, stats, xs = self.left[0].raw(x, want_stats=self.left[1].training, want_alias=True)
+            y, stats, xs = self.left[0].raw(x, want_stats=wants_stats(self.left[1]), want_alias=True)
             out = ops.bn_act(y, self.left[1], stats=stats, act=_lib.ACT_RELU)
         else:
             out, xs = _cba(self.left, x, 0), x

@@ -98,6 +98,44 @@ class BatchNorm2d(tnn.BatchNorm2d):
         return ops.bn_act(ops.as_activation(x, act_dtype(x)), self, act=_lib.ACT_NONE)
 
 
+class GroupNorm(tnn.GroupNorm):
+    """nn.GroupNorm over NHWC activations; containers fuse it with the activation that follows (ops.gn_act)."""
+
+    def forward(self, x):
+        return ops.gn_act(x, self, act=_lib.ACT_NONE)
+
+
+def is_group_norm(norm):
+    return isinstance(norm, tnn.GroupNorm)
+
+
+def wants_stats(norm):
+    """Whether the normalisation takes the per-channel sums of its input from the convolution's epilogue."""
+    return norm.training and not is_group_norm(norm)
+
+
+def to_group_norm(module, num_groups=32):
+    """Replace every BatchNorm2d inside `module` by a GroupNorm over the same channels, in place, and return the module (a
+    BatchNorm2d itself: its replacement).  Weight, bias, eps and training mode are kept, running statistics are dropped.
+    num_groups: the largest number of groups; layers whose channels it does not divide get the largest divisor below it.
+    Call it before an optimiser or a data-parallel wrapper takes the parameters."""
+    if int(num_groups) < 1:
+        raise ValueError("to_group_norm: num_groups must be positive (got %r)" % (num_groups,))
+    if isinstance(module, tnn.BatchNorm2d):
+        c = module.num_features
+        groups = max(g for g in range(1, min(int(num_groups), c) + 1) if c % g == 0)
+        gn = GroupNorm(groups, c, eps=module.eps, affine=module.affine)
+        if module.affine:
+            gn.weight, gn.bias = module.weight, module.bias
+        gn.train(module.training)
+        return gn
+    for name, child in list(module.named_children()):
+        new = to_group_norm(child, num_groups)
+        if new is not child:
+            setattr(module, name, new)
+    return module
+
+
 class ReLU(tnn.ReLU):
     """inplace is accepted for signature compatibility; the kernel writes a new tensor."""
 
@@ -190,13 +228,14 @@ fuse_eval_bn = True          # False: inference runs convolution and BatchNorm a
 
 
 def conv_bn_act(x, conv, bn, act=_lib.ACT_RELU, residual=None, out=None, pool=False, out_stats=False):
-    """conv -> BatchNorm (training statistics taken from the conv kernel's epilogue) -> (+residual) -> act.
+    """conv -> BatchNorm (training statistics taken from the conv kernel's epilogue) -> (+residual) -> act; `bn` may be a
+    GroupNorm.
     Inference (bn in eval mode under torch.no_grad()): BatchNorm is folded into the convolution's epilogue."""
-    if (fuse_eval_bn and not bn.training and not torch.is_grad_enabled() and isinstance(conv, Conv2d) and conv.groups == 1
+    if (fuse_eval_bn and not is_group_norm(bn) and not bn.training and not torch.is_grad_enabled() and isinstance(conv, Conv2d) and conv.groups == 1
             and conv.bias is None and (conv._k, conv._s, conv._p) == (3, 1, 1)):
         xa = ops.as_activation(x, act_dtype(x), allow_window=True)
         z = ops.conv3x3_bn_eval(xa, conv.weight, conv._packs, bn, act, residual, out)
         if z is not None:
             return z
-    y, stats = conv.raw(x, want_stats=bn.training)
+    y, stats = conv.raw(x, want_stats=wants_stats(bn))
     return ops.bn_act(y, bn, residual=residual, stats=stats, act=act, out=out, pool=pool, out_stats=out_stats)

@@ -6,12 +6,14 @@ memory, streams and the autograd tape only: all arithmetic runs in the hand-writ
 kernels.  Parameters and their gradients are fp32 in PyTorch's native layouts, so
 state_dicts are interchangeable with the reference's.
 """
+import contextlib
 import ctypes as C
 import os
 import weakref
 
 import torch
 from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import ConvDesc, call, query
@@ -46,6 +48,11 @@ def _require_gpu(t):
     if not t.is_cuda:
         raise _lib.UResNetHipError("u-resnet_amd operators run on the GPU only (got a %s tensor); "
                                    "there is no CPU fallback" % t.device)
+
+
+def _on(device):
+    """Context in which launches, allocations and streams are those of `device`."""
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def empty_nhwc(n, c, h, w, dtype, device):
@@ -128,6 +135,12 @@ def _channel_pitch(x):
     if s[1] == 1 and ld >= c and s[2] == w * ld and s[0] == h * w * ld:
         return ld
     return 0
+
+
+def _pitch(x):
+    """Channel pitch of a dense NHWC tensor or a channel window of one; 0 if x is neither.  (Sizes of one leave strides
+    without meaning: a dense tensor is recognised by its memory format.)"""
+    return x.shape[1] if _is_nhwc_dense(x) else _channel_pitch(x)
 
 
 def _g(g):
@@ -990,7 +1003,9 @@ def bn_act(y, bn, residual=None, stats=None, act=_lib.ACT_RELU, out=None, pool=F
     where the fused kernel covers the shape the pooled tensor is computed in the same pass and travels with the result
     (attribute `_ur_pooled`).  out_stats: the caller normalises the result with another BatchNorm next
     (bn_relu_conv1x1_pair); where the fused kernel covers the shape the per-channel sums of the result travel with it
-    (attribute `_ur_out_stats`)."""
+    (attribute `_ur_out_stats`).  `bn` may be a GroupNorm: then this is gn_act, and stats, pool and out_stats say nothing."""
+    if isinstance(bn, torch.nn.GroupNorm):
+        return gn_act(y, bn, residual=residual, act=act, out=out)
     training = bn.training or bn.running_mean is None
     if training and bn.momentum is None:
         raise NotImplementedError("BatchNorm2d(momentum=None) (cumulative average) is not implemented")
@@ -1012,6 +1027,94 @@ def bn_act(y, bn, residual=None, stats=None, act=_lib.ACT_RELU, out=None, pool=F
     if ohold:
         z._ur_out_stats = (ohold[0], z.data_ptr(), z._version)
     return z
+
+
+class _GNAct(Function):
+    """act(GroupNorm(x) (+ residual)).  Saved: x, the residual (its activation's derivative needs the sum) and the fp64
+    {mean, rstd} of every image and group; the pre-activation is recomputed from them in backward."""
+
+    @staticmethod
+    def forward(ctx, x, gamma, beta, residual, groups, eps, act, slope, out):
+        n, c, h, w = x.shape
+        dev = x.device
+        if out is None:
+            z, z_ld = empty_nhwc(n, c, h, w, x.dtype, dev), c
+        else:                                        # (window,): a channel window of a wider tensor (alias_window)
+            z = out[0]
+            z_ld = _channel_pitch(z)
+            if tuple(z.shape) != tuple(x.shape) or z.dtype != x.dtype or z.device != dev or not z_ld:
+                raise RuntimeError("gn_act: `out` must be a channel window with x's shape, dtype and device")
+        stats = torch.empty((n, groups, 2), dtype=torch.float64, device=dev)
+        tb = x.numel() * x.element_size()
+        with _on(dev), _Timed("hbm:gn_fwd", tb * (3 if residual is not None else 2)):
+            ws = _workspace(query("ur_gn_fwd_workspace", _dt(x), n, h * w, c, groups), dev)
+            call("ur_gn_act_fwd", x.data_ptr(), _pitch(x), _p(residual), 0 if residual is None else _pitch(residual), _p(gamma),
+                 _p(beta), z.data_ptr(), z_ld, stats.data_ptr(), _dt(x), n, h * w, c, groups, eps, act, slope, ws.data_ptr(),
+                 ws.numel(), _stream())
+        # without an activation the residual's gradient is dz itself and nothing depends on the residual's values
+        ctx.save_for_backward(x, gamma, beta, residual if act != _lib.ACT_NONE else None, stats)
+        ctx.groups, ctx.act, ctx.slope, ctx.has_res = groups, act, slope, residual is not None
+        return z
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dz):
+        x, gamma, beta, residual, stats = ctx.saved_tensors
+        need_x, need_gamma, need_beta, need_res = ctx.needs_input_grad[:4]
+        n, c, h, w = x.shape
+        dev = x.device
+        dz_ld = _pitch(dz) if dz.dtype == x.dtype else 0
+        if not dz_ld:
+            dz, dz_ld = (_g(dz) if dz.dtype == x.dtype else to_nhwc_raw(dz, x.dtype)), c
+        if residual is None and not (need_x or need_gamma or need_beta):
+            return None, None, None, (dz if need_res else None), None, None, None, None, None
+        need_dres = residual is not None and need_res
+        dx = empty_nhwc(n, c, h, w, x.dtype, dev) if (need_x or need_dres) else None
+        dres = empty_nhwc(n, c, h, w, x.dtype, dev) if need_dres else None
+        dgamma = grad_buffer(gamma) if need_gamma else None
+        dbeta = grad_buffer(beta) if need_beta else None
+        tb = x.numel() * x.element_size()
+        with _on(dev), _Timed("hbm:gn_bwd", tb * (2 + (dx is not None) + (residual is not None) + need_dres)):
+            ws = _workspace(query("ur_gn_bwd_workspace", _dt(x), n, h * w, c, ctx.groups), dev)
+            call("ur_gn_act_bwd", dz.data_ptr(), dz_ld, x.data_ptr(), _pitch(x), _p(residual),
+                 0 if residual is None else _pitch(residual), _p(gamma), _p(beta), stats.data_ptr(), _p(dx), _p(dres), _p(dgamma),
+                 _p(dbeta), _dt(x), n, h * w, c, ctx.groups, ctx.act, ctx.slope, ws.data_ptr(), ws.numel(), _stream())
+        if ctx.has_res and residual is None and need_res:
+            dres = dz                                # no activation: d residual = dz
+        return dx if need_x else None, dgamma, dbeta, dres, None, None, None, None, None
+
+
+def gn_act(x, gn, residual=None, act=_lib.ACT_RELU, slope=0.0, out=None):
+    """GroupNorm module `gn` (torch.nn.GroupNorm or nn.GroupNorm) applied to x, fused with an optional residual add and an
+    activation (_lib.ACT_*, ACT_SILU included; `slope` for ACT_LEAKYRELU): act(gn(x) + residual).
+
+    x: NCHW-shaped, bf16 or fp32, channels last or a channel window of a wider channels-last
+    tensor (other layouts are converted first); residual: x's shape and dtype.  out: optional channel window (alias_window)
+    to write the result into.  Training and evaluation are the same computation.  A group of one value normalises to zero.
+    Gradients flow to x, the module's weight and bias and the residual, once (no double backward)."""
+    if not 0 <= act <= _lib.ACT_SILU:
+        raise ValueError("gn_act: unknown activation code %r" % (act,))
+    if x.dim() != 4:
+        raise ValueError("gn_act: expected a 4-D NCHW tensor, got shape %s" % (tuple(x.shape),))
+    _require_gpu(x)
+    _dt(x)
+    c = x.shape[1]
+    if c != gn.num_channels:
+        raise RuntimeError("gn_act: %d channels, the GroupNorm has %d" % (c, gn.num_channels))
+    if 0 in x.shape:
+        raise _lib.UResNetHipError("gn_act: non-positive size in shape %s" % (tuple(x.shape),))
+    for name, p in (("weight", gn.weight), ("bias", gn.bias)):
+        if p is not None and (p.dtype != torch.float32 or p.device != x.device or not p.is_contiguous()):
+            raise _lib.UResNetHipError("gn_act: the GroupNorm's %s must be a contiguous fp32 tensor on %s" % (name, x.device))
+    with _on(x.device):
+        x = as_activation(x, x.dtype, allow_window=True)
+        if residual is not None:
+            if residual.shape != x.shape or residual.device != x.device:
+                raise RuntimeError("gn_act: the residual is %s on %s, expected %s on %s"
+                                   % (tuple(residual.shape), residual.device, tuple(x.shape), x.device))
+            residual = as_activation(residual, x.dtype, allow_window=True)
+    return _GNAct.apply(x, gn.weight, gn.bias, residual, gn.num_groups, float(gn.eps), int(act), float(slope),
+                        None if out is None else (out,))
 
 
 fuse_bn_into_conv1x1 = os.environ.get("URESNET_BN_PW", "1") != "0"   # False: BatchNorm+ReLU and the 1x1 convolution stay separate
@@ -1148,6 +1251,8 @@ class _BNReluConv1x1(Function):
 def bn_relu_conv1x1(y, bn, conv, stats=None, out=None):
     """conv(relu(bn(y))) for a BatchNorm2d `bn` and a 1x1 stride-1 Conv2d `conv`, fused as _BNReluConv1x1 where the streaming
     kernels cover the shape in all three directions; None otherwise (the caller then runs the two modules separately)."""
+    if isinstance(bn, torch.nn.GroupNorm):
+        return None
     weight, bias = conv.weight, conv.bias
     if (not (fuse_bn_into_conv1x1 and use_pw_kernel) or not y.is_cuda or y.dim() != 4 or y.dtype != torch.bfloat16
             or not _is_nhwc_dense(y) or y.data_ptr() % 16 or tuple(weight.shape[2:]) != (1, 1) or weight.dtype != torch.float32
@@ -1310,6 +1415,8 @@ fuse_head_bn_apply = os.environ.get("URESNET_HEAD_BN_APPLY", "1") != "0"   # Fal
 
 def bn_relu_conv1x1_pair_supported(n, ca, cb, h, w, dtype, bn, conv):
     """Whether bn_relu_conv1x1_pair covers conv(relu(bn(cat))) for two dense bf16 tensors of ca and cb channels."""
+    if isinstance(bn, torch.nn.GroupNorm):
+        return False
     weight = conv.weight
     c = ca + cb
     if not (fuse_merge_into_head and fuse_bn_into_conv1x1 and use_pw_kernel) or dtype != torch.bfloat16 or ca % 8 or cb % 8:

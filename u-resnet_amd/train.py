@@ -1,12 +1,15 @@
 """Loss, mask and optimiser-step counterparts of the reference's training loops, on HIP kernels.
 
   compute_loss      Segmentation/Cityscapes/train_UResNetAblitionStudy.py:62-68
+  AdamW, clipping   no counterpart (the reference trains with Adam and without clipping)
   Adam / SGD        optim.Adam(lr=1e-4) (same file :203), optim.SGD(lr=0.01) (Classification/CNN-CIFAR10.py:130)
   train steps       train_UResNetAblitionStudy.py:115-122, CNN-CIFAR10.py:145-149, Ice-Seg/TrainingCode.py:107-115
   masks             preds.argmax(1) (train_UResNetAblitionStudy.py:73), sigmoid(outputs) > 0.5 (TrainingCode.py:132)
   metrics           calculate_metrics / validate (train_UResNetAblitionStudy.py:70-100, 128-164)
   checkpoints       the dict written at train_UResNetAblitionStudy.py:244-252 (save_checkpoint / load_checkpoint)
 """
+import ctypes as C
+
 import torch
 
 from . import _lib, ops
@@ -296,12 +299,292 @@ class SGD(_MultiTensorOptimizer):
         return loss
 
 
+class _ParamList:
+    """Tensors of one launch as the C entry points take them (ur_param rows in host memory): built, used and dropped within
+    a call."""
+
+    def __init__(self, rows, device):
+        self.count, self.device = len(rows) // 5, device
+        self._rows = (C.c_longlong * len(rows))(*rows)
+        self.table = torch.empty(_lib.query("ur_param_table_bytes", self.count), dtype=torch.uint8, device=device)
+        self.chunks = C.c_longlong()
+
+    def write(self, steps=None, lr=0.0, betas=(0.0, 0.0)):
+        _lib.call("ur_param_table", self._rows, self.count, self.table.data_ptr(), self.table.numel(), ops._p(steps), lr, betas[0],
+                  betas[1], C.byref(self.chunks), ops._stream())
+
+    def sqnorm(self, parts, at):
+        """Partial sums of the squared gradients into parts[at:]; returns the place behind them."""
+        n = C.c_int()
+        _lib.call("ur_grad_sqnorm", self.table.data_ptr(), self.count, self.chunks.value, parts.data_ptr() + 8 * at, C.byref(n),
+                  ops._stream())
+        return at + n.value
+
+
+def _check_grad(g, device, what):
+    if g.layout is not torch.strided or g.dtype is not torch.float32 or g.device != device or not g.is_cuda:
+        raise _lib.UResNetHipError("%s: gradients must be dense fp32 tensors on one GPU (got %s, %s on %s)"
+                                   % (what, g.layout, g.dtype, g.device))
+
+
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
+    """torch.nn.utils.clip_grad_norm_ for fp32 gradients on one GPU: scales them in place by min(1, max_norm / (norm + 1e-6))
+    and returns their norm before that as a 0-dim device tensor.  No host synchronisation (except with error_if_nonfinite,
+    which raises before anything is scaled), no staging buffers: it can be captured in a graph.  A norm within the limit
+    leaves the gradients untouched.  Only the 2-norm."""
+    if norm_type != 2:
+        raise NotImplementedError("clip_grad_norm_: only norm_type=2 is implemented (got %r)" % (norm_type,))
+    max_norm = float(max_norm)
+    if not max_norm >= 0:
+        raise ValueError("clip_grad_norm_: max_norm must not be negative (got %r)" % (max_norm,))
+    if torch.is_tensor(parameters):
+        parameters = [parameters]
+    grads = [g for g in (p.grad for p in parameters) if g is not None]
+    if not grads:
+        return torch.tensor(0.0)
+    device, rows, seen = grads[0].device, [], set()
+    for g in grads:
+        _check_grad(g, device, "clip_grad_norm_")
+        if not (g.is_contiguous() or g.is_contiguous(memory_format=ops.CL) if g.dim() == 4 else g.is_contiguous()):
+            raise _lib.UResNetHipError("clip_grad_norm_: a gradient of shape %s is not dense" % (tuple(g.shape),))
+        n = g.numel()
+        if n:
+            ptr = g.data_ptr()
+            if ptr in seen:
+                raise ValueError("clip_grad_norm_: a gradient is listed twice")
+            seen.add(ptr)
+            rows += (0, ptr, n, 0, 0)
+    with ops._on(device):
+        if not rows:
+            return torch.zeros((), device=device)
+        norm = torch.empty((), device=device)
+        plist = _ParamList(rows, device)
+        parts = torch.empty(_lib.query("ur_grad_sqnorm_max_parts"), dtype=torch.float64, device=device)
+        plist.write()
+        nparts = plist.sqnorm(parts, 0)
+        if error_if_nonfinite and not bool(torch.isfinite(parts[:nparts].sum().float())):
+            raise RuntimeError("clip_grad_norm_: the total norm of the gradients is not finite")
+        _lib.call("ur_grad_clip", plist.table.data_ptr(), plist.count, plist.chunks.value, parts.data_ptr(), nparts, max_norm,
+                  norm.data_ptr(), ops._stream())
+    return norm
+
+
+class _MomentPool:
+    """The moments of one parameter group in flat buffers: every parameter starts at a multiple of 256 elements (what lies
+    between stays zero), step counts in one int32 array.  state[p] holds views."""
+    BLOCK = 256
+
+    def __init__(self, group, state):
+        self.params, self.bits, self.device = list(group['params']), group['state_bits'], group['params'][0].device
+        self.sizes = [p.numel() for p in self.params]
+        self.blocks, at = [], 0
+        for p, n in zip(self.params, self.sizes):
+            if p.dtype != torch.float32 or not p.is_contiguous() or p.device != self.device:
+                raise _lib.UResNetHipError("AdamW: the parameters of a group must be contiguous fp32 tensors on one device")
+            self.blocks.append(at)
+            at += -(-n // self.BLOCK)
+        self.steps = torch.zeros(len(self.params), dtype=torch.int32, device=self.device)
+        many = at * self.BLOCK
+        if self.bits == 32:
+            self.buffers = {k: torch.zeros(many, device=self.device) for k in ('exp_avg', 'exp_avg_sq')}
+        else:
+            self.buffers = {}
+            for k in ('exp_avg', 'exp_avg_sq_root'):
+                self.buffers[k] = torch.zeros(many, dtype=torch.uint8, device=self.device).view(torch.float8_e4m3fn)
+                self.buffers[k + '_scale'] = torch.zeros(at, device=self.device)
+        for i, p in enumerate(self.params):                    # what the parameters bring along
+            old = state.get(p)
+            if old:
+                new = self.views(i)
+                for k, v in new.items():
+                    v.copy_(torch.as_tensor(old[k]).reshape(v.shape))
+                state[p] = new
+
+    def holds(self, group):
+        ps = group['params']
+        return (len(ps) == len(self.params) and all(a is b for a, b in zip(ps, self.params)) and group['state_bits'] == self.bits
+                and ps[0].device == self.device)
+
+    def views(self, i):
+        b, n, p = self.blocks[i], self.sizes[i], self.params[i]
+        out = {'step': self.steps[i]}
+        for k, buf in self.buffers.items():
+            if k.endswith('_scale'):
+                out[k] = buf[b:b + -(-n // self.BLOCK)]
+            else:
+                out[k] = buf[b * self.BLOCK:b * self.BLOCK + n].view(p.shape)
+        return out
+
+
+class AdamW(torch.optim.Optimizer):
+    """torch.optim.AdamW semantics (decoupled weight decay, no amsgrad) over all tensors of a group in one launch.
+
+    state_bits (also per group): 32, or 8 -- both moments as e4m3 codes with one fp32 scale per 256 elements, 2 bytes per
+    element instead of 8.  The second moment is held by its root and rounded in proportion (in the expectation it follows
+    the recurrence); the same step gives the same bits.  Norm and bias parameters are best left at 32 in a group of their own.
+    max_grad_norm: clip by the global norm of all groups' gradients, as clip_grad_norm_ would before the step, but without
+    writing the gradients; `grad_norm` is the norm before clipping (a 0-dim device tensor; None without clipping).
+    grad_scale multiplies every gradient first, as in the other optimisers here.
+
+    Step counts live on the device and nothing is staged on the host: after one eager step a step can be captured in a graph
+    and replayed (learning rate and the other constants are then those of the capture).  state_dict() has torch.optim.AdamW's
+    layout with 32-bit moments and loads into it; 8-bit moments load into 8-bit groups only.  Checkpoints hold `exp_avg` and
+    `exp_avg_sq_root` as float8_e4m3fn beside their `_scale`s.  An infinite or NaN gradient makes its own element NaN only."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, max_grad_norm=None):
+        self._pools = {}                       # group index -> _MomentPool
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits))
+        if max_grad_norm is not None and not float(max_grad_norm) > 0:
+            raise ValueError("AdamW: max_grad_norm must be positive (got %r)" % (max_grad_norm,))
+        self.max_grad_norm = max_grad_norm
+        self.grad_scale = 1.0
+        self.grad_norm = None
+
+    def add_param_group(self, group):
+        g = {**self.defaults, **group}
+        if g['state_bits'] not in (32, 8):
+            raise ValueError("AdamW: state_bits is 32 or 8 (got %r)" % (g['state_bits'],))
+        if torch.is_tensor(g['lr']):
+            raise TypeError("AdamW: lr is a number, not a tensor")
+        if not (g['lr'] >= 0 and g['eps'] >= 0 and g['weight_decay'] >= 0 and all(0 <= b < 1 for b in g['betas'])):
+            raise ValueError("AdamW: lr, eps and weight_decay must not be negative, betas lie in [0, 1)")
+        super().add_param_group(group)
+
+    def __setstate__(self, state):             # copied or unpickled: the pools are built again from `state`
+        super().__setstate__(state)
+        self._pools = {}
+        for k, v in (('max_grad_norm', None), ('grad_scale', 1.0), ('grad_norm', None)):
+            self.__dict__.setdefault(k, v)
+
+    def __getstate__(self):
+        return {**super().__getstate__(), 'max_grad_norm': self.max_grad_norm, 'grad_scale': self.grad_scale}
+
+    def _pool(self, gi, group):
+        pool = self._pools.get(gi)
+        if pool is None or not pool.holds(group):
+            dev = group['params'][0].device
+            if dev.type == 'cuda' and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("AdamW: run at least one eager step before capturing")
+            pool = self._pools[gi] = _MomentPool(group, self.state)
+        return pool
+
+    def state_buffers(self, group=0):
+        """The moments of a parameter group as flat tensors, parameters in order, each at a multiple of 256 elements (32 bits:
+        exp_avg, exp_avg_sq; 8 bits: exp_avg, exp_avg_sq_root and a scale per 256 elements).  The optimiser's own buffers."""
+        return dict(self._pool(group, self.param_groups[group]).buffers)
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        work = []
+        for gi, group in enumerate(self.param_groups):
+            if not group['params']:
+                continue
+            pool, rows, held = self._pool(gi, group), [], []
+            state, dev = self.state, pool.device
+            for i, p in enumerate(pool.params):
+                g = p.grad
+                if g is None:
+                    continue
+                if g.dtype is not torch.float32 or not g.is_contiguous() or g.is_sparse:
+                    _check_grad(g, dev, "AdamW")
+                    g = g.contiguous()
+                    held.append(g)                             # until the launches that read it are queued
+                if p not in state:
+                    state[p] = pool.views(i)
+                n = pool.sizes[i]
+                if p.numel() != n or p.device != dev or g.numel() != n or not p.is_contiguous():
+                    raise _lib.UResNetHipError("AdamW: a parameter changed its size, layout or device")
+                if n:
+                    rows += (p.data_ptr(), g.data_ptr(), n, pool.blocks[i], i)
+            if rows:
+                if dev.type != 'cuda':
+                    raise _lib.UResNetHipError("AdamW: parameters must be on a GPU (got %s)" % dev)
+                work.append((group, pool, rows, held))
+        if not work:
+            return loss
+        dev = work[0][1].device
+        if any(w[1].device != dev for w in work):
+            raise _lib.UResNetHipError("AdamW: all parameters must be on one GPU")
+        with ops._on(dev):
+            lists = []
+            for group, pool, rows, _ in work:
+                lists.append(_ParamList(rows, dev))
+                lists[-1].write(pool.steps, float(group['lr']), group['betas'])
+            parts, nparts, norm = None, 0, None
+            if self.max_grad_norm is not None:
+                norm = torch.empty((), device=dev)
+                parts = torch.empty(len(lists) * _lib.query("ur_grad_sqnorm_max_parts"), dtype=torch.float64, device=dev)
+                for plist in lists:
+                    nparts = plist.sqnorm(parts, nparts)
+            for (group, pool, _, _), plist in zip(work, lists):
+                names = list(pool.buffers)
+                if pool.bits == 32:
+                    m, v, ms, vs = pool.buffers['exp_avg'], pool.buffers['exp_avg_sq'], None, None
+                else:
+                    m, ms, v, vs = (pool.buffers[k] for k in names)
+                _lib.call("ur_adamw_multi", plist.table.data_ptr(), plist.count, plist.chunks.value, pool.bits, m.data_ptr(), v.data_ptr(),
+                          ops._p(ms), ops._p(vs), float(group['lr']), group['betas'][0], group['betas'][1], group['eps'],
+                          group['weight_decay'], ops._p(parts), nparts, float(self.max_grad_norm or 0.0), float(self.grad_scale),
+                          ops._p(norm), ops._stream())
+            self.grad_norm = norm
+        ops.bump_weights_epoch()
+        return loss
+
+    def state_dict(self):
+        sd = super().state_dict()
+        host = {gi: pool.steps.cpu() for gi, pool in self._pools.items()}          # one device read per group
+        order = [(gi, i) for gi, group in enumerate(self.param_groups) for i in range(len(group['params']))]
+
+        def step_of(k, v):
+            gi, i = order[k]
+            return float(host[gi][i]) if gi in host and self._pools[gi].holds(self.param_groups[gi]) else float(v['step'])
+        sd['state'] = {k: {**v, 'step': torch.tensor(step_of(k, v))} for k, v in sd['state'].items()}
+        for g in sd['param_groups']:                 # torch.optim.AdamW's remaining group keys, at their defaults
+            for k, v in (('amsgrad', False), ('maximize', False), ('foreach', None), ('capturable', False),
+                         ('differentiable', False), ('fused', None), ('decoupled_weight_decay', True)):
+                g.setdefault(k, v)
+        return sd
+
+    def load_state_dict(self, state_dict):
+        groups, saved = self.param_groups, state_dict['param_groups']
+        if [len(g['params']) for g in groups] != [len(g['params']) for g in saved]:
+            raise ValueError("AdamW: the loaded state has other parameter groups")
+        state = {}
+        for group, old in zip(groups, saved):
+            if old.get('amsgrad') or old.get('maximize') or old.get('decoupled_weight_decay') is False:
+                raise NotImplementedError("AdamW: amsgrad, maximize and coupled weight decay states cannot be loaded")
+            bits = old.get('state_bits', group['state_bits'])
+            names = {'exp_avg', 'exp_avg_sq'} if bits == 32 else {'exp_avg', 'exp_avg_scale', 'exp_avg_sq_root', 'exp_avg_sq_root_scale'}
+            for p, k in zip(group['params'], old['params']):
+                entry = state_dict['state'].get(k)
+                if not entry:
+                    continue
+                if not names | {'step'} <= set(entry) or bits != group['state_bits']:
+                    raise ValueError("AdamW: the loaded moments are not %d-bit ones" % group['state_bits'])
+                if entry['exp_avg'].numel() != p.numel():
+                    raise ValueError("AdamW: loaded moments of shape %s for a parameter of shape %s"
+                                     % (tuple(entry['exp_avg'].shape), tuple(p.shape)))
+                state[p] = {**{n: entry[n] for n in names}, 'step': torch.as_tensor(entry['step']).round().to(torch.int32)}
+        for group, old in zip(groups, saved):
+            group.update({k: old[k] for k in ('lr', 'betas', 'eps', 'weight_decay') if k in old})
+        self.state.clear()
+        self.state.update(state)
+        self._pools = {}
+        for gi, group in enumerate(groups):
+            if group['params']:
+                self._pool(gi, group)
+
+
 class GraphedStep:
     """One training step captured as a HIP graph and replayed: for small inputs the step is bound by the few hundred
     host-side launches, not by the GPU (CIFAR-shaped batch: 9 ms eager).  `step_fn(model, optimizer, *inputs)` is one of
     the *_train_step functions; inputs are copied into static buffers before each replay, the returned loss / outputs
-    are static tensors that the next replay overwrites.  Works with this module's SGD and Adam (whose step counts live on
-    the device); shapes are fixed at construction; BatchNorm running statistics and counters advance on the device as in
+    are static tensors that the next replay overwrites.  Works with this module's SGD, Adam and AdamW (whose step counts live
+    on the device); shapes are fixed at construction; BatchNorm running statistics and counters advance on the device as in
     eager mode."""
 
     def __init__(self, step_fn, model, optimizer, *example_inputs, warmup=3):
