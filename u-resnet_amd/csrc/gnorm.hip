@@ -56,7 +56,7 @@ template <int ACT> __device__ __forceinline__ float gn_act(float p, float slope)
     if constexpr (ACT == UR_ACT_LEAKYRELU) return p > 0.f ? p : p * slope;
     if constexpr (ACT == UR_ACT_GELU) return 0.5f * p * (1.f + erff(p * 0.70710678118654752f));
     if constexpr (ACT == UR_ACT_HSWISH) return p <= -3.f ? 0.f : (p >= 3.f ? p : p * (p + 3.f) * (1.f / 6.f));
-    if constexpr (ACT == UR_ACT_SILU) return p / (1.f + __expf(-p));
+    if constexpr (ACT == UR_ACT_SILU) return p * __builtin_amdgcn_rcpf(1.f + __expf(-p));
     return p;
 }
 template <int ACT, typename F> __device__ __forceinline__ float gn_act_grad(F p, float slope) {
@@ -68,7 +68,7 @@ template <int ACT, typename F> __device__ __forceinline__ float gn_act_grad(F p,
     if constexpr (ACT == UR_ACT_GELU)
         return 0.5f * (1.f + erff(q * 0.70710678118654752f)) + q * 0.3989422804014327f * __expf(-0.5f * q * q);
     if constexpr (ACT == UR_ACT_SILU) {
-        const float s = 1.f / (1.f + __expf(-q));
+        const float s = __builtin_amdgcn_rcpf(1.f + __expf(-q));
         return s * (1.f + q * (1.f - s));
     }
     return 1.f;
@@ -91,24 +91,371 @@ struct GnShape {
     int chunks;                   // workgroups over one image's pixels
 };
 
-// A workgroup owns pixels [r0, r1) of image blockIdx.y and the channel vectors of slab blockIdx.z; thread (slot, cg) walks
-// pixels r0 + slot, r0 + slot + slots, ... of one channel vector.
+// A workgroup owns pixels of image blockIdx.y and the channel vectors of slab blockIdx.z; thread (slot, cg) one channel
+// vector.  The workgroups of an image sweep it together: trip t of workgroup b covers the U * slots pixels from
+// (t * chunks + b) * U * slots on, so that the chip reads one moving window per image.
 struct Place {
     int slot, slots, cg, col;
     bool active;
-    long long r0, r1;
     template <int V> __device__ __forceinline__ void set(const GnShape& s) {
         slots = NT / s.cqb;
         slot = threadIdx.x / s.cqb;
         cg = threadIdx.x - slot * s.cqb;
         col = (blockIdx.z * s.cqb + cg) * V;
         active = slot < slots && col < s.c;
-        r0 = s.hw * blockIdx.x / s.chunks;
-        r1 = s.hw * (blockIdx.x + 1) / s.chunks;
+    }
+    // full(r): U pixels r, r + slots, ...; one(r): a single pixel (the end of the image)
+    template <int U, typename Full, typename One>
+    __device__ __forceinline__ void walk(const GnShape& s, const Full& full, const One& one) const {
+        const long long step = (long long)s.chunks * U * slots;
+        for (long long r = (long long)blockIdx.x * U * slots + slot; r < s.hw; r += step) {
+            if (r + (U - 1) * slots < s.hw) full(r);
+            else for (long long q = r; q < s.hw; q += slots) one(q);
+        }
     }
 };
 
-// ------------------------------------------------------------------ forward: sums of one image's groups
+// folds the rows of red[values][slots * cqb] over the slots in halves, always in the same order; result at slot 0
+template <typename F, int N>
+__device__ __forceinline__ void fold_slots(F (*red)[N], int values, int slot, int slots, int cqb) {
+    __syncthreads();
+    for (int n = slots; n > 1;) {
+        const int half = (n + 1) >> 1;
+        if (slot + half < n)
+            for (int i = 0; i < values; ++i) red[i][threadIdx.x] += red[i][threadIdx.x + half * cqb];
+        __syncthreads();
+        n = half;
+    }
+}
+
+__device__ __forceinline__ void mean_rstd(double a, double q, double count, float eps, double& mean, double& rstd) {
+    mean = a / count;
+    double var = q / count - mean * mean;
+    if (var < 0.0) var = 0.0;                              // (a NaN stays one)
+    rstd = 1.0 / sqrt(var + (double)eps);
+}
+
+// the constants of V channels of one image: pre = (x - mean_hi) * a + b.  stats: {mean, rstd} of the groups from g0 on
+template <int V> struct Affine {
+    float m[V], a[V], b[V];
+    __device__ __forceinline__ void load(const double* stats, int g0, const float* __restrict__ gamma, const float* __restrict__ beta,
+                                         int col, int k) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const double* st = stats + ((col + i) / k - g0) * 2;
+            const double ga = gamma ? (double)gamma[col + i] : 1.0, be = beta ? (double)beta[col + i] : 0.0;
+            m[i] = (float)st[0];
+            a[i] = (float)(st[1] * ga);
+            b[i] = (float)(be - (st[0] - (double)m[i]) * (st[1] * ga));
+        }
+    }
+};
+
+template <typename T, int V, int ACT, bool RES>
+__device__ __forceinline__ Chunk<T, V> fwd_vector(const Affine<V>& k, const Chunk<T, V>& v, const Chunk<T, V>& w, float slope) {
+    Chunk<T, V> o;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        float p = fmaf(v.get(i) - k.m[i], k.a[i], k.b[i]);
+        if constexpr (RES) p += w.get(i);
+        o.set(i, gn_act<ACT>(p, slope));
+    }
+    return o;
+}
+
+// g = dy * act'(pre) of a vector, d = x - mean_hi.  One branch per vector decides whether any element lies near a kink.
+template <typename T, int V, int ACT, bool RES>
+__device__ __forceinline__ void bwd_vector(const Affine<V>& k, const Chunk<T, V>& u, const Chunk<T, V>& v, const Chunk<T, V>& w, float slope,
+                                           const double* stats, int g0, const float* __restrict__ gamma, const float* __restrict__ beta,
+                                           int col, int per, float (&g)[V], float (&d)[V]) {
+    bool near = false;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        d[i] = v.get(i) - k.m[i];
+        float p = fmaf(d[i], k.a[i], k.b[i]), size = fabsf(k.b[i]);
+        if constexpr (RES) { p += w.get(i); size += fabsf(w.get(i)); }
+        near |= gn_near_kink<ACT>(p, size);
+        g[i] = u.get(i) * gn_act_grad<ACT, float>(p, slope);
+    }
+    if constexpr (ACT == UR_ACT_RELU || ACT == UR_ACT_LEAKYRELU || ACT == UR_ACT_RELU6 || ACT == UR_ACT_HSWISH) {
+        if (near) {
+#pragma unroll 1
+            for (int i = 0; i < V; ++i) {
+                const double* st = stats + ((col + i) / per - g0) * 2;
+                const double ga = gamma ? (double)gamma[col + i] : 1.0, be = beta ? (double)beta[col + i] : 0.0;
+                float xv = 0.f, uv = 0.f, wv = 0.f;
+#pragma unroll
+                for (int j = 0; j < V; ++j) if (j == i) { xv = v.get(j); uv = u.get(j); if constexpr (RES) wv = w.get(j); }
+                const double e = ((double)xv - st[0]) * st[1] * ga + be + (double)wv;
+                const float r = uv * gn_act_grad<ACT, double>(e, slope);
+#pragma unroll
+                for (int j = 0; j < V; ++j) if (j == i) g[j] = r;
+            }
+        }
+    }
+}
+
+#define GN_ACT(act, ...)                                                              \
+    switch (act) {                                                                    \
+    case UR_ACT_NONE: { constexpr int ACT = UR_ACT_NONE; __VA_ARGS__; } break;         \
+    case UR_ACT_RELU: { constexpr int ACT = UR_ACT_RELU; __VA_ARGS__; } break;         \
+    case UR_ACT_RELU6: { constexpr int ACT = UR_ACT_RELU6; __VA_ARGS__; } break;       \
+    case UR_ACT_LEAKYRELU: { constexpr int ACT = UR_ACT_LEAKYRELU; __VA_ARGS__; } break; \
+    case UR_ACT_GELU: { constexpr int ACT = UR_ACT_GELU; __VA_ARGS__; } break;         \
+    case UR_ACT_HSWISH: { constexpr int ACT = UR_ACT_HSWISH; __VA_ARGS__; } break;     \
+    default: { constexpr int ACT = UR_ACT_SILU; __VA_ARGS__; } break;                  \
+    }
+
+// ================================================================== one workgroup per cell
+// Small and middle sizes: a cell is one image x a slab of channels that holds whole groups, and one workgroup keeps it in
+// registers: one launch, one read, no sums through memory.
+constexpr int CT = 512;                                    // threads per cell
+
+struct Cell {
+    int hw, c, groups, k, slab, slabs;                     // slab: channels per cell (the last one of an image may have fewer)
+};
+
+struct CellPlace {
+    int n, c0, sc, cqs, slot, slots, cg, col;
+    bool active;
+    template <int V> __device__ __forceinline__ void set(const Cell& s) {
+        n = blockIdx.x / s.slabs;
+        c0 = (blockIdx.x - n * s.slabs) * s.slab;
+        sc = min(s.slab, s.c - c0);
+        cqs = sc / V;
+        slots = CT / cqs;
+        slot = threadIdx.x / cqs;
+        cg = threadIdx.x - slot * cqs;
+        col = c0 + cg * V;
+        active = slot < slots;
+    }
+};
+
+template <typename T, int V, int K, bool RES>
+__global__ __launch_bounds__(CT) void gn_fwd_cell_kernel(const T* __restrict__ x, int ld, const T* __restrict__ res, int res_ld,
+                                                         const float* __restrict__ gamma, const float* __restrict__ beta, float eps, int act,
+                                                         float slope, T* __restrict__ y, int y_ld, double* __restrict__ stats, Cell s) {
+    extern __shared__ double cell_lds[];
+    CellPlace at;
+    at.set<V>(s);
+    const size_t row0 = (size_t)at.n * s.hw;
+    Chunk<T, V> v[K];
+    const T* xp = x + row0 * ld + at.col;
+#pragma unroll
+    for (int j = 0; j < K; ++j) {
+        const int r = at.slot + j * at.slots;
+        if (at.active && r < s.hw) v[j].load(xp + (size_t)r * ld);
+    }
+    double a[V], q[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) a[i] = q[i] = 0.0;
+#pragma unroll
+    for (int j = 0; j < K; ++j) {
+        if (at.active && at.slot + j * at.slots < s.hw) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const double f = (double)v[j].get(i);
+                a[i] += f;
+                q[i] = fma(f, f, q[i]);
+            }
+        }
+    }
+    // channels of the vector that share a group are added first: span of them (1, 2, 4 or 8)
+    int span = 1;
+#pragma unroll
+    for (int w = 1; w < V; w *= 2) {
+        if (s.k % (2 * w) == 0) {
+#pragma unroll
+            for (int i = 0; i < V; i += 2 * w) { a[i] += a[i + w]; q[i] += q[i + w]; }
+            span = 2 * w;
+        }
+    }
+    // sums and squares folded together, or one after the other where eight of each per thread would not fit the LDS at once
+    double(*red)[CT] = reinterpret_cast<double(*)[CT]>(cell_lds);
+    const int na = V / span, rows = na > 4 ? na : 2 * na;
+    double* mine = cell_lds + rows * CT;
+    const int gs = at.sc / s.k, g0 = at.c0 / s.k, g = threadIdx.x;         // a slab begins with a group and has at most CT
+    const auto group_sum = [&](int first) {
+        double t = 0.0;
+        if (g < gs)
+            for (int ch = g * s.k; ch < (g + 1) * s.k; ch += span) t += red[first + (ch % V) / span][ch / V];
+        return t;
+    };
+    double sa, sq;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+        if (i % span == 0) {
+            red[i / span][threadIdx.x] = a[i];
+            if (rows > na) red[na + i / span][threadIdx.x] = q[i];
+        }
+    fold_slots(red, rows, at.slot, at.slots, at.cqs);
+    sa = group_sum(0);
+    if (rows > na) sq = group_sum(na);
+    else {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (i % span == 0) red[i / span][threadIdx.x] = q[i];
+        fold_slots(red, rows, at.slot, at.slots, at.cqs);
+        sq = group_sum(0);
+    }
+    if (g < gs) {
+        double mean, rstd;
+        mean_rstd(sa, sq, (double)s.hw * s.k, eps, mean, rstd);
+        mine[2 * g] = mean;
+        mine[2 * g + 1] = rstd;
+        double* st = stats + ((size_t)at.n * s.groups + g0 + g) * 2;
+        st[0] = mean;
+        st[1] = rstd;
+    }
+    __syncthreads();
+    if (!at.active) return;
+    Affine<V> k;
+    k.load(mine, g0, gamma, beta, at.col, s.k);
+    T* yp = y + row0 * y_ld + at.col;
+    const T* rp = RES ? res + row0 * res_ld + at.col : nullptr;
+    GN_ACT(act, {
+_Pragma("unroll")
+        for (int j = 0; j < K; ++j) {
+            const int r = at.slot + j * at.slots;
+            if (r < s.hw) {
+                Chunk<T, V> w;
+                if constexpr (RES) w.load(rp + (size_t)r * res_ld);
+                fwd_vector<T, V, ACT, RES>(k, v[j], w, slope).store(yp + (size_t)r * y_ld);
+            }
+        }
+    });
+}
+
+// sums: {S1, S2} of every image and channel; one image: dgamma and dbeta themselves
+template <typename T, int V, int K, bool RES>
+__global__ __launch_bounds__(CT) void gn_bwd_cell_kernel(const T* __restrict__ dy, int dy_ld, const T* __restrict__ x, int ld,
+                                                         const T* __restrict__ res, int res_ld, const double* __restrict__ stats,
+                                                         const float* __restrict__ gamma, const float* __restrict__ beta, int act, float slope,
+                                                         T* __restrict__ dx, T* __restrict__ dres, double* __restrict__ sums,
+                                                         float* __restrict__ dgamma, float* __restrict__ dbeta, Cell s) {
+    extern __shared__ double cell_lds[];
+    float(*red)[CT] = reinterpret_cast<float(*)[CT]>(cell_lds);           // [2 V][CT] floats, then [sc][2] doubles, [gs][2] floats
+    CellPlace at;
+    at.set<V>(s);
+    const size_t row0 = (size_t)at.n * s.hw;
+    const int g0 = at.c0 / s.k, gs = at.sc / s.k;
+    double* ch_sums = reinterpret_cast<double*>(red + 2 * V);
+    float* coef = reinterpret_cast<float*>(ch_sums + 2 * at.sc);
+    const double* st0 = stats + ((size_t)at.n * s.groups + g0) * 2;
+    Chunk<T, V> u[K], v[K], w;
+    const T* gp = dy + row0 * dy_ld + at.col;
+    const T* xp = x + row0 * ld + at.col;
+    const T* rp = RES ? res + row0 * res_ld + at.col : nullptr;
+#pragma unroll
+    for (int j = 0; j < K; ++j) {
+        const int r = at.slot + j * at.slots;
+        if (at.active && r < s.hw) { u[j].load(gp + (size_t)r * dy_ld); v[j].load(xp + (size_t)r * ld); }
+    }
+    Affine<V> k;
+    if (at.active) k.load(st0, g0, gamma, beta, at.col, s.k);
+    float s1[V], s2[V], g[V], d[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.f;
+    if (at.active) {
+        GN_ACT(act, {
+_Pragma("unroll")
+            for (int j = 0; j < K; ++j) {
+                const int r = at.slot + j * at.slots;
+                if (r < s.hw) {
+                    if constexpr (RES) w.load(rp + (size_t)r * res_ld);
+                    bwd_vector<T, V, ACT, RES>(k, u[j], v[j], w, slope, st0, g0, gamma, beta, at.col, s.k, g, d);
+_Pragma("unroll")
+                    for (int i = 0; i < V; ++i) { s1[i] += g[i]; s2[i] = fmaf(g[i], d[i], s2[i]); }
+                }
+            }
+        });
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) { red[2 * i][threadIdx.x] = s1[i]; red[2 * i + 1][threadIdx.x] = s2[i]; }
+    fold_slots(red, 2 * V, at.slot, at.slots, at.cqs);
+    if (at.slot == 0) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const double* st = st0 + ((at.col + i) / s.k - g0) * 2;
+            const double a = red[2 * i][threadIdx.x], b = red[2 * i + 1][threadIdx.x];
+            const double q = (b - (st[0] - (double)(float)st[0]) * a) * st[1];         // xhat = (x - mean) * rstd
+            const int c = at.col + i;
+            ch_sums[2 * (c - at.c0)] = a;
+            ch_sums[2 * (c - at.c0) + 1] = q;
+            if (sums) {
+                sums[((size_t)at.n * s.c + c) * 2] = a;
+                sums[((size_t)at.n * s.c + c) * 2 + 1] = q;
+            } else {
+                if (dbeta) dbeta[c] = (float)a;
+                if (dgamma) dgamma[c] = (float)q;
+            }
+        }
+    }
+    if (!dx) return;
+    __syncthreads();
+    const double m = (double)s.hw * s.k;
+    for (int h = threadIdx.x; h < gs; h += CT) {
+        double p1 = 0.0, p2 = 0.0;
+        for (int c = h * s.k; c < (h + 1) * s.k; ++c) {
+            const double ga = gamma ? (double)gamma[at.c0 + c] : 1.0;
+            p1 += ga * ch_sums[2 * c];
+            p2 += ga * ch_sums[2 * c + 1];
+        }
+        const double mean = st0[2 * h], rstd = st0[2 * h + 1], lo = mean - (double)(float)mean;
+        coef[2 * h] = (float)(rstd * (lo * rstd * p2 - p1) / m);
+        coef[2 * h + 1] = (float)(-rstd * rstd * p2 / m);
+    }
+    __syncthreads();
+    if (!at.active) return;
+    float k1[V], k2[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) { const int h = (at.col + i) / s.k - g0; k1[i] = coef[2 * h]; k2[i] = coef[2 * h + 1]; }
+    T* op = dx + row0 * s.c + at.col;
+    T* qp = RES && dres ? dres + row0 * s.c + at.col : nullptr;
+    GN_ACT(act, {
+_Pragma("unroll")
+        for (int j = 0; j < K; ++j) {
+            const int r = at.slot + j * at.slots;
+            if (r < s.hw) {
+                Chunk<T, V> o, t;
+                if constexpr (RES) w.load(rp + (size_t)r * res_ld);
+                bwd_vector<T, V, ACT, RES>(k, u[j], v[j], w, slope, st0, g0, gamma, beta, at.col, s.k, g, d);
+_Pragma("unroll")
+                for (int i = 0; i < V; ++i) { o.set(i, fmaf(g[i], k.a[i], fmaf(d[i], k2[i], k1[i]))); t.set(i, g[i]); }
+                o.store(op + (size_t)r * s.c);
+                if constexpr (RES) { if (qp) t.store(qp + (size_t)r * s.c); }
+            }
+        }
+    });
+}
+
+// dgamma, dbeta: {S1, S2} added over the images, 32 channels x 8 image slots per workgroup
+__device__ __forceinline__ void sum_images(const double* __restrict__ sums, int images, int c_all, int block, float* __restrict__ dgamma,
+                                           float* __restrict__ dbeta) {
+    __shared__ double red[8][32][2];
+    const int ch = threadIdx.x & 31, slot = threadIdx.x >> 5, c = block * 32 + ch;
+    double a = 0.0, b = 0.0;
+    if (c < c_all && slot < 8)
+        for (int n = slot; n < images; n += 8) { const double* p = sums + ((size_t)n * c_all + c) * 2; a += p[0]; b += p[1]; }
+    if (slot < 8) { red[slot][ch][0] = a; red[slot][ch][1] = b; }
+    __syncthreads();
+    if (slot == 0 && c < c_all) {
+        for (int j = 1; j < 8; ++j) { a += red[j][ch][0]; b += red[j][ch][1]; }
+        if (dbeta) dbeta[c] = (float)a;
+        if (dgamma) dgamma[c] = (float)b;
+    }
+    __syncthreads();
+}
+__global__ __launch_bounds__(NT) void gn_params_kernel(const double* __restrict__ sums, int images, int c_all, float* __restrict__ dgamma,
+                                                       float* __restrict__ dbeta) {
+    sum_images(sums, images, c_all, blockIdx.x, dgamma, dbeta);
+}
+
+// ================================================================== streaming passes
+// Large sizes: two passes over memory with the sums of all workgroups between them.
+constexpr int UNR = 4, SUNR = 8;                           // pixels in flight per thread; in the statistics
+
 // SPAN: channels of a vector that share a group (a power of two that divides both V and k): V / SPAN pairs of sums per thread
 template <typename T, int V, int SPAN>
 __global__ __launch_bounds__(NT) void gn_stats_kernel(const T* __restrict__ x, int ld, GnShape s, double* __restrict__ partial) {
@@ -121,30 +468,25 @@ __global__ __launch_bounds__(NT) void gn_stats_kernel(const T* __restrict__ x, i
     for (int i = 0; i < NA; ++i) a[i] = q[i] = 0.0;
     if (at.active) {
         const T* p = x + (size_t)blockIdx.y * s.hw * ld + at.col;
-#pragma unroll 4
-        for (long long r = at.r0 + at.slot; r < at.r1; r += at.slots) {
-            Chunk<T, V> v;
-            v.load(p + (size_t)r * ld);
+        const auto add = [&](const Chunk<T, V>& v) {
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 const double f = (double)v.get(i);
                 a[i / SPAN] += f;
                 q[i / SPAN] = fma(f, f, q[i / SPAN]);
             }
-        }
+        };
+        at.walk<SUNR>(s, [&](long long r) {
+            Chunk<T, V> v[SUNR];
+#pragma unroll
+            for (int j = 0; j < SUNR; ++j) v[j].load(p + (size_t)(r + j * at.slots) * ld);
+#pragma unroll
+            for (int j = 0; j < SUNR; ++j) add(v[j]);
+        }, [&](long long r) { Chunk<T, V> v; v.load(p + (size_t)r * ld); add(v); });
     }
 #pragma unroll
     for (int i = 0; i < NA; ++i) { red[2 * i][threadIdx.x] = a[i]; red[2 * i + 1][threadIdx.x] = q[i]; }
-    __syncthreads();
-    for (int n = at.slots; n > 1;) {                     // slots folded in halves, always in the same order
-        const int half = (n + 1) >> 1;
-        if (at.slot + half < n) {
-#pragma unroll
-            for (int i = 0; i < 2 * NA; ++i) red[i][threadIdx.x] += red[i][threadIdx.x + half * s.cqb];
-        }
-        __syncthreads();
-        n = half;
-    }
+    fold_slots(red, 2 * NA, at.slot, at.slots, s.cqb);
     // channels to groups; groups without a channel in this slab get zeros, so that the slabs' rows can simply be added
     double* out = partial + (((size_t)blockIdx.y * s.chunks + blockIdx.x) * gridDim.z + blockIdx.z) * s.groups * 2;
     const int c_lo = blockIdx.z * s.cqb * V, c_hi = min(s.c, c_lo + s.cqb * V);
@@ -170,29 +512,12 @@ __global__ __launch_bounds__(64) void gn_finalize_kernel(const double* __restric
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) { a += __shfl_xor(a, o, 64); q += __shfl_xor(q, o, 64); }
     if (lane == 0) {
-        const double mean = a / count;
-        double var = q / count - mean * mean;
-        if (var < 0.0) var = 0.0;
+        double mean, rstd;
+        mean_rstd(a, q, count, eps, mean, rstd);
         stats[((size_t)n * groups + g) * 2] = mean;
-        stats[((size_t)n * groups + g) * 2 + 1] = 1.0 / sqrt(var + (double)eps);
+        stats[((size_t)n * groups + g) * 2 + 1] = rstd;
     }
 }
-
-// the constants of V channels of one image: pre = (x - mean_hi) * a + b
-template <int V> struct Affine {
-    float m[V], a[V], b[V];
-    __device__ __forceinline__ void load(const double* __restrict__ stats, const float* __restrict__ gamma,
-                                         const float* __restrict__ beta, int n, int col, const GnShape& s) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const double* st = stats + ((size_t)n * s.groups + (col + i) / s.k) * 2;
-            const double ga = gamma ? (double)gamma[col + i] : 1.0, be = beta ? (double)beta[col + i] : 0.0;
-            m[i] = (float)st[0];
-            a[i] = (float)(st[1] * ga);
-            b[i] = (float)(be - (st[0] - (double)m[i]) * (st[1] * ga));
-        }
-    }
-};
 
 template <typename T, int V, int ACT, bool RES>
 __global__ __launch_bounds__(NT) void gn_fwd_kernel(const T* __restrict__ x, int ld, const T* __restrict__ res, int res_ld,
@@ -204,43 +529,25 @@ __global__ __launch_bounds__(NT) void gn_fwd_kernel(const T* __restrict__ x, int
     if (!at.active) return;
     const int n = blockIdx.y;
     Affine<V> k;
-    k.load(stats, gamma, beta, n, at.col, s);
+    k.load(stats + (size_t)n * s.groups * 2, 0, gamma, beta, at.col, s.k);
     const T* xp = x + (size_t)n * s.hw * ld + at.col;
     const T* rp = RES ? res + (size_t)n * s.hw * res_ld + at.col : nullptr;
     T* yp = y + (size_t)n * s.hw * y_ld + at.col;
-#pragma unroll 4
-    for (long long r = at.r0 + at.slot; r < at.r1; r += at.slots) {
-        Chunk<T, V> v, w, o;
+    at.walk<UNR>(s, [&](long long r) {
+        Chunk<T, V> v[UNR], w[UNR];
+#pragma unroll
+        for (int j = 0; j < UNR; ++j) {
+            v[j].load(xp + (size_t)(r + j * at.slots) * ld);
+            if constexpr (RES) w[j].load(rp + (size_t)(r + j * at.slots) * res_ld);
+        }
+#pragma unroll
+        for (int j = 0; j < UNR; ++j) fwd_vector<T, V, ACT, RES>(k, v[j], w[j], slope).store(yp + (size_t)(r + j * at.slots) * y_ld);
+    }, [&](long long r) {
+        Chunk<T, V> v, w;
         v.load(xp + (size_t)r * ld);
         if constexpr (RES) w.load(rp + (size_t)r * res_ld);
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            float p = fmaf(v.get(i) - k.m[i], k.a[i], k.b[i]);
-            if constexpr (RES) p += w.get(i);
-            o.set(i, gn_act<ACT>(p, slope));
-        }
-        o.store(yp + (size_t)r * y_ld);
-    }
-}
-
-// ------------------------------------------------------------------ backward
-// act'(pre) of element i of a vector, with the kinks decided in 64 bits
-template <int V, int ACT, bool RES>
-__device__ __forceinline__ float gn_slope_at(const Affine<V>& k, int i, float xv, float d, float rv, float slope,
-                                             const double* __restrict__ stats, const float* __restrict__ gamma,
-                                             const float* __restrict__ beta, int n, int col, const GnShape& s) {
-    if constexpr (ACT == UR_ACT_NONE) return 1.f;
-    float p = fmaf(d, k.a[i], k.b[i]);
-    float size = fabsf(k.b[i]);
-    if constexpr (RES) { p += rv; size += fabsf(rv); }
-    if (gn_near_kink<ACT>(p, size)) {
-        const double* st = stats + ((size_t)n * s.groups + (col + i) / s.k) * 2;
-        const double ga = gamma ? (double)gamma[col + i] : 1.0, be = beta ? (double)beta[col + i] : 0.0;
-        double e = ((double)xv - st[0]) * st[1] * ga + be;
-        if constexpr (RES) e += (double)rv;
-        return gn_act_grad<ACT, double>(e, slope);
-    }
-    return gn_act_grad<ACT, float>(p, slope);
+        fwd_vector<T, V, ACT, RES>(k, v, w, slope).store(yp + (size_t)r * y_ld);
+    });
 }
 
 // per (image, chunk, channel): {sum g, sum g * (x - mean_hi)}
@@ -253,42 +560,43 @@ __global__ __launch_bounds__(NT) void gn_bwd_reduce_kernel(const T* __restrict__
     Place at;
     at.set<V>(s);
     const int n = blockIdx.y;
+    const double* st0 = stats + (size_t)n * s.groups * 2;
     float s1[V], s2[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.f;
     if (at.active) {
         Affine<V> k;
-        k.load(stats, gamma, beta, n, at.col, s);
+        k.load(st0, 0, gamma, beta, at.col, s.k);
         const T* gp = dy + (size_t)n * s.hw * dy_ld + at.col;
         const T* xp = x + (size_t)n * s.hw * ld + at.col;
         const T* rp = RES ? res + (size_t)n * s.hw * res_ld + at.col : nullptr;
-#pragma unroll 4
-        for (long long r = at.r0 + at.slot; r < at.r1; r += at.slots) {
+        const auto add = [&](const Chunk<T, V>& u, const Chunk<T, V>& v, const Chunk<T, V>& w) {
+            float g[V], d[V];
+            bwd_vector<T, V, ACT, RES>(k, u, v, w, slope, st0, 0, gamma, beta, at.col, s.k, g, d);
+#pragma unroll
+            for (int i = 0; i < V; ++i) { s1[i] += g[i]; s2[i] = fmaf(g[i], d[i], s2[i]); }
+        };
+        at.walk<UNR>(s, [&](long long r) {
+            Chunk<T, V> u[UNR], v[UNR], w[UNR];
+#pragma unroll
+            for (int j = 0; j < UNR; ++j) {
+                u[j].load(gp + (size_t)(r + j * at.slots) * dy_ld);
+                v[j].load(xp + (size_t)(r + j * at.slots) * ld);
+                if constexpr (RES) w[j].load(rp + (size_t)(r + j * at.slots) * res_ld);
+            }
+#pragma unroll
+            for (int j = 0; j < UNR; ++j) add(u[j], v[j], w[j]);
+        }, [&](long long r) {
             Chunk<T, V> u, v, w;
             u.load(gp + (size_t)r * dy_ld);
             v.load(xp + (size_t)r * ld);
             if constexpr (RES) w.load(rp + (size_t)r * res_ld);
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const float xv = v.get(i), d = xv - k.m[i];
-                const float g = u.get(i) * gn_slope_at<V, ACT, RES>(k, i, xv, d, RES ? w.get(i) : 0.f, slope, stats, gamma, beta, n, at.col, s);
-                s1[i] += g;
-                s2[i] = fmaf(g, d, s2[i]);
-            }
-        }
+            add(u, v, w);
+        });
     }
 #pragma unroll
     for (int i = 0; i < V; ++i) { red[2 * i][threadIdx.x] = s1[i]; red[2 * i + 1][threadIdx.x] = s2[i]; }
-    __syncthreads();
-    for (int m = at.slots; m > 1;) {
-        const int half = (m + 1) >> 1;
-        if (at.slot + half < m) {
-#pragma unroll
-            for (int i = 0; i < 2 * V; ++i) red[i][threadIdx.x] += red[i][threadIdx.x + half * s.cqb];
-        }
-        __syncthreads();
-        m = half;
-    }
+    fold_slots(red, 2 * V, at.slot, at.slots, s.cqb);
     if (at.slot == 0 && at.active) {
         float* out = partial + (((size_t)n * s.chunks + blockIdx.x) * s.c + at.col) * 2;
 #pragma unroll
@@ -296,70 +604,74 @@ __global__ __launch_bounds__(NT) void gn_bwd_reduce_kernel(const T* __restrict__
     }
 }
 
-// the chunks of one image added per channel in 64 bits: sums[image][channel] = {S1, S2}
-__global__ __launch_bounds__(NT) void gn_bwd_sums_kernel(const float* __restrict__ partial, const double* __restrict__ stats,
-                                                         GnShape s, double* __restrict__ sums) {
-    __shared__ double red[8][32][2];
-    const int n = blockIdx.y, ch = threadIdx.x & 31, slot = threadIdx.x >> 5, c = blockIdx.x * 32 + ch;
-    double a = 0.0, b = 0.0;
-    if (c < s.c) {
-        const float2* p = reinterpret_cast<const float2*>(partial) + (size_t)n * s.chunks * s.c + c;
-        for (int r = slot; r < s.chunks; r += 8) { const float2 v = p[(size_t)r * s.c]; a += v.x; b += v.y; }
+// The sums of one image's channels and the constants of its groups: a workgroup owns `bundle` groups of image blockIdx.y.
+// sums[image][channel] = {S1, S2};  dx = g * a + d * k2 + k1 with coef[image][group] = {k1, k2}
+constexpr int COEF_WAVES = 16;
+__global__ __launch_bounds__(64 * COEF_WAVES) void gn_bwd_coef_kernel(const float* __restrict__ partial, const double* __restrict__ stats,
+                                                         const float* __restrict__ gamma, GnShape s, int bundle,
+                                                         double* __restrict__ sums, float* __restrict__ coef) {
+    __shared__ double red[COEF_WAVES][64][2];
+    const int n = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int g_lo = blockIdx.x * bundle, g_hi = min(s.groups, g_lo + bundle), c_lo = g_lo * s.k, c_hi = g_hi * s.k;
+    double* mine = sums + (size_t)n * s.c * 2;
+    for (int c0 = c_lo; c0 < c_hi; c0 += 64) {
+        const int c = c0 + lane;
+        double a = 0.0, b = 0.0;
+        if (c < c_hi) {
+            const float2* p = reinterpret_cast<const float2*>(partial) + (size_t)n * s.chunks * s.c + c;
+#pragma unroll 8
+            for (int r = wave; r < s.chunks; r += COEF_WAVES) { const float2 v = p[(size_t)r * s.c]; a += v.x; b += v.y; }
+        }
+        red[wave][lane][0] = a;
+        red[wave][lane][1] = b;
+        __syncthreads();
+        if (wave == 0 && c < c_hi) {
+            for (int j = 1; j < COEF_WAVES; ++j) { a += red[j][lane][0]; b += red[j][lane][1]; }
+            const double* st = stats + ((size_t)n * s.groups + c / s.k) * 2;
+            mine[2 * c] = a;
+            mine[2 * c + 1] = (b - (st[0] - (double)(float)st[0]) * a) * st[1];          // xhat = (x - mean) * rstd
+        }
+        __syncthreads();
     }
-    red[slot][ch][0] = a;
-    red[slot][ch][1] = b;
-    __syncthreads();
-    if (slot || c >= s.c) return;
-    for (int j = 1; j < 8; ++j) { a += red[j][ch][0]; b += red[j][ch][1]; }
-    const double* st = stats + ((size_t)n * s.groups + c / s.k) * 2;
-    sums[((size_t)n * s.c + c) * 2] = a;
-    sums[((size_t)n * s.c + c) * 2 + 1] = (b - (st[0] - (double)(float)st[0]) * a) * st[1];        // xhat = (x - mean) * rstd
-}
-
-// dx = g * a + d * k2 + k1 with the group's k1, k2 (coef[image][group]); workgroups beyond the images: dgamma, dbeta
-__global__ __launch_bounds__(NT) void gn_bwd_coef_kernel(const double* __restrict__ sums, const double* __restrict__ stats,
-                                                         const float* __restrict__ gamma, int images, GnShape s,
-                                                         float* __restrict__ coef, float* __restrict__ dgamma,
-                                                         float* __restrict__ dbeta) {
-    if ((int)blockIdx.x < images) {
-        const int n = blockIdx.x;
-        const double m = (double)s.hw * s.k;
-        for (int g = threadIdx.x; g < s.groups; g += NT) {
-            double p1 = 0.0, p2 = 0.0;
-            for (int c = g * s.k; c < (g + 1) * s.k; ++c) {
-                const double ga = gamma ? (double)gamma[c] : 1.0;
-                p1 += ga * sums[((size_t)n * s.c + c) * 2];
-                p2 += ga * sums[((size_t)n * s.c + c) * 2 + 1];
-            }
-            p1 /= m;
-            p2 /= m;
+    const double m = (double)s.hw * s.k;
+    for (int g = g_lo + wave; g < g_hi; g += COEF_WAVES) {           // a wave per group
+        double p1 = 0.0, p2 = 0.0;
+        for (int c = g * s.k + lane; c < (g + 1) * s.k; c += 64) {
+            const double ga = gamma ? (double)gamma[c] : 1.0;
+            p1 += ga * mine[2 * c];
+            p2 += ga * mine[2 * c + 1];
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) { p1 += __shfl_xor(p1, o, 64); p2 += __shfl_xor(p2, o, 64); }
+        if (lane == 0) {
             const double* st = stats + ((size_t)n * s.groups + g) * 2;
             const double lo = st[0] - (double)(float)st[0];
-            coef[((size_t)n * s.groups + g) * 2] = (float)(st[1] * (lo * st[1] * p2 - p1));
-            coef[((size_t)n * s.groups + g) * 2 + 1] = (float)(-st[1] * st[1] * p2);
+            coef[((size_t)n * s.groups + g) * 2] = (float)(st[1] * (lo * st[1] * p2 - p1) / m);
+            coef[((size_t)n * s.groups + g) * 2 + 1] = (float)(-st[1] * st[1] * p2 / m);
         }
-        return;
     }
-    const int c = (blockIdx.x - images) * NT + threadIdx.x;
-    if (c >= s.c) return;
-    double a = 0.0, b = 0.0;
-    for (int n = 0; n < images; ++n) { a += sums[((size_t)n * s.c + c) * 2]; b += sums[((size_t)n * s.c + c) * 2 + 1]; }
-    if (dbeta) dbeta[c] = (float)a;
-    if (dgamma) dgamma[c] = (float)b;
 }
 
+// image row gridDim.y - 1 of the grid adds the images' sums to dgamma and dbeta instead
 template <typename T, int V, int ACT, bool RES>
 __global__ __launch_bounds__(NT) void gn_bwd_apply_kernel(const T* __restrict__ dy, int dy_ld, const T* __restrict__ x, int ld,
                                                           const T* __restrict__ res, int res_ld, const double* __restrict__ stats,
                                                           const float* __restrict__ gamma, const float* __restrict__ beta,
                                                           const float* __restrict__ coef, float slope, T* __restrict__ dx,
-                                                          T* __restrict__ dres, GnShape s) {
+                                                          T* __restrict__ dres, const double* __restrict__ sums, float* __restrict__ dgamma,
+                                                          float* __restrict__ dbeta, GnShape s) {
+    const int n = blockIdx.y;
+    if (n == (int)gridDim.y - 1) {
+        if (blockIdx.z == 0)
+            for (int b = blockIdx.x; b * 32 < s.c; b += gridDim.x) sum_images(sums, n, s.c, b, dgamma, dbeta);
+        return;
+    }
     Place at;
     at.set<V>(s);
     if (!at.active) return;
-    const int n = blockIdx.y;
+    const double* st0 = stats + (size_t)n * s.groups * 2;
     Affine<V> k;
-    k.load(stats, gamma, beta, n, at.col, s);
+    k.load(st0, 0, gamma, beta, at.col, s.k);
     float k1[V], k2[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -371,23 +683,33 @@ __global__ __launch_bounds__(NT) void gn_bwd_apply_kernel(const T* __restrict__ 
     const T* xp = x + (size_t)n * s.hw * ld + at.col;
     const T* rp = RES ? res + (size_t)n * s.hw * res_ld + at.col : nullptr;
     T* op = dx + (size_t)n * s.hw * s.c + at.col;
-    T* qp = dres ? dres + (size_t)n * s.hw * s.c + at.col : nullptr;
-#pragma unroll 4
-    for (long long r = at.r0 + at.slot; r < at.r1; r += at.slots) {
-        Chunk<T, V> u, v, w, o, t;
+    T* qp = RES && dres ? dres + (size_t)n * s.hw * s.c + at.col : nullptr;
+    const auto one = [&](const Chunk<T, V>& u, const Chunk<T, V>& v, const Chunk<T, V>& w, long long row) {
+        float g[V], d[V];
+        bwd_vector<T, V, ACT, RES>(k, u, v, w, slope, st0, 0, gamma, beta, at.col, s.k, g, d);
+        Chunk<T, V> o, t;
+#pragma unroll
+        for (int i = 0; i < V; ++i) { o.set(i, fmaf(g[i], k.a[i], fmaf(d[i], k2[i], k1[i]))); t.set(i, g[i]); }
+        o.store(op + (size_t)row * s.c);
+        if constexpr (RES) { if (qp) t.store(qp + (size_t)row * s.c); }
+    };
+    at.walk<UNR>(s, [&](long long r) {
+        Chunk<T, V> u[UNR], v[UNR], w[UNR];
+#pragma unroll
+        for (int j = 0; j < UNR; ++j) {
+            u[j].load(gp + (size_t)(r + j * at.slots) * dy_ld);
+            v[j].load(xp + (size_t)(r + j * at.slots) * ld);
+            if constexpr (RES) w[j].load(rp + (size_t)(r + j * at.slots) * res_ld);
+        }
+#pragma unroll
+        for (int j = 0; j < UNR; ++j) one(u[j], v[j], w[j], r + j * at.slots);
+    }, [&](long long r) {
+        Chunk<T, V> u, v, w;
         u.load(gp + (size_t)r * dy_ld);
         v.load(xp + (size_t)r * ld);
         if constexpr (RES) w.load(rp + (size_t)r * res_ld);
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const float xv = v.get(i), d = xv - k.m[i];
-            const float g = u.get(i) * gn_slope_at<V, ACT, RES>(k, i, xv, d, RES ? w.get(i) : 0.f, slope, stats, gamma, beta, n, at.col, s);
-            o.set(i, fmaf(g, k.a[i], fmaf(d, k2[i], k1[i])));
-            if constexpr (RES) t.set(i, g);
-        }
-        o.store(op + (size_t)r * s.c);
-        if constexpr (RES) { if (qp) t.store(qp + (size_t)r * s.c); }
-    }
+        one(u, v, w, r);
+    });
 }
 
 // ------------------------------------------------------------------ host
@@ -407,12 +729,44 @@ Plan make_plan(int dtype, int n, long long hw, int c, int groups, bool vec) {
     p.s.cqb = cq < NT ? cq : NT;
     p.zs = (cq + p.s.cqb - 1) / p.s.cqb;
     const int slots = NT / p.s.cqb;
-    // about four workgroups per CU, each with at least four pixels per slot
-    long long chunks = 1024 / ((long long)n * p.zs), most = (hw + 4LL * slots - 1) / (4LL * slots);
-    if (chunks > most) chunks = most;
+    // Eight workgroups per CU where each still makes three trips (6x64x512x1024 bf16, forward + backward: 663 us at two per
+    // CU, 632 at four, 606 at eight; 6x512x64x128: 174, 172 and, with one and a half trips, 185), trips spread evenly.
+    const long long trips = (hw + (long long)UNR * slots - 1) / ((long long)UNR * slots);
+    long long chunks = 2048 / ((long long)n * p.zs);
+    if (chunks > trips / 3) chunks = trips / 3;
+    if (chunks < 1) chunks = 1;
+    const long long each = (trips + chunks - 1) / chunks;
+    chunks = (trips + each - 1) / each;
     p.s.chunks = chunks < 1 ? 1 : (int)chunks;
     return p;
 }
+
+// The cell kernels' split, or slabs = 0 where a cell of whole groups does not fit `most` vectors per thread.  Slabs are as
+// narrow as 128 bytes (one memory line) if there would be fewer than 256 cells otherwise, or 64 where only that fits.
+Cell make_cell(int dtype, int n, long long hw, int c, int groups, bool vec, int most) {
+    Cell s = {(int)hw, c, groups, c / groups, 0, 0};
+    if (!vec || hw > 64 * CT) return s;
+    const int v = dtype == UR_BF16 ? 8 : 4, esz = dtype == UR_BF16 ? 2 : 4;
+    int base = s.k;
+    while (base % v) base += s.k;                          // whole groups and whole vectors; divides c
+    if (base / v > CT) return s;
+    const int units = c / base;
+    const auto fits = [&](int m) {
+        const int cqs = m * base / v;
+        return (cqs <= 64 || m == 1) && (hw + CT / cqs - 1) / (CT / cqs) <= most;
+    };
+    int m = units;
+    while (m > 1 && (!fits(m) || (long long)n * ((units + m - 1) / m) < 256)) {
+        if (fits(m) && (m - 1) * base * esz < 128) break;
+        --m;
+    }
+    if (!fits(m) || (m * base * esz < 64 && m < units)) return s;
+    if ((long long)n * ((units + m - 1) / m) > 0x7fffffffLL) return s;
+    s.slab = m * base;
+    s.slabs = (units + m - 1) / m;
+    return s;
+}
+int cell_vectors(const Cell& s, int v) { const int slots = CT / (s.slab / v); return (s.hw + slots - 1) / slots; }
 
 bool aligned(const void* p, int dtype, long long ld) { return p == nullptr || ((((uintptr_t)p) & 15) == 0 && ld % (dtype == UR_BF16 ? 8 : 4) == 0); }
 
@@ -429,16 +783,6 @@ void launch_stats(const void* x, int ld, const Plan& p, int n, double* partial, 
     hipLaunchKernelGGL((gn_stats_kernel<T, V, 1>), grid, dim3(NT), 0, st, (const T*)x, ld, p.s, partial);
 }
 
-#define GN_ACT(act, ...)                                                              \
-    switch (act) {                                                                    \
-    case UR_ACT_NONE: { constexpr int ACT = UR_ACT_NONE; __VA_ARGS__; } break;         \
-    case UR_ACT_RELU: { constexpr int ACT = UR_ACT_RELU; __VA_ARGS__; } break;         \
-    case UR_ACT_RELU6: { constexpr int ACT = UR_ACT_RELU6; __VA_ARGS__; } break;       \
-    case UR_ACT_LEAKYRELU: { constexpr int ACT = UR_ACT_LEAKYRELU; __VA_ARGS__; } break; \
-    case UR_ACT_GELU: { constexpr int ACT = UR_ACT_GELU; __VA_ARGS__; } break;         \
-    case UR_ACT_HSWISH: { constexpr int ACT = UR_ACT_HSWISH; __VA_ARGS__; } break;     \
-    default: { constexpr int ACT = UR_ACT_SILU; __VA_ARGS__; } break;                  \
-    }
 #define GN_TYPE(dtype, v, ...)                                                                                   \
     do {                                                                                                         \
         if ((dtype) == UR_BF16 && (v) == 8) { typedef bf16_t T; constexpr int V = 8; __VA_ARGS__; }               \
@@ -446,19 +790,37 @@ void launch_stats(const void* x, int ld, const Plan& p, int n, double* partial, 
         else if ((v) == 4) { typedef float T; constexpr int V = 4; __VA_ARGS__; }                                 \
         else { typedef float T; constexpr int V = 1; __VA_ARGS__; }                                               \
     } while (0)
+#define GN_VEC_TYPE(dtype, ...)                                                                                   \
+    do {                                                                                                          \
+        if ((dtype) == UR_BF16) { typedef bf16_t T; constexpr int V = 8; __VA_ARGS__; }                            \
+        else { typedef float T; constexpr int V = 4; __VA_ARGS__; }                                                \
+    } while (0)
+// vectors per thread of a cell, rounded up to a built size
+#define GN_K2(k, ...)                                                                     \
+    do {                                                                                  \
+        if ((k) <= 2) { constexpr int K = 2; __VA_ARGS__; }                                \
+        else { constexpr int K = 8; __VA_ARGS__; }                                         \
+    } while (0)
+#define GN_K3(k, ...)                                                                     \
+    do {                                                                                  \
+        if ((k) <= 2) { constexpr int K = 2; __VA_ARGS__; }                                \
+        else if ((k) <= 8) { constexpr int K = 8; __VA_ARGS__; }                           \
+        else { constexpr int K = 16; __VA_ARGS__; }                                        \
+    } while (0)
+constexpr int FWD_MOST = 16, BWD_MOST = 8;
 
 int check(const char* what, int dtype, int n, long long hw, int c, int groups, int act) {
     UR_REQUIRE(dtype == UR_F32 || dtype == UR_BF16, "%s: bad dtype %d", what, dtype);
     UR_REQUIRE(n > 0 && hw > 0 && c > 0 && groups > 0, "%s: non-positive sizes (n %d, pixels %lld, channels %d, groups %d)", what, n, hw, c, groups);
     UR_REQUIRE(c % groups == 0, "%s: %d channels are not divisible by %d groups", what, c, groups);
-    UR_REQUIRE(n <= 65535 && hw <= (1LL << 40) && c <= (1 << 20), "%s: sizes beyond the limits (65535 images, 2^40 pixels, 2^20 channels)", what);
+    UR_REQUIRE(n < 65535 && hw <= (1LL << 40) && c <= (1 << 20), "%s: sizes beyond the limits (65534 images, 2^40 pixels, 2^20 channels)", what);
     UR_REQUIRE(act >= UR_ACT_NONE && act <= UR_ACT_SILU, "%s: bad activation %d", what, act);
     return UR_OK;
 }
 
-// the larger of what the vector and the element-wise plan need: the caller need not know which one a call takes
+// the largest of what the variants need: the caller need not know which one a call takes
 size_t fwd_bytes(int dtype, int n, long long hw, int c, int groups) {
-    size_t most = 0;
+    size_t most = 16;
     for (int vec = 0; vec < 2; ++vec) {
         if (vec && c % (dtype == UR_BF16 ? 8 : 4)) continue;
         const Plan p = make_plan(dtype, n, hw, c, groups, vec);
@@ -467,6 +829,7 @@ size_t fwd_bytes(int dtype, int n, long long hw, int c, int groups) {
     }
     return most;
 }
+size_t bwd_sums_bytes(int n, int c) { return (size_t)n * c * 2 * sizeof(double); }
 size_t bwd_bytes(int dtype, int n, long long hw, int c, int groups) {
     size_t most = 0;
     for (int vec = 0; vec < 2; ++vec) {
@@ -475,8 +838,7 @@ size_t bwd_bytes(int dtype, int n, long long hw, int c, int groups) {
         const size_t b = (size_t)n * p.s.chunks * c * 2 * sizeof(float);
         if (b > most) most = b;
     }
-    most = (most + 15) / 16 * 16;
-    return most + (size_t)n * c * 2 * sizeof(double) + (size_t)n * groups * 2 * sizeof(float);
+    return bwd_sums_bytes(n, c) + most + (size_t)n * groups * 2 * sizeof(float);
 }
 
 }  // namespace
@@ -502,6 +864,20 @@ int ur_gn_act_fwd(const void* x, int x_ld, const void* residual, int res_ld, con
     UR_REQUIRE(ws_bytes >= fwd_bytes(dtype, n, hw, c, groups), "gn_act_fwd: workspace too small");
     hipStream_t st = (hipStream_t)s;
     const bool vec = c % (dtype == UR_BF16 ? 8 : 4) == 0 && aligned(x, dtype, x_ld) && aligned(residual, dtype, res_ld) && aligned(y, dtype, y_ld);
+    const Cell cell = make_cell(dtype, n, hw, c, groups, vec, FWD_MOST);
+    if (cell.slabs) {
+        GN_VEC_TYPE(dtype, {
+            const int span = cell.k % V == 0 ? V : cell.k % 4 == 0 ? 4 : cell.k % 2 == 0 ? 2 : 1;
+            const int na = V / span;
+            const size_t lds = sizeof(double) * ((na > 4 ? na : 2 * na) * CT + 2 * (cell.slab / cell.k));
+            const dim3 grid(n * cell.slabs);
+            GN_K3(cell_vectors(cell, V), {
+                if (residual) hipLaunchKernelGGL((gn_fwd_cell_kernel<T, V, K, true>), grid, dim3(CT), lds, st, (const T*)x, x_ld, (const T*)residual, res_ld, gamma, beta, eps, act, slope, (T*)y, y_ld, stats, cell);
+                else hipLaunchKernelGGL((gn_fwd_cell_kernel<T, V, K, false>), grid, dim3(CT), lds, st, (const T*)x, x_ld, (const T*)nullptr, 0, gamma, beta, eps, act, slope, (T*)y, y_ld, stats, cell);
+            });
+        });
+        return ur_check_launch("gn_act_fwd");
+    }
     const Plan p = make_plan(dtype, n, hw, c, groups, vec);
     double* partial = (double*)workspace;
     const dim3 grid(p.s.chunks, n, p.zs);
@@ -529,22 +905,39 @@ int ur_gn_act_bwd(const void* dy, int dy_ld, const void* x, int x_ld, const void
     hipStream_t st = (hipStream_t)s;
     const bool vec = c % (dtype == UR_BF16 ? 8 : 4) == 0 && aligned(x, dtype, x_ld) && aligned(dy, dtype, dy_ld)
                      && aligned(residual, dtype, res_ld) && aligned(dx, dtype, c) && aligned(dres, dtype, c);
+    double* sums = (double*)workspace;
+    const Cell cell = make_cell(dtype, n, hw, c, groups, vec, BWD_MOST);
+    if (cell.slabs) {
+        GN_VEC_TYPE(dtype, {
+            const size_t lds = sizeof(float) * 2 * V * CT + sizeof(double) * 2 * cell.slab + sizeof(float) * 2 * (cell.slab / cell.k);
+            const dim3 grid(n * cell.slabs);
+            double* to = n > 1 ? sums : nullptr;
+            GN_K2(cell_vectors(cell, V), {
+                if (residual) hipLaunchKernelGGL((gn_bwd_cell_kernel<T, V, K, true>), grid, dim3(CT), lds, st, (const T*)dy, dy_ld, (const T*)x, x_ld, (const T*)residual, res_ld, stats, gamma, beta, act, slope, (T*)dx, (T*)dres, to, dgamma, dbeta, cell);
+                else hipLaunchKernelGGL((gn_bwd_cell_kernel<T, V, K, false>), grid, dim3(CT), lds, st, (const T*)dy, dy_ld, (const T*)x, x_ld, (const T*)nullptr, 0, stats, gamma, beta, act, slope, (T*)dx, (T*)nullptr, to, dgamma, dbeta, cell);
+            });
+        });
+        if (n > 1 && (dgamma || dbeta)) hipLaunchKernelGGL(gn_params_kernel, dim3(ur_cdiv(c, 32)), dim3(NT), 0, st, sums, n, c, dgamma, dbeta);
+        return ur_check_launch("gn_act_bwd");
+    }
     const Plan p = make_plan(dtype, n, hw, c, groups, vec);
-    float* partial = (float*)workspace;
-    double* sums = (double*)((char*)workspace + ((size_t)n * p.s.chunks * c * 2 * sizeof(float) + 15) / 16 * 16);
-    float* coef = (float*)(sums + (size_t)n * c * 2);
+    float* partial = (float*)(sums + (size_t)n * c * 2);
+    float* coef = partial + (size_t)n * p.s.chunks * c * 2;
     const dim3 grid(p.s.chunks, n, p.zs);
     GN_TYPE(dtype, p.v, GN_ACT(act, {
         if (residual) hipLaunchKernelGGL((gn_bwd_reduce_kernel<T, V, ACT, true>), grid, dim3(NT), 0, st, (const T*)dy, dy_ld, (const T*)x, x_ld, (const T*)residual, res_ld, stats, gamma, beta, slope, p.s, partial);
         else hipLaunchKernelGGL((gn_bwd_reduce_kernel<T, V, ACT, false>), grid, dim3(NT), 0, st, (const T*)dy, dy_ld, (const T*)x, x_ld, (const T*)nullptr, 0, stats, gamma, beta, slope, p.s, partial);
     }));
-    hipLaunchKernelGGL(gn_bwd_sums_kernel, dim3(ur_cdiv(c, 32), n), dim3(NT), 0, st, partial, stats, p.s, sums);
-    hipLaunchKernelGGL(gn_bwd_coef_kernel, dim3(n + ur_cdiv(c, NT)), dim3(NT), 0, st, sums, stats, gamma, n, p.s, coef, dgamma, dbeta);
+    const int bundle = p.s.k >= 32 ? 1 : 32 / p.s.k;
+    hipLaunchKernelGGL(gn_bwd_coef_kernel, dim3(ur_cdiv(groups, bundle), n), dim3(64 * COEF_WAVES), 0, st, partial, stats, gamma, p.s, bundle, sums, coef);
     if (dx) {
+        const dim3 grid2(p.s.chunks, n + 1, p.zs);
         GN_TYPE(dtype, p.v, GN_ACT(act, {
-            if (residual) hipLaunchKernelGGL((gn_bwd_apply_kernel<T, V, ACT, true>), grid, dim3(NT), 0, st, (const T*)dy, dy_ld, (const T*)x, x_ld, (const T*)residual, res_ld, stats, gamma, beta, coef, slope, (T*)dx, (T*)dres, p.s);
-            else hipLaunchKernelGGL((gn_bwd_apply_kernel<T, V, ACT, false>), grid, dim3(NT), 0, st, (const T*)dy, dy_ld, (const T*)x, x_ld, (const T*)nullptr, 0, stats, gamma, beta, coef, slope, (T*)dx, (T*)nullptr, p.s);
+            if (residual) hipLaunchKernelGGL((gn_bwd_apply_kernel<T, V, ACT, true>), grid2, dim3(NT), 0, st, (const T*)dy, dy_ld, (const T*)x, x_ld, (const T*)residual, res_ld, stats, gamma, beta, coef, slope, (T*)dx, (T*)dres, sums, dgamma, dbeta, p.s);
+            else hipLaunchKernelGGL((gn_bwd_apply_kernel<T, V, ACT, false>), grid2, dim3(NT), 0, st, (const T*)dy, dy_ld, (const T*)x, x_ld, (const T*)nullptr, 0, stats, gamma, beta, coef, slope, (T*)dx, (T*)nullptr, sums, dgamma, dbeta, p.s);
         }));
+    } else if (dgamma || dbeta) {
+        hipLaunchKernelGGL(gn_params_kernel, dim3(ur_cdiv(c, 32)), dim3(NT), 0, st, sums, n, c, dgamma, dbeta);
     }
     return ur_check_launch("gn_act_bwd");
 }

@@ -1029,6 +1029,15 @@ def bn_act(y, bn, residual=None, stats=None, act=_lib.ACT_RELU, out=None, pool=F
     return z
 
 
+def _gn_call(name, dev, tag, nbytes, *args):
+    """One GroupNorm entry point on `dev` and its current stream (appended to args)."""
+    if kernel_timings is None and dev.index == torch.cuda.current_device():
+        call(name, *args, torch._C._cuda_getCurrentRawStream(dev.index))
+    else:
+        with _on(dev), _Timed(tag, nbytes):
+            call(name, *args, _stream())
+
+
 class _GNAct(Function):
     """act(GroupNorm(x) (+ residual)).  Saved: x, the residual (its activation's derivative needs the sum) and the fp64
     {mean, rstd} of every image and group; the pre-activation is recomputed from them in backward."""
@@ -1036,7 +1045,8 @@ class _GNAct(Function):
     @staticmethod
     def forward(ctx, x, gamma, beta, residual, groups, eps, act, slope, out):
         n, c, h, w = x.shape
-        dev = x.device
+        dev, dt = x.device, _DT[x.dtype]
+        x_ld, r_ld = _pitch(x), 0 if residual is None else _pitch(residual)
         if out is None:
             z, z_ld = empty_nhwc(n, c, h, w, x.dtype, dev), c
         else:                                        # (window,): a channel window of a wider tensor (alias_window)
@@ -1045,40 +1055,39 @@ class _GNAct(Function):
             if tuple(z.shape) != tuple(x.shape) or z.dtype != x.dtype or z.device != dev or not z_ld:
                 raise RuntimeError("gn_act: `out` must be a channel window with x's shape, dtype and device")
         stats = torch.empty((n, groups, 2), dtype=torch.float64, device=dev)
-        tb = x.numel() * x.element_size()
-        with _on(dev), _Timed("hbm:gn_fwd", tb * (3 if residual is not None else 2)):
-            ws = _workspace(query("ur_gn_fwd_workspace", _dt(x), n, h * w, c, groups), dev)
-            call("ur_gn_act_fwd", x.data_ptr(), _pitch(x), _p(residual), 0 if residual is None else _pitch(residual), _p(gamma),
-                 _p(beta), z.data_ptr(), z_ld, stats.data_ptr(), _dt(x), n, h * w, c, groups, eps, act, slope, ws.data_ptr(),
-                 ws.numel(), _stream())
+        ws_bytes = query("ur_gn_fwd_workspace", dt, n, h * w, c, groups)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        _gn_call("ur_gn_act_fwd", dev, "hbm:gn_fwd", x.numel() * x.element_size() * (3 if residual is not None else 2), x.data_ptr(), x_ld,
+                 _p(residual), r_ld, _p(gamma), _p(beta), z.data_ptr(), z_ld, stats.data_ptr(), dt, n, h * w, c, groups, eps, act, slope,
+                 ws.data_ptr(), ws_bytes)
         # without an activation the residual's gradient is dz itself and nothing depends on the residual's values
         ctx.save_for_backward(x, gamma, beta, residual if act != _lib.ACT_NONE else None, stats)
-        ctx.groups, ctx.act, ctx.slope, ctx.has_res = groups, act, slope, residual is not None
+        ctx.args = (x_ld, r_ld, dt, n, h * w, c, groups, act, slope)
+        ctx.has_res = residual is not None
         return z
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dz):
         x, gamma, beta, residual, stats = ctx.saved_tensors
+        x_ld, r_ld, dt, n, hw, c, groups, act, slope = ctx.args
         need_x, need_gamma, need_beta, need_res = ctx.needs_input_grad[:4]
-        n, c, h, w = x.shape
+        if residual is None and not (need_x or need_gamma or need_beta):
+            return None, None, None, dz, None, None, None, None, None
         dev = x.device
         dz_ld = _pitch(dz) if dz.dtype == x.dtype else 0
         if not dz_ld:
             dz, dz_ld = (_g(dz) if dz.dtype == x.dtype else to_nhwc_raw(dz, x.dtype)), c
-        if residual is None and not (need_x or need_gamma or need_beta):
-            return None, None, None, (dz if need_res else None), None, None, None, None, None
         need_dres = residual is not None and need_res
-        dx = empty_nhwc(n, c, h, w, x.dtype, dev) if (need_x or need_dres) else None
-        dres = empty_nhwc(n, c, h, w, x.dtype, dev) if need_dres else None
+        dx = torch.empty_like(x, memory_format=CL) if (need_x or need_dres) else None
+        dres = torch.empty_like(x, memory_format=CL) if need_dres else None
         dgamma = grad_buffer(gamma) if need_gamma else None
         dbeta = grad_buffer(beta) if need_beta else None
-        tb = x.numel() * x.element_size()
-        with _on(dev), _Timed("hbm:gn_bwd", tb * (2 + (dx is not None) + (residual is not None) + need_dres)):
-            ws = _workspace(query("ur_gn_bwd_workspace", _dt(x), n, h * w, c, ctx.groups), dev)
-            call("ur_gn_act_bwd", dz.data_ptr(), dz_ld, x.data_ptr(), _pitch(x), _p(residual),
-                 0 if residual is None else _pitch(residual), _p(gamma), _p(beta), stats.data_ptr(), _p(dx), _p(dres), _p(dgamma),
-                 _p(dbeta), _dt(x), n, h * w, c, ctx.groups, ctx.act, ctx.slope, ws.data_ptr(), ws.numel(), _stream())
+        ws_bytes = query("ur_gn_bwd_workspace", dt, n, hw, c, groups)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        _gn_call("ur_gn_act_bwd", dev, "hbm:gn_bwd", x.numel() * x.element_size() * (2 + (dx is not None) + (residual is not None) + need_dres),
+                 dz.data_ptr(), dz_ld, x.data_ptr(), x_ld, _p(residual), r_ld, _p(gamma), _p(beta), stats.data_ptr(), _p(dx), _p(dres),
+                 _p(dgamma), _p(dbeta), dt, n, hw, c, groups, act, slope, ws.data_ptr(), ws_bytes)
         if ctx.has_res and residual is None and need_res:
             dres = dz                                # no activation: d residual = dz
         return dx if need_x else None, dgamma, dbeta, dres, None, None, None, None, None
@@ -1107,7 +1116,8 @@ def gn_act(x, gn, residual=None, act=_lib.ACT_RELU, slope=0.0, out=None):
         if p is not None and (p.dtype != torch.float32 or p.device != x.device or not p.is_contiguous()):
             raise _lib.UResNetHipError("gn_act: the GroupNorm's %s must be a contiguous fp32 tensor on %s" % (name, x.device))
     with _on(x.device):
-        x = as_activation(x, x.dtype, allow_window=True)
+        if not _pitch(x):
+            x = as_activation(x, x.dtype, allow_window=True)
         if residual is not None:
             if residual.shape != x.shape or residual.device != x.device:
                 raise RuntimeError("gn_act: the residual is %s on %s, expected %s on %s"
