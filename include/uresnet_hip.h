@@ -486,26 +486,23 @@ int ur_sgd_multi(const void* const* ptrs, const long long* sizes, int ntensors, 
  * with Adam and without clipping.  The tensors are listed in HOST memory and travel as kernel arguments: no staging
  * buffer, every call can be captured in a graph.
  *   1. ur_param_table writes the list as a table in device memory (ur_param_table_bytes), counts the chunks of work into
- *      *nchunks (host) and, where `steps` (int32 counts in device memory) is given, adds 1 to steps[slot] of every tensor
- *      and stores the bias corrections of the new count.  Every slot at most once per call.
+ *      *nchunks (host) and, where `steps` (device memory, one int32 count per tensor) is given, adds 1 to the count of every
+ *      tensor with a gradient and stores the bias corrections of the new count.
+ *      params, grads, sizes: host arrays of addresses and element counts (params may be NULL where no step follows); a zero
+ *      gradient skips the tensor.  blocks: device array, each tensor's first block of 256 elements in the state buffers (may
+ *      be NULL where no step follows).
  *   2. ur_grad_sqnorm (optional) writes *nparts (host; at most ur_grad_sqnorm_max_parts()) partial sums of the squared
  *      gradients.  Several lists (parameter groups) can share one norm: give each its place in one array.
  *   3. ur_adamw_multi makes the step.  nparts > 0: gradients are scaled by min(1, max_norm / (norm + 1e-6)), norm over all
  *      `nparts` sums, and out_norm (may be NULL) gets the norm before clipping.  grad_scale multiplies every gradient first.
- *      Moments lie in buffers of blocks of 256 elements, a tensor's first one at `block`: state_bits 32: fp32;
- *      8: e4m3 codes of m and of sqrt(v) and an fp32 scale per block.
+ *      Moments lie in buffers of blocks of 256 elements: state_bits 32: fp32; 8: e4m3 codes of m and of sqrt(v) and an
+ *      fp32 scale per block.
  *   or ur_grad_clip scales the gradients in place.
  * Parameters and gradients are dense fp32; tensors of a list must not overlap. */
-typedef struct {
-    void* param;      /* may be NULL for ur_grad_sqnorm / ur_grad_clip */
-    void* grad;
-    long long n;      /* elements */
-    long long block;  /* first block of 256 elements in the state buffers */
-    long long slot;   /* index into steps */
-} ur_param;
 size_t ur_param_table_bytes(int ntensors);
-int ur_param_table(const ur_param* list, int ntensors, void* table, size_t table_bytes, int* steps, double lr, double beta1,
-                   double beta2, long long* nchunks, ur_stream_t s);
+int ur_param_table(const long long* params, const long long* grads, const long long* sizes, const long long* blocks, int ntensors,
+                   void* table, size_t table_bytes, int* steps, double lr, double beta1, double beta2, long long* nchunks,
+                   ur_stream_t s);
 int ur_grad_sqnorm_max_parts(void);
 int ur_grad_sqnorm(const void* table, int ntensors, long long nchunks, double* parts, int* nparts, ur_stream_t s);
 int ur_grad_clip(const void* table, int ntensors, long long nchunks, const double* parts, int nparts, float max_norm,

@@ -4,6 +4,7 @@ The library is the product path: if it is missing, loading fails loudly -- there
 CPU or ATen fallback anywhere in this package.
 """
 import ctypes as C
+import importlib.util
 import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -150,7 +151,7 @@ SIGNATURES = {
     "ur_adam_multi_dev": (_i, [_vp, _vp, _i, _ll, _f, _f, _f, _f, _f, _f, _vp]),
     "ur_sgd_multi": (_i, [_vp, _vp, _i, _ll, _f, _f, _f, _vp]),
     "ur_param_table_bytes": (_sz, [_i]),
-    "ur_param_table": (_i, [_vp, _i, _vp, _sz, _vp, _d, _d, _d, _vp, _vp]),
+    "ur_param_table": (_i, [_vp, _vp, _vp, _vp, _i, _vp, _sz, _vp, _d, _d, _d, _vp, _vp]),
     "ur_grad_sqnorm_max_parts": (_i, []),
     "ur_grad_sqnorm": (_i, [_vp, _i, _ll, _vp, _vp, _vp]),
     "ur_grad_clip": (_i, [_vp, _i, _ll, _vp, _i, _f, _vp, _vp]),
@@ -176,6 +177,24 @@ def load():
         fn.argtypes = args
     _lib = lib
     return lib
+
+
+_param_list = None
+
+
+def param_list():
+    """The host module that reads parameter lists (csrc/param_list.cpp), loaded once."""
+    global _param_list
+    if _param_list is None:
+        path = os.path.join(_HERE, "lib", "_param_list.so")
+        if not os.path.exists(path):
+            raise UResNetHipError("_param_list.so not found at %s -- build it with `python __graft_entry__.py build`" % path)
+        spec = importlib.util.spec_from_file_location("_param_list", path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        module.set_error_type(UResNetHipError)
+        _param_list = module
+    return _param_list
 
 
 def call(name, *args):

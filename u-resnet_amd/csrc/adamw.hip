@@ -7,9 +7,9 @@
 // Bound by HBM: 28 bytes per element with 32-bit moments, 16 + 1/16 with 8-bit ones, 4 more where the norm is taken (the
 // gradients are read twice, the second time partly from the last-level cache).
 //
-// Work list.  The host hands over the tensors by value (ur_param rows, as kernel arguments); param_table_kernel writes them
-// as a table in the caller's workspace, advances the step counts and derives the bias corrections.  No staging buffer and
-// no copy from the host: a captured graph replays the whole step.  The other kernels walk chunks of 2048 elements of all
+// Work list.  The host hands over the tensors by value (as kernel arguments); param_table_kernel writes them as a table in
+// the caller's workspace, advances the step counts and derives the bias corrections.  No staging buffer and no copy from
+// the host: a captured graph replays the whole step.  The other kernels walk chunks of 2048 elements of all
 // tensors in one launch and find a chunk's tensor in the sorted list of first chunks, 64 entries per look.
 //
 // 8-bit moments.  m and r = sqrt(v) are stored as e4m3 codes (3 mantissa bits, exponents over 2^17) with one fp32 scale per
@@ -26,7 +26,7 @@ namespace {
 constexpr int NT = 256;
 constexpr int BLOCK = 256;                   // elements per scale
 constexpr int CHUNK = 2048;                  // elements per unit of work: two 16-byte accesses per thread and tensor
-constexpr int BATCH = 80;                    // rows per table launch: kernel arguments stay under 4 KB
+constexpr int BATCH = 136;                   // rows per table launch: kernel arguments stay under 4 KB
 constexpr int MAX_PARTS = 1024;              // partial sums of the norm
 constexpr float TOP = 448.f;
 
@@ -43,43 +43,40 @@ struct Row {
     unsigned pad;
 };
 
-struct ListRow {
-    void* p;
-    void* g;
-    long long n, block;
-    int slot, first;
-};
 struct ListBatch {
     int count, at;
-    ListRow r[BATCH];
+    void* p[BATCH];
+    void* g[BATCH];                          // null: nothing to do for this tensor
+    long long n[BATCH];
+    int first[BATCH];
 };
 
 // table: Row[ntensors], then int first[ntensors] (first chunk of every tensor)
 __device__ __forceinline__ const int* firsts(const Row* rows, int ntensors) { return reinterpret_cast<const int*>(rows + ntensors); }
 
-__global__ __launch_bounds__(128) void param_table_kernel(ListBatch b, Row* __restrict__ rows, int ntensors, int* __restrict__ steps,
-                                                          double lr, double beta1, double beta2) {
-    const int i = threadIdx.x;
+__global__ __launch_bounds__(192) void param_table_kernel(ListBatch b, Row* __restrict__ rows, int ntensors,
+                                                          const long long* __restrict__ blocks, int* __restrict__ steps, double lr,
+                                                          double beta1, double beta2) {
+    const int i = threadIdx.x, t = b.at + i;
     if (i >= b.count) return;
-    const ListRow l = b.r[i];
     Row w;
-    w.p = (float*)l.p;
-    w.g = (float*)l.g;
-    w.n = l.n;
-    w.block = l.block;
+    w.p = (float*)b.p[i];
+    w.g = (float*)b.g[i];
+    w.n = b.g[i] ? b.n[i] : 0;
+    w.block = blocks ? blocks[t] : 0;
     w.step_size = 0.f;
     w.bc2_sqrt = 1.f;
     w.step = 0;
     w.pad = 0;
-    if (steps) {
-        const int t = steps[l.slot] + 1;
-        steps[l.slot] = t;
-        w.step = (unsigned)t;
-        w.step_size = (float)(lr / (1.0 - pow(beta1, (double)t)));
-        w.bc2_sqrt = (float)sqrt(1.0 - pow(beta2, (double)t));
+    if (steps && w.n) {
+        const int step = steps[t] + 1;
+        steps[t] = step;
+        w.step = (unsigned)step;
+        w.step_size = (float)(lr / (1.0 - pow(beta1, (double)step)));
+        w.bc2_sqrt = (float)sqrt(1.0 - pow(beta2, (double)step));
     }
-    rows[b.at + i] = w;
-    reinterpret_cast<int*>(rows + ntensors)[b.at + i] = l.first;
+    rows[t] = w;
+    reinterpret_cast<int*>(rows + ntensors)[t] = b.first[i];
 }
 
 // the tensor that a chunk belongs to: the last entry of the sorted list that is not above it (a whole wave looks)
@@ -300,16 +297,6 @@ __global__ __launch_bounds__(NT) void adamw_kernel(const Row* __restrict__ rows,
     }
 }
 
-// chunks of all tensors; -1: a bad row
-long long count_chunks(const ur_param* list, int ntensors) {
-    long long chunks = 0;
-    for (int i = 0; i < ntensors; ++i) {
-        if (!list[i].grad || list[i].n <= 0 || list[i].n > (1LL << 40) || list[i].block < 0 || list[i].slot < 0 || list[i].slot > 0x7fffffffLL) return -1;
-        chunks += (list[i].n + CHUNK - 1) / CHUNK;
-    }
-    return chunks;
-}
-
 int norm_parts(long long chunks) { return (int)(chunks < MAX_PARTS ? chunks : MAX_PARTS); }
 
 }  // namespace
@@ -319,29 +306,30 @@ extern "C" {
 size_t ur_param_table_bytes(int ntensors) { return ntensors <= 0 ? 0 : (size_t)ntensors * (sizeof(Row) + sizeof(int)); }
 int ur_grad_sqnorm_max_parts(void) { return MAX_PARTS; }
 
-int ur_param_table(const ur_param* list, int ntensors, void* table, size_t table_bytes, int* steps, double lr, double beta1, double beta2,
-                   long long* nchunks, ur_stream_t s) {
-    UR_REQUIRE(list && ntensors > 0 && table && nchunks, "param_table: bad arguments");
+int ur_param_table(const long long* params, const long long* grads, const long long* sizes, const long long* blocks, int ntensors,
+                   void* table, size_t table_bytes, int* steps, double lr, double beta1, double beta2, long long* nchunks,
+                   ur_stream_t s) {
+    UR_REQUIRE(grads && sizes && ntensors > 0 && table && nchunks, "param_table: bad arguments");
     UR_REQUIRE(table_bytes >= ur_param_table_bytes(ntensors), "param_table: table too small");
-    const long long chunks = count_chunks(list, ntensors);
-    UR_REQUIRE(chunks > 0 && chunks <= 0x7fffffffLL, "param_table: a tensor without gradient or elements, or too many elements");
+    long long chunks = 0;
+    for (int i = 0; i < ntensors; ++i) {
+        UR_REQUIRE(sizes[i] >= 0 && sizes[i] <= (1LL << 40), "param_table: a tensor of %lld elements", sizes[i]);
+        if (grads[i]) chunks += (sizes[i] + CHUNK - 1) / CHUNK;
+    }
+    UR_REQUIRE(chunks > 0 && chunks <= 0x7fffffffLL, "param_table: no gradient with elements, or too many elements");
     int first = 0;
     for (int at = 0; at < ntensors; at += BATCH) {
-        ListBatch b;
+        ListBatch b = {};
         b.count = ntensors - at < BATCH ? ntensors - at : BATCH;
         b.at = at;
         for (int i = 0; i < b.count; ++i) {
-            const ur_param& l = list[at + i];
-            b.r[i].p = l.param;
-            b.r[i].g = l.grad;
-            b.r[i].n = l.n;
-            b.r[i].block = l.block;
-            b.r[i].slot = (int)l.slot;
-            b.r[i].first = first;
-            first += (int)((l.n + CHUNK - 1) / CHUNK);
+            b.p[i] = params ? (void*)params[at + i] : nullptr;
+            b.g[i] = sizes[at + i] ? (void*)grads[at + i] : nullptr;
+            b.n[i] = sizes[at + i];
+            b.first[i] = first;
+            if (b.g[i]) first += (int)((b.n[i] + CHUNK - 1) / CHUNK);
         }
-        for (int i = b.count; i < BATCH; ++i) b.r[i] = b.r[0];
-        hipLaunchKernelGGL(param_table_kernel, dim3(1), dim3(128), 0, (hipStream_t)s, b, (Row*)table, ntensors, steps, lr, beta1, beta2);
+        hipLaunchKernelGGL(param_table_kernel, dim3(1), dim3(192), 0, (hipStream_t)s, b, (Row*)table, ntensors, blocks, steps, lr, beta1, beta2);
     }
     *nchunks = chunks;
     return ur_check_launch("param_table");

@@ -23,6 +23,20 @@ for s in "${SRCS[@]}"; do
         pids+=($!)
     fi
 done
+# the optimisers' parameter lists: host code against torch's headers, with the interpreter that will load it
+PY="${PYTHON:-python3}"
+LIST="$OUT/_param_list.so"
+if [ ! -f "$LIST" ] || [ "$HERE/param_list.cpp" -nt "$LIST" ]; then
+    (
+        TORCH="$($PY -c 'import os, torch; print(os.path.dirname(torch.__file__))')"
+        PYINC="$($PY -c 'import sysconfig; print(sysconfig.get_paths()["include"])')"
+        ABI="$($PY -c 'import torch; print(int(torch._C._GLIBCXX_USE_CXX11_ABI))')"
+        "${CXX:-g++}" -O2 -std=c++17 -fPIC -shared -Wall -D_GLIBCXX_USE_CXX11_ABI="$ABI" -isystem "$TORCH/include" \
+            -isystem "$TORCH/include/torch/csrc/api/include" -I"$PYINC" "$HERE/param_list.cpp" -o "$LIST" \
+            -L"$TORCH/lib" -ltorch_python -ltorch_cpu -lc10 -Wl,-rpath,"$TORCH/lib"
+    ) &
+    pids+=($!)
+fi
 for p in "${pids[@]:-}"; do [ -n "$p" ] && wait "$p"; done
 objs=()
 for s in "${SRCS[@]}"; do objs+=("$OBJ/$s.o"); done

@@ -8,7 +8,9 @@
   metrics           calculate_metrics / validate (train_UResNetAblitionStudy.py:70-100, 128-164)
   checkpoints       the dict written at train_UResNetAblitionStudy.py:244-252 (save_checkpoint / load_checkpoint)
 """
+import array
 import ctypes as C
+import operator
 
 import torch
 
@@ -300,72 +302,58 @@ class SGD(_MultiTensorOptimizer):
 
 
 class _ParamList:
-    """Tensors of one launch as the C entry points take them (ur_param rows in host memory): built, used and dropped within
-    a call."""
+    """Tensors of one launch: addresses and sizes as int64 arrays in host memory (_lib.param_list()), their table and, where
+    the norm is taken, room for its partial sums in device memory."""
+    PARTS = 1024                                 # ur_grad_sqnorm_max_parts()
 
-    def __init__(self, rows, device):
-        self.count, self.device = len(rows) // 5, device
-        self._rows = (C.c_longlong * len(rows))(*rows)
-        self.table = torch.empty(_lib.query("ur_param_table_bytes", self.count), dtype=torch.uint8, device=device)
-        self.chunks = C.c_longlong()
+    def __init__(self, params, grads, sizes, device, parts=0):
+        self.params, self.grads, self.sizes, self.count = params, grads, sizes, len(sizes) // 8
+        self.bytes = -(-_lib.query("ur_param_table_bytes", self.count) // 16) * 16
+        self.buf = torch.empty(self.bytes + 8 * parts, dtype=torch.uint8, device=device)
+        self.table = self.buf.data_ptr()
+        self.parts = self.table + self.bytes
+        self.chunks = 0
 
-    def write(self, steps=None, lr=0.0, betas=(0.0, 0.0)):
-        _lib.call("ur_param_table", self._rows, self.count, self.table.data_ptr(), self.table.numel(), ops._p(steps), lr, betas[0],
-                  betas[1], C.byref(self.chunks), ops._stream())
+    def write(self, stream, blocks=None, steps=None, lr=0.0, betas=(0.0, 0.0)):
+        n = C.c_longlong()
+        _lib.call("ur_param_table", self.params, self.grads, self.sizes, blocks, self.count, self.table, self.bytes, steps, lr, betas[0],
+                  betas[1], C.byref(n), stream)
+        self.chunks = n.value
 
-    def sqnorm(self, parts, at):
-        """Partial sums of the squared gradients into parts[at:]; returns the place behind them."""
+    def sqnorm(self, parts, stream):
+        """Partial sums of the squared gradients at the address `parts`; returns their number."""
         n = C.c_int()
-        _lib.call("ur_grad_sqnorm", self.table.data_ptr(), self.count, self.chunks.value, parts.data_ptr() + 8 * at, C.byref(n),
-                  ops._stream())
-        return at + n.value
-
-
-def _check_grad(g, device, what):
-    if g.layout is not torch.strided or g.dtype is not torch.float32 or g.device != device or not g.is_cuda:
-        raise _lib.UResNetHipError("%s: gradients must be dense fp32 tensors on one GPU (got %s, %s on %s)"
-                                   % (what, g.layout, g.dtype, g.device))
+        _lib.call("ur_grad_sqnorm", self.table, self.count, self.chunks, parts, C.byref(n), stream)
+        return n.value
 
 
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
     """torch.nn.utils.clip_grad_norm_ for fp32 gradients on one GPU: scales them in place by min(1, max_norm / (norm + 1e-6))
     and returns their norm before that as a 0-dim device tensor.  No host synchronisation (except with error_if_nonfinite,
     which raises before anything is scaled), no staging buffers: it can be captured in a graph.  A norm within the limit
-    leaves the gradients untouched.  Only the 2-norm."""
+    leaves the gradients untouched.  Only the 2-norm; gradients must not overlap."""
     if norm_type != 2:
         raise NotImplementedError("clip_grad_norm_: only norm_type=2 is implemented (got %r)" % (norm_type,))
     max_norm = float(max_norm)
     if not max_norm >= 0:
         raise ValueError("clip_grad_norm_: max_norm must not be negative (got %r)" % (max_norm,))
-    if torch.is_tensor(parameters):
-        parameters = [parameters]
-    grads = [g for g in (p.grad for p in parameters) if g is not None]
-    if not grads:
+    grads, sizes, count, index = _lib.param_list().clip_rows([parameters] if torch.is_tensor(parameters) else list(parameters))
+    if index < 0:
         return torch.tensor(0.0)
-    device, rows, seen = grads[0].device, [], set()
-    for g in grads:
-        _check_grad(g, device, "clip_grad_norm_")
-        if not (g.is_contiguous() or g.is_contiguous(memory_format=ops.CL) if g.dim() == 4 else g.is_contiguous()):
-            raise _lib.UResNetHipError("clip_grad_norm_: a gradient of shape %s is not dense" % (tuple(g.shape),))
-        n = g.numel()
-        if n:
-            ptr = g.data_ptr()
-            if ptr in seen:
-                raise ValueError("clip_grad_norm_: a gradient is listed twice")
-            seen.add(ptr)
-            rows += (0, ptr, n, 0, 0)
+    device = torch.device("cuda", index)
     with ops._on(device):
-        if not rows:
+        if not count:
             return torch.zeros((), device=device)
+        stream = ops._stream()
         norm = torch.empty((), device=device)
-        plist = _ParamList(rows, device)
-        parts = torch.empty(_lib.query("ur_grad_sqnorm_max_parts"), dtype=torch.float64, device=device)
-        plist.write()
-        nparts = plist.sqnorm(parts, 0)
-        if error_if_nonfinite and not bool(torch.isfinite(parts[:nparts].sum().float())):
-            raise RuntimeError("clip_grad_norm_: the total norm of the gradients is not finite")
-        _lib.call("ur_grad_clip", plist.table.data_ptr(), plist.count, plist.chunks.value, parts.data_ptr(), nparts, max_norm,
-                  norm.data_ptr(), ops._stream())
+        plist = _ParamList(None, grads, sizes, device, _ParamList.PARTS)
+        plist.write(stream)
+        nparts = plist.sqnorm(plist.parts, stream)
+        if error_if_nonfinite:
+            total = plist.buf[plist.bytes:plist.bytes + 8 * nparts].view(torch.float64).sum()
+            if not bool(torch.isfinite(total)):
+                raise RuntimeError("clip_grad_norm_: the total norm of the gradients is not finite")
+        _lib.call("ur_grad_clip", plist.table, plist.count, plist.chunks, plist.parts, nparts, max_norm, norm.data_ptr(), stream)
     return norm
 
 
@@ -376,13 +364,15 @@ class _MomentPool:
 
     def __init__(self, group, state):
         self.params, self.bits, self.device = list(group['params']), group['state_bits'], group['params'][0].device
-        self.sizes = [p.numel() for p in self.params]
+        sizes = [p.numel() for p in self.params]
         self.blocks, at = [], 0
-        for p, n in zip(self.params, self.sizes):
+        for p, n in zip(self.params, sizes):
             if p.dtype != torch.float32 or not p.is_contiguous() or p.device != self.device:
                 raise _lib.UResNetHipError("AdamW: the parameters of a group must be contiguous fp32 tensors on one device")
             self.blocks.append(at)
             at += -(-n // self.BLOCK)
+        self.sizes = array.array('q', sizes).tobytes()
+        self.blocks_there = torch.tensor(self.blocks, dtype=torch.int64, device=self.device)
         self.steps = torch.zeros(len(self.params), dtype=torch.int32, device=self.device)
         many = at * self.BLOCK
         if self.bits == 32:
@@ -392,9 +382,12 @@ class _MomentPool:
             for k in ('exp_avg', 'exp_avg_sq_root'):
                 self.buffers[k] = torch.zeros(many, dtype=torch.uint8, device=self.device).view(torch.float8_e4m3fn)
                 self.buffers[k + '_scale'] = torch.zeros(at, device=self.device)
-        for i, p in enumerate(self.params):                    # what the parameters bring along
+        self.waiting = []                                      # parameters without a state: no gradient yet
+        for i, p in enumerate(self.params):                    # what the others bring along
             old = state.get(p)
-            if old:
+            if not old:
+                self.waiting.append(i)
+            else:
                 new = self.views(i)
                 for k, v in new.items():
                     v.copy_(torch.as_tensor(old[k]).reshape(v.shape))
@@ -402,11 +395,12 @@ class _MomentPool:
 
     def holds(self, group):
         ps = group['params']
-        return (len(ps) == len(self.params) and all(a is b for a, b in zip(ps, self.params)) and group['state_bits'] == self.bits
+        return (len(ps) == len(self.params) and all(map(operator.is_, ps, self.params)) and group['state_bits'] == self.bits
                 and ps[0].device == self.device)
 
     def views(self, i):
-        b, n, p = self.blocks[i], self.sizes[i], self.params[i]
+        b, p = self.blocks[i], self.params[i]
+        n = p.numel()
         out = {'step': self.steps[i]}
         for k, buf in self.buffers.items():
             if k.endswith('_scale'):
@@ -473,66 +467,63 @@ class AdamW(torch.optim.Optimizer):
         exp_avg, exp_avg_sq; 8 bits: exp_avg, exp_avg_sq_root and a scale per 256 elements).  The optimiser's own buffers."""
         return dict(self._pool(group, self.param_groups[group]).buffers)
 
-    @torch.no_grad()
     def step(self, closure=None):
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        if sum(len(pool.params) - len(pool.waiting) for pool in self._pools.values()) != len(self.state):
+            self._pools = {}                                   # `state` was cleared or replaced: built again from it
         work = []
         for gi, group in enumerate(self.param_groups):
             if not group['params']:
                 continue
-            pool, rows, held = self._pool(gi, group), [], []
-            state, dev = self.state, pool.device
-            for i, p in enumerate(pool.params):
-                g = p.grad
-                if g is None:
-                    continue
-                if g.dtype is not torch.float32 or not g.is_contiguous() or g.is_sparse:
-                    _check_grad(g, dev, "AdamW")
-                    g = g.contiguous()
-                    held.append(g)                             # until the launches that read it are queued
-                if p not in state:
-                    state[p] = pool.views(i)
-                n = pool.sizes[i]
-                if p.numel() != n or p.device != dev or g.numel() != n or not p.is_contiguous():
-                    raise _lib.UResNetHipError("AdamW: a parameter changed its size, layout or device")
-                if n:
-                    rows += (p.data_ptr(), g.data_ptr(), n, pool.blocks[i], i)
-            if rows:
-                if dev.type != 'cuda':
-                    raise _lib.UResNetHipError("AdamW: parameters must be on a GPU (got %s)" % dev)
-                work.append((group, pool, rows, held))
-        if not work:
-            return loss
-        dev = work[0][1].device
-        if any(w[1].device != dev for w in work):
-            raise _lib.UResNetHipError("AdamW: all parameters must be on one GPU")
-        with ops._on(dev):
-            lists = []
-            for group, pool, rows, _ in work:
-                lists.append(_ParamList(rows, dev))
-                lists[-1].write(pool.steps, float(group['lr']), group['betas'])
-            parts, nparts, norm = None, 0, None
-            if self.max_grad_norm is not None:
-                norm = torch.empty((), device=dev)
-                parts = torch.empty(len(lists) * _lib.query("ur_grad_sqnorm_max_parts"), dtype=torch.float64, device=dev)
-                for plist in lists:
-                    nparts = plist.sqnorm(parts, nparts)
-            for (group, pool, _, _), plist in zip(work, lists):
-                names = list(pool.buffers)
-                if pool.bits == 32:
-                    m, v, ms, vs = pool.buffers['exp_avg'], pool.buffers['exp_avg_sq'], None, None
-                else:
-                    m, ms, v, vs = (pool.buffers[k] for k in names)
-                _lib.call("ur_adamw_multi", plist.table.data_ptr(), plist.count, plist.chunks.value, pool.bits, m.data_ptr(), v.data_ptr(),
-                          ops._p(ms), ops._p(vs), float(group['lr']), group['betas'][0], group['betas'][1], group['eps'],
-                          group['weight_decay'], ops._p(parts), nparts, float(self.max_grad_norm or 0.0), float(self.grad_scale),
-                          ops._p(norm), ops._stream())
-            self.grad_norm = norm
-        ops.bump_weights_epoch()
+            pool, rows = self._pool(gi, group), _lib.param_list().adamw_rows
+            params, grads, live, uneven = rows(pool.params, pool.sizes, None)
+            held = None
+            if uneven:                                         # copies, until the launches that read them are queued
+                with torch.no_grad():
+                    held = [p.grad if p.grad is None else p.grad.contiguous() for p in pool.params]
+                params, grads, live, _ = rows(pool.params, pool.sizes, held)
+            if pool.waiting:
+                for i in [i for i in pool.waiting if pool.params[i].grad is not None]:
+                    pool.waiting.remove(i)
+                    self.state[pool.params[i]] = pool.views(i)
+            if live and any(grads):
+                work.append((group, pool, params, grads, held))
+        self.grad_norm = None
+        if work:
+            dev = work[0][1].device
+            if any(w[1].device != dev for w in work):
+                raise _lib.UResNetHipError("AdamW: all parameters must be on one GPU")
+            with ops._on(dev):
+                self._launch(work, dev)
+            ops.bump_weights_epoch()
         return loss
+
+    def _launch(self, work, dev):
+        stream = ops._stream()
+        clip = self.max_grad_norm is not None
+        lists, parts, nparts, norm = [], None, 0, None
+        for group, pool, params, grads, _ in work:
+            plist = _ParamList(params, grads, pool.sizes, dev, _ParamList.PARTS * len(work) if clip and not lists else 0)
+            plist.write(stream, pool.blocks_there.data_ptr(), pool.steps.data_ptr(), float(group['lr']), group['betas'])
+            lists.append(plist)
+        if clip:
+            norm, parts = torch.empty((), device=dev), lists[0].parts
+            for plist in lists:
+                nparts += plist.sqnorm(parts + 8 * nparts, stream)
+        for (group, pool, _, _, _), plist in zip(work, lists):
+            buf = pool.buffers
+            if pool.bits == 32:
+                state = (buf['exp_avg'].data_ptr(), buf['exp_avg_sq'].data_ptr(), None, None)
+            else:
+                state = (buf['exp_avg'].data_ptr(), buf['exp_avg_sq_root'].data_ptr(), buf['exp_avg_scale'].data_ptr(),
+                         buf['exp_avg_sq_root_scale'].data_ptr())
+            _lib.call("ur_adamw_multi", plist.table, plist.count, plist.chunks, pool.bits, *state, float(group['lr']), group['betas'][0],
+                      group['betas'][1], group['eps'], group['weight_decay'], parts, nparts, float(self.max_grad_norm or 0.0),
+                      float(self.grad_scale), ops._p(norm), stream)
+        self.grad_norm = norm
 
     def state_dict(self):
         sd = super().state_dict()
