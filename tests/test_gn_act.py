@@ -330,9 +330,19 @@ def test_double_backward_and_bad_arguments_are_refused():
     x, dy, r, gn = make((2, 16, 5, 7, 4), torch.float32, 11, residual=True)
     gn = gn.to(DEV)
     xd = x.to(DEV).requires_grad_()
-    gx = torch.autograd.grad(ops.gn_act(xd, gn, act=ACTS["silu"]).square().sum(), xd, create_graph=True)[0]
-    with pytest.raises(RuntimeError):
-        gx.sum().backward()
+    with pytest.raises(RuntimeError, match="double backward"):
+        torch.autograd.grad(ops.gn_act(xd, gn, act=ACTS["silu"]).square().sum(), xd, create_graph=True)
+    y = ops.gn_act(xd, gn)
+    first = torch.autograd.grad(y.sum(), xd, retain_graph=True)[0]
+    assert torch.equal(torch.autograd.grad(y.sum(), xd)[0], first)
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(y.sum(), xd)
+    xc = xd.detach().contiguous(memory_format=torch.channels_last).requires_grad_()       # (NCHW inputs are saved as a copy)
+    y = ops.gn_act(xc, gn)
+    with torch.no_grad():
+        xc.add_(1.0)                                            # a saved tensor that changed
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
     with pytest.raises(RuntimeError, match="channels"):
         ops.gn_act(torch.randn(1, 8, 4, 4, device=DEV), gn)
     with pytest.raises(RuntimeError, match="residual"):

@@ -179,22 +179,25 @@ def load():
     return lib
 
 
-_param_list = None
+_host = None
 
 
-def param_list():
-    """The host module that reads parameter lists (csrc/param_list.cpp), loaded once."""
-    global _param_list
-    if _param_list is None:
-        path = os.path.join(_HERE, "lib", "_param_list.so")
+def host():
+    """The host module (csrc/host), loaded once and told where the kernel library's entry points are."""
+    global _host
+    if _host is None:
+        path = os.path.join(_HERE, "lib", "_host.so")
         if not os.path.exists(path):
-            raise UResNetHipError("_param_list.so not found at %s -- build it with `python __graft_entry__.py build`" % path)
-        spec = importlib.util.spec_from_file_location("_param_list", path)
+            raise UResNetHipError("_host.so not found at %s -- build it with `python __graft_entry__.py build`" % path)
+        lib = load()
+        spec = importlib.util.spec_from_file_location("_host", path)
         module = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(module)
         module.set_error_type(UResNetHipError)
-        _param_list = module
-    return _param_list
+        module.set_entry_points(*(C.cast(getattr(lib, name), C.c_void_p).value for name in
+                                  ("ur_gn_fwd_workspace", "ur_gn_bwd_workspace", "ur_gn_act_fwd", "ur_gn_act_bwd", "ur_last_error")))
+        _host = module
+    return _host
 
 
 def call(name, *args):

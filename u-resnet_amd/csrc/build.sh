@@ -23,22 +23,26 @@ for s in "${SRCS[@]}"; do
         pids+=($!)
     fi
 done
-# the optimisers' parameter lists: host code against torch's headers, with the interpreter that will load it
+# the host module: host code against torch's headers, for the interpreter that will load it
 PY="${PYTHON:-python3}"
-LIST="$OUT/_param_list.so"
-if [ ! -f "$LIST" ] || [ "$HERE/param_list.cpp" -nt "$LIST" ]; then
-    (
-        TORCH="$($PY -c 'import os, torch; print(os.path.dirname(torch.__file__))')"
-        PYINC="$($PY -c 'import sysconfig; print(sysconfig.get_paths()["include"])')"
-        ABI="$($PY -c 'import torch; print(int(torch._C._GLIBCXX_USE_CXX11_ABI))')"
-        "${CXX:-g++}" -O2 -std=c++17 -fPIC -shared -Wall -D_GLIBCXX_USE_CXX11_ABI="$ABI" -isystem "$TORCH/include" \
-            -isystem "$TORCH/include/torch/csrc/api/include" -I"$PYINC" "$HERE/param_list.cpp" -o "$LIST" \
-            -L"$TORCH/lib" -ltorch_python -ltorch_cpu -lc10 -Wl,-rpath,"$TORCH/lib"
-    ) &
-    pids+=($!)
-fi
+HOST="$OUT/_host.so"
+HOSTSRC=(module param_list gn_function)
+TORCH="$($PY -c 'import importlib.util as u; print(u.find_spec("torch").submodule_search_locations[0])')"
+PYINC="$($PY -c 'import sysconfig; print(sysconfig.get_paths()["include"])')"
+for s in "${HOSTSRC[@]}"; do
+    src="$HERE/host/$s.cpp"
+    obj="$OBJ/host_$s.o"
+    if [ ! -f "$obj" ] || [ "$src" -nt "$obj" ] || [ "$HERE/host/host.h" -nt "$obj" ] || [ "$HERE/../../include/uresnet_hip.h" -nt "$obj" ]; then
+        ( "${CXX:-g++}" -O2 -std=c++17 -fPIC -Wall -D__HIP_PLATFORM_AMD__=1 -isystem "$TORCH/include" \
+            -isystem "$TORCH/include/torch/csrc/api/include" -isystem "${ROCM_PATH:-/opt/rocm}/include" -I"$PYINC" -c "$src" -o "$obj" ) &
+        pids+=($!)
+    fi
+done
 for p in "${pids[@]:-}"; do [ -n "$p" ] && wait "$p"; done
 objs=()
 for s in "${SRCS[@]}"; do objs+=("$OBJ/$s.o"); done
 $HIPCC --offload-arch=gfx950 -shared -fPIC -o "$OUT/liburesnet_hip.so" "${objs[@]}"
+hobjs=()
+for s in "${HOSTSRC[@]}"; do hobjs+=("$OBJ/host_$s.o"); done
+"${CXX:-g++}" -shared -fPIC -o "$HOST" "${hobjs[@]}" -L"$TORCH/lib" -ltorch_python -ltorch_cpu -lc10_hip -lc10 -Wl,-rpath,"$TORCH/lib"
 echo "built $OUT/liburesnet_hip.so"

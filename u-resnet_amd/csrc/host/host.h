@@ -1,0 +1,24 @@
+// The host module (_host): what a step does per tensor or per call outside the kernels, where the interpreter would cost more
+// than the launch.  Host code only, against torch's C++ interface; the kernels are reached through the C ABI, whose addresses
+// the loader hands over (set_entry_points), so that one library serves both.
+#pragma once
+#include <Python.h>
+#include <torch/csrc/autograd/python_variable.h>
+
+#include <string>
+
+#include "../../../include/uresnet_hip.h"
+
+struct EntryPoints {
+    decltype(&ur_gn_fwd_workspace) gn_fwd_workspace;
+    decltype(&ur_gn_bwd_workspace) gn_bwd_workspace;
+    decltype(&ur_gn_act_fwd) gn_act_fwd;
+    decltype(&ur_gn_act_bwd) gn_act_bwd;
+    decltype(&ur_last_error) last_error;
+};
+extern EntryPoints entry;
+
+PyObject* fail(const std::string& text);                   // raises the package's error type
+PyObject* adamw_rows(PyObject* self, PyObject* args);
+PyObject* clip_rows(PyObject* self, PyObject* params);
+PyObject* gn_act(PyObject* self, PyObject* args);

@@ -1,28 +1,17 @@
 // Reads lists of parameters for the multi-tensor optimiser entry points: addresses and sizes of parameters and gradients as
 // arrays, with the checks that the kernels rely on.  Host code only; a call per step instead of some ten interpreter calls per
 // parameter (134 tensors: 130 us -> 3 us).
-#include <Python.h>
-#include <torch/csrc/autograd/python_variable.h>
+#include "host.h"
 
 #include <algorithm>
-#include <exception>
-#include <string>
 #include <vector>
 
 namespace {
-
-PyObject* error_type = nullptr;
-
-PyObject* fail(const std::string& text) {
-    PyErr_SetString(error_type ? error_type : PyExc_RuntimeError, text.c_str());
-    return nullptr;
-}
 
 std::string told(const at::Tensor& t) {
     return std::string(c10::toString(t.layout())) + " " + c10::toString(t.scalar_type()) + " on " + t.device().str();
 }
 
-// nullptr, or what is wrong with a gradient
 bool plain_gpu_f32(const at::Tensor& g, c10::Device device) {
     return g.layout() == c10::kStrided && g.scalar_type() == at::kFloat && g.device() == device && device.is_cuda();
 }
@@ -39,6 +28,8 @@ bool get_tensor(PyObject* o, at::Tensor& out) {
     out = THPVariable_Unpack(o);
     return true;
 }
+
+}  // namespace
 
 // adamw_rows(params, sizes, grads or None) -> (params, grads, live, uneven): addresses as int64 arrays; a parameter without
 // gradient has a zero.  live: how many have one.  uneven: whether a gradient is not contiguous (its address is left zero).
@@ -97,30 +88,3 @@ PyObject* clip_rows(PyObject*, PyObject* params) {
     }
     return Py_BuildValue("NNni", bytes_of(gs), bytes_of(ns), (Py_ssize_t)gs.size(), device);
 }
-
-PyObject* set_error_type(PyObject*, PyObject* type) {
-    Py_INCREF(type);
-    Py_XDECREF(error_type);
-    error_type = type;
-    Py_RETURN_NONE;
-}
-
-// C++ exceptions become Python ones
-template <PyObject* (*F)(PyObject*, PyObject*)>
-PyObject* guarded(PyObject* self, PyObject* args) {
-    try {
-        return F(self, args);
-    } catch (const std::exception& e) {
-        return fail(e.what());
-    }
-}
-
-PyMethodDef methods[] = {{"adamw_rows", guarded<adamw_rows>, METH_VARARGS, "addresses of parameters and gradients"},
-                         {"clip_rows", guarded<clip_rows>, METH_O, "addresses and sizes of gradients"},
-                         {"set_error_type", set_error_type, METH_O, "exception type for refused tensors"},
-                         {nullptr, nullptr, 0, nullptr}};
-PyModuleDef module = {PyModuleDef_HEAD_INIT, "_param_list", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
-
-}  // namespace
-
-PyMODINIT_FUNC PyInit__param_list(void) { return PyModule_Create(&module); }

@@ -13,7 +13,6 @@ import weakref
 
 import torch
 from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import ConvDesc, call, query
@@ -1029,102 +1028,25 @@ def bn_act(y, bn, residual=None, stats=None, act=_lib.ACT_RELU, out=None, pool=F
     return z
 
 
-def _gn_call(name, dev, tag, nbytes, *args):
-    """One GroupNorm entry point on `dev` and its current stream (appended to args)."""
-    if kernel_timings is None and dev.index == torch.cuda.current_device():
-        call(name, *args, torch._C._cuda_getCurrentRawStream(dev.index))
-    else:
-        with _on(dev), _Timed(tag, nbytes):
-            call(name, *args, _stream())
-
-
-class _GNAct(Function):
-    """act(GroupNorm(x) (+ residual)).  Saved: x, the residual (its activation's derivative needs the sum) and the fp64
-    {mean, rstd} of every image and group; the pre-activation is recomputed from them in backward."""
-
-    @staticmethod
-    def forward(ctx, x, gamma, beta, residual, groups, eps, act, slope, out):
-        n, c, h, w = x.shape
-        dev, dt = x.device, _DT[x.dtype]
-        x_ld, r_ld = _pitch(x), 0 if residual is None else _pitch(residual)
-        if out is None:
-            z, z_ld = empty_nhwc(n, c, h, w, x.dtype, dev), c
-        else:                                        # (window,): a channel window of a wider tensor (alias_window)
-            z = out[0]
-            z_ld = _channel_pitch(z)
-            if tuple(z.shape) != tuple(x.shape) or z.dtype != x.dtype or z.device != dev or not z_ld:
-                raise RuntimeError("gn_act: `out` must be a channel window with x's shape, dtype and device")
-        stats = torch.empty((n, groups, 2), dtype=torch.float64, device=dev)
-        ws_bytes = query("ur_gn_fwd_workspace", dt, n, h * w, c, groups)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-        _gn_call("ur_gn_act_fwd", dev, "hbm:gn_fwd", x.numel() * x.element_size() * (3 if residual is not None else 2), x.data_ptr(), x_ld,
-                 _p(residual), r_ld, _p(gamma), _p(beta), z.data_ptr(), z_ld, stats.data_ptr(), dt, n, h * w, c, groups, eps, act, slope,
-                 ws.data_ptr(), ws_bytes)
-        # without an activation the residual's gradient is dz itself and nothing depends on the residual's values
-        ctx.save_for_backward(x, gamma, beta, residual if act != _lib.ACT_NONE else None, stats)
-        ctx.args = (x_ld, r_ld, dt, n, h * w, c, groups, act, slope)
-        ctx.has_res = residual is not None
-        return z
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dz):
-        x, gamma, beta, residual, stats = ctx.saved_tensors
-        x_ld, r_ld, dt, n, hw, c, groups, act, slope = ctx.args
-        need_x, need_gamma, need_beta, need_res = ctx.needs_input_grad[:4]
-        if residual is None and not (need_x or need_gamma or need_beta):
-            return None, None, None, dz, None, None, None, None, None
-        dev = x.device
-        dz_ld = _pitch(dz) if dz.dtype == x.dtype else 0
-        if not dz_ld:
-            dz, dz_ld = (_g(dz) if dz.dtype == x.dtype else to_nhwc_raw(dz, x.dtype)), c
-        need_dres = residual is not None and need_res
-        dx = torch.empty_like(x, memory_format=CL) if (need_x or need_dres) else None
-        dres = torch.empty_like(x, memory_format=CL) if need_dres else None
-        dgamma = grad_buffer(gamma) if need_gamma else None
-        dbeta = grad_buffer(beta) if need_beta else None
-        ws_bytes = query("ur_gn_bwd_workspace", dt, n, hw, c, groups)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-        _gn_call("ur_gn_act_bwd", dev, "hbm:gn_bwd", x.numel() * x.element_size() * (2 + (dx is not None) + (residual is not None) + need_dres),
-                 dz.data_ptr(), dz_ld, x.data_ptr(), x_ld, _p(residual), r_ld, _p(gamma), _p(beta), stats.data_ptr(), _p(dx), _p(dres),
-                 _p(dgamma), _p(dbeta), dt, n, hw, c, groups, act, slope, ws.data_ptr(), ws_bytes)
-        if ctx.has_res and residual is None and need_res:
-            dres = dz                                # no activation: d residual = dz
-        return dx if need_x else None, dgamma, dbeta, dres, None, None, None, None, None
-
-
 def gn_act(x, gn, residual=None, act=_lib.ACT_RELU, slope=0.0, out=None):
     """GroupNorm module `gn` (torch.nn.GroupNorm or nn.GroupNorm) applied to x, fused with an optional residual add and an
     activation (_lib.ACT_*, ACT_SILU included; `slope` for ACT_LEAKYRELU): act(gn(x) + residual).
 
-    x: NCHW-shaped, bf16 or fp32, channels last or a channel window of a wider channels-last
-    tensor (other layouts are converted first); residual: x's shape and dtype.  out: optional channel window (alias_window)
-    to write the result into.  Training and evaluation are the same computation.  A group of one value normalises to zero.
-    Gradients flow to x, the module's weight and bias and the residual, once (no double backward)."""
-    if not 0 <= act <= _lib.ACT_SILU:
-        raise ValueError("gn_act: unknown activation code %r" % (act,))
-    if x.dim() != 4:
-        raise ValueError("gn_act: expected a 4-D NCHW tensor, got shape %s" % (tuple(x.shape),))
-    _require_gpu(x)
-    _dt(x)
-    c = x.shape[1]
-    if c != gn.num_channels:
-        raise RuntimeError("gn_act: %d channels, the GroupNorm has %d" % (c, gn.num_channels))
-    if 0 in x.shape:
-        raise _lib.UResNetHipError("gn_act: non-positive size in shape %s" % (tuple(x.shape),))
-    for name, p in (("weight", gn.weight), ("bias", gn.bias)):
-        if p is not None and (p.dtype != torch.float32 or p.device != x.device or not p.is_contiguous()):
-            raise _lib.UResNetHipError("gn_act: the GroupNorm's %s must be a contiguous fp32 tensor on %s" % (name, x.device))
-    with _on(x.device):
-        if not _pitch(x):
-            x = as_activation(x, x.dtype, allow_window=True)
-        if residual is not None:
-            if residual.shape != x.shape or residual.device != x.device:
-                raise RuntimeError("gn_act: the residual is %s on %s, expected %s on %s"
-                                   % (tuple(residual.shape), residual.device, tuple(x.shape), x.device))
-            residual = as_activation(residual, x.dtype, allow_window=True)
-    return _GNAct.apply(x, gn.weight, gn.bias, residual, gn.num_groups, float(gn.eps), int(act), float(slope),
-                        None if out is None else (out,))
+    x: NCHW-shaped, bf16 or fp32, channels last or a channel window of a wider channels-last tensor (other layouts are
+    converted first); residual: x's shape and dtype.  out: optional channel window (alias_window) to write the result into.
+    Training and evaluation are the same computation.  A group of one value normalises to zero.  Gradients flow to x, the
+    module's weight and bias and the residual, once: a backward pass with create_graph=True is refused.
+
+    The tape node lives in the host module (csrc/host/gn_function.cpp): it saves x, the residual (where an activation needs
+    the sum) and the fp64 {mean, rstd} of every image and group, and recomputes the pre-activation from them."""
+    if x.is_cuda and x.dim() == 4 and x.dtype in _DT:
+        if not _pitch(x) and x.numel():
+            with _on(x.device):
+                x = as_activation(x, x.dtype, allow_window=True)
+        if residual is not None and residual.is_cuda and residual.shape == x.shape and not _pitch(residual) and x.numel():
+            with _on(x.device):
+                residual = as_activation(residual, x.dtype, allow_window=True)
+    return _lib.host().gn_act(x, gn.weight, gn.bias, residual, out, gn.num_groups, gn.num_channels, gn.eps, act, slope)
 
 
 fuse_bn_into_conv1x1 = os.environ.get("URESNET_BN_PW", "1") != "0"   # False: BatchNorm+ReLU and the 1x1 convolution stay separate

@@ -302,7 +302,7 @@ class SGD(_MultiTensorOptimizer):
 
 
 class _ParamList:
-    """Tensors of one launch: addresses and sizes as int64 arrays in host memory (_lib.param_list()), their table and, where
+    """Tensors of one launch: addresses and sizes as int64 arrays in host memory (_lib.host()), their table and, where
     the norm is taken, room for its partial sums in device memory."""
     PARTS = 1024                                 # ur_grad_sqnorm_max_parts()
 
@@ -337,7 +337,7 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     max_norm = float(max_norm)
     if not max_norm >= 0:
         raise ValueError("clip_grad_norm_: max_norm must not be negative (got %r)" % (max_norm,))
-    grads, sizes, count, index = _lib.param_list().clip_rows([parameters] if torch.is_tensor(parameters) else list(parameters))
+    grads, sizes, count, index = _lib.host().clip_rows([parameters] if torch.is_tensor(parameters) else list(parameters))
     if index < 0:
         return torch.tensor(0.0)
     device = torch.device("cuda", index)
@@ -478,7 +478,7 @@ class AdamW(torch.optim.Optimizer):
         for gi, group in enumerate(self.param_groups):
             if not group['params']:
                 continue
-            pool, rows = self._pool(gi, group), _lib.param_list().adamw_rows
+            pool, rows = self._pool(gi, group), _lib.host().adamw_rows
             params, grads, live, uneven = rows(pool.params, pool.sizes, None)
             held = None
             if uneven:                                         # copies, until the launches that read them are queued
