@@ -499,6 +499,7 @@ int ur_sgd_multi(const void* const* ptrs, const long long* sizes, int ntensors, 
  *      fp32 scale per block.
  *   or ur_grad_clip scales the gradients in place.
  * Parameters and gradients are dense fp32; tensors of a list must not overlap. */
+int ur_param_table_max_rows(void); /* tensors per table; longer lists take several */
 size_t ur_param_table_bytes(int ntensors);
 int ur_param_table(const long long* params, const long long* grads, const long long* sizes, const long long* blocks, int ntensors,
                    void* table, size_t table_bytes, int* steps, double lr, double beta1, double beta2, long long* nchunks,

@@ -120,6 +120,9 @@ def test_entry_points_refuse_before_any_launch():
         with pytest.raises(_lib.UResNetHipError, match="param_table"):
             table(**kw)
     assert _lib.query("ur_grad_sqnorm_max_parts") == train._ParamList.PARTS
+    assert _lib.query("ur_param_table_max_rows") == train._ParamList.ROWS
+    with pytest.raises(_lib.UResNetHipError, match="more than"):
+        table(grads=(16,) * 1025, sizes=(1,) * 1025)
     def adamw(bits=32, m=16, scale=16, chunks=1, nparts=0, parts=None):
         _lib.call("ur_adamw_multi", 16, 1, chunks, bits, m, 16, scale, scale, 1e-3, 0.9, 0.999, 1e-8, 0.0, parts, nparts, 1.0, 1.0, None, None)
     for kw in (dict(bits=16), dict(m=None), dict(m=24), dict(bits=8, scale=None), dict(chunks=0), dict(nparts=3)):
@@ -361,7 +364,7 @@ def test_clipping_with_a_nan_or_infinite_norm_follows_torch():
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("sizes", [SIZES, [(1,)], [(40001,)] * 3, [(7,)] * 200, [(1 << 22,), (5,)]])
+@pytest.mark.parametrize("sizes", [SIZES, [(1,)], [(40001,)] * 3, [(7,)] * 200, [(1 << 22,), (5,)], [(5,)] * 2500])
 @pytest.mark.parametrize("limit", [0.25, 1e9])
 def test_clip_grad_norm(sizes, limit):
     grads = tensors(6, sizes, 1.0)
@@ -425,10 +428,11 @@ def test_unaligned_views_channels_last_gradients_and_refused_layouts():
 def test_groups_late_parameters_and_many_tensors(bits):
     """More tensors than one table launch takes, groups of their own constants under one norm, parameters without gradients,
     counts per parameter."""
-    vals = tensors(8, [(17 + i,) for i in range(200)])
-    grads = tensors(9, [(17 + i,) for i in range(200)], 0.5)
+    count, cut = 1500, 1300
+    vals = tensors(8, [(17 + i % 400,) for i in range(count)])
+    grads = tensors(9, [(17 + i % 400,) for i in range(count)], 0.5)
     ps = params_on_gpu(vals, [None if i % 3 == 1 else g for i, g in enumerate(grads)])
-    opt = train.AdamW([{"params": ps[:150], "lr": 1e-2, "state_bits": bits}, {"params": ps[150:], "lr": 1e-3, "weight_decay": 0.0}],
+    opt = train.AdamW([{"params": ps[:cut], "lr": 1e-2, "state_bits": bits}, {"params": ps[cut:], "lr": 1e-3, "weight_decay": 0.0}],
                       weight_decay=0.1, max_grad_norm=0.75)
     opt.grad_scale = 0.5
     opt.step()
@@ -439,7 +443,7 @@ def test_groups_late_parameters_and_many_tensors(bits):
         if i % 3 == 1:
             assert torch.equal(p.detach().cpu(), v) and p not in opt.state
             continue
-        lr, wd = (1e-2, 0.1) if i < 150 else (1e-3, 0.0)
+        lr, wd = (1e-2, 0.1) if i < cut else (1e-3, 0.0)
         zero = torch.zeros(v.shape)
         want, _, _, upd = reference_step(v, g, zero, zero, 1, lr, 0.9, 0.999, 1e-8, wd, factor)
         within(p, want, 4 * E24 * want.abs() + 32 * E24 * upd, "p")

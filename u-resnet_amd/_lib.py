@@ -150,6 +150,7 @@ SIGNATURES = {
     "ur_adam_multi": (_i, [_vp, _vp, _i, _ll, _f, _f, _f, _f, _f, _i, _f, _vp]),
     "ur_adam_multi_dev": (_i, [_vp, _vp, _i, _ll, _f, _f, _f, _f, _f, _f, _vp]),
     "ur_sgd_multi": (_i, [_vp, _vp, _i, _ll, _f, _f, _f, _vp]),
+    "ur_param_table_max_rows": (_i, []),
     "ur_param_table_bytes": (_sz, [_i]),
     "ur_param_table": (_i, [_vp, _vp, _vp, _vp, _i, _vp, _sz, _vp, _d, _d, _d, _vp, _vp]),
     "ur_grad_sqnorm_max_parts": (_i, []),

@@ -305,6 +305,12 @@ class _ParamList:
     """Tensors of one launch: addresses and sizes as int64 arrays in host memory (_lib.host()), their table and, where
     the norm is taken, room for its partial sums in device memory."""
     PARTS = 1024                                 # ur_grad_sqnorm_max_parts()
+    ROWS = 1024                                  # ur_param_table_max_rows()
+
+    @classmethod
+    def spans(cls, count):
+        """Slices of a list of `count` tensors that fit a table, as byte offsets into its int64 arrays and the first index."""
+        return [(slice(8 * a, 8 * min(a + cls.ROWS, count)), a) for a in range(0, count, cls.ROWS)]
 
     def __init__(self, params, grads, sizes, device, parts=0):
         self.params, self.grads, self.sizes, self.count = params, grads, sizes, len(sizes) // 8
@@ -346,14 +352,19 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
             return torch.zeros((), device=device)
         stream = ops._stream()
         norm = torch.empty((), device=device)
-        plist = _ParamList(None, grads, sizes, device, _ParamList.PARTS)
-        plist.write(stream)
-        nparts = plist.sqnorm(plist.parts, stream)
+        spans = _ParamList.spans(count)
+        lists, nparts = [], 0
+        for span, _ in spans:
+            plist = _ParamList(None, grads[span], sizes[span], device, 0 if lists else _ParamList.PARTS * len(spans))
+            plist.write(stream)
+            lists.append(plist)
+            nparts += plist.sqnorm(lists[0].parts + 8 * nparts, stream)
         if error_if_nonfinite:
-            total = plist.buf[plist.bytes:plist.bytes + 8 * nparts].view(torch.float64).sum()
+            total = lists[0].buf[lists[0].bytes:lists[0].bytes + 8 * nparts].view(torch.float64).sum()
             if not bool(torch.isfinite(total)):
                 raise RuntimeError("clip_grad_norm_: the total norm of the gradients is not finite")
-        _lib.call("ur_grad_clip", plist.table, plist.count, plist.chunks, plist.parts, nparts, max_norm, norm.data_ptr(), stream)
+        for plist in lists:
+            _lib.call("ur_grad_clip", plist.table, plist.count, plist.chunks, lists[0].parts, nparts, max_norm, norm.data_ptr(), stream)
     return norm
 
 
@@ -505,15 +516,17 @@ class AdamW(torch.optim.Optimizer):
         stream = ops._stream()
         clip = self.max_grad_norm is not None
         lists, parts, nparts, norm = [], None, 0, None
-        for group, pool, params, grads, _ in work:
-            plist = _ParamList(params, grads, pool.sizes, dev, _ParamList.PARTS * len(work) if clip and not lists else 0)
-            plist.write(stream, pool.blocks_there.data_ptr(), pool.steps.data_ptr(), float(group['lr']), group['betas'])
+        work = [(group, pool, params[span], grads[span], pool.sizes[span], at) for group, pool, params, grads, _ in work
+                for span, at in _ParamList.spans(len(pool.params)) if any(grads[span])]
+        for group, pool, params, grads, sizes, at in work:
+            plist = _ParamList(params, grads, sizes, dev, _ParamList.PARTS * len(work) if clip and not lists else 0)
+            plist.write(stream, pool.blocks_there.data_ptr() + 8 * at, pool.steps.data_ptr() + 4 * at, float(group['lr']), group['betas'])
             lists.append(plist)
         if clip:
             norm, parts = torch.empty((), device=dev), lists[0].parts
             for plist in lists:
                 nparts += plist.sqnorm(parts + 8 * nparts, stream)
-        for (group, pool, _, _, _), plist in zip(work, lists):
+        for (group, pool, *_), plist in zip(work, lists):
             buf = pool.buffers
             if pool.bits == 32:
                 state = (buf['exp_avg'].data_ptr(), buf['exp_avg_sq'].data_ptr(), None, None)
