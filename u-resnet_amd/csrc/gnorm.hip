@@ -24,37 +24,60 @@ namespace {
 constexpr int NT = 256;
 
 typedef __attribute__((ext_vector_type(4))) float fvec4_t;
+typedef __attribute__((ext_vector_type(4))) unsigned uvec4_t;
 
-// V consecutive channels of one pixel: 16 bytes (8 bf16, 4 fp32) or one element
+// V consecutive channels of one pixel: 16 bytes (8 bf16, 4 fp32) or one element.  bf16 vectors are kept as four words: the
+// compiler spreads a bf16 vector that lives across branches over eight registers.  forget(): the compiler no longer knows
+// what it computed from the vector, so that it does not keep unpacked copies of data that waits in registers.
 template <typename T, int V> struct Chunk;
 template <> struct Chunk<bf16_t, 8> {
-    bf16x8_t d;
-    __device__ __forceinline__ void load(const bf16_t* p) { d = __builtin_nontemporal_load(reinterpret_cast<const bf16x8_t*>(p)); }
-    __device__ __forceinline__ void store(bf16_t* p) const { __builtin_nontemporal_store(d, reinterpret_cast<bf16x8_t*>(p)); }
-    __device__ __forceinline__ float get(int i) const { return (float)d[i]; }
-    __device__ __forceinline__ void set(int i, float v) { d[i] = (bf16_t)v; }
+    uvec4_t d;
+    __device__ __forceinline__ void load(const bf16_t* p) { d = __builtin_nontemporal_load(reinterpret_cast<const uvec4_t*>(p)); }
+    __device__ __forceinline__ void store(bf16_t* p) const { __builtin_nontemporal_store(d, reinterpret_cast<uvec4_t*>(p)); }
+    __device__ __forceinline__ float get(int i) const { return __uint_as_float(i & 1 ? d[i >> 1] & 0xffff0000u : d[i >> 1] << 16); }
+    __device__ __forceinline__ void put(const float (&v)[8]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const bf16x2_t w = {(bf16_t)v[2 * i], (bf16_t)v[2 * i + 1]};
+            d[i] = __builtin_bit_cast(unsigned, w);
+        }
+    }
+    __device__ __forceinline__ void forget() { asm volatile("" : "+v"(d)); }
 };
 template <> struct Chunk<float, 4> {
     fvec4_t d;
     __device__ __forceinline__ void load(const float* p) { d = __builtin_nontemporal_load(reinterpret_cast<const fvec4_t*>(p)); }
     __device__ __forceinline__ void store(float* p) const { __builtin_nontemporal_store(d, reinterpret_cast<fvec4_t*>(p)); }
     __device__ __forceinline__ float get(int i) const { return d[i]; }
-    __device__ __forceinline__ void set(int i, float v) { d[i] = v; }
+    __device__ __forceinline__ void put(const float (&v)[4]) { d = fvec4_t{v[0], v[1], v[2], v[3]}; }
+    __device__ __forceinline__ void forget() { asm volatile("" : "+v"(d)); }
 };
 template <typename T> struct Chunk<T, 1> {
     T d;
     __device__ __forceinline__ void load(const T* p) { d = *p; }
     __device__ __forceinline__ void store(T* p) const { *p = d; }
     __device__ __forceinline__ float get(int) const { return ur_to_float(d); }
-    __device__ __forceinline__ void set(int, float v) { d = ur_from_float<T>(v); }
+    __device__ __forceinline__ void put(const float (&v)[1]) { d = ur_from_float<T>(v[0]); }
 };
 
 // ------------------------------------------------------------------ activations
+// Phi(p) = (1 + erf(p / sqrt 2)) / 2 and e = exp(-p^2 / 2): Abramowitz and Stegun 7.1.26, off by at most 0.75e-7, without the
+// branches of erff (they cost registers in unrolled loops) and with the exponential that the derivative needs as well
+__device__ __forceinline__ float gn_phi(float p, float& e) {
+    const float z = fabsf(p) * 0.70710678118654752f, t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, z, 1.f));
+    float s = fmaf(t, 1.061405429f, -1.453152027f);
+    s = fmaf(t, s, 1.421413741f);
+    s = fmaf(t, s, -0.284496736f);
+    s = fmaf(t, s, 0.254829592f);
+    e = __expf(-0.5f * p * p);
+    const float tail = 0.5f * t * s * e;
+    return p < 0.f ? tail : 1.f - tail;
+}
 template <int ACT> __device__ __forceinline__ float gn_act(float p, float slope) {
     if constexpr (ACT == UR_ACT_RELU) return p <= 0.f ? 0.f : p;                       // (NaN stays NaN)
     if constexpr (ACT == UR_ACT_RELU6) return p <= 0.f ? 0.f : (p >= 6.f ? 6.f : p);
     if constexpr (ACT == UR_ACT_LEAKYRELU) return p > 0.f ? p : p * slope;
-    if constexpr (ACT == UR_ACT_GELU) return 0.5f * p * (1.f + erff(p * 0.70710678118654752f));
+    if constexpr (ACT == UR_ACT_GELU) { float e; return p * gn_phi(p, e); }
     if constexpr (ACT == UR_ACT_HSWISH) return p <= -3.f ? 0.f : (p >= 3.f ? p : p * (p + 3.f) * (1.f / 6.f));
     if constexpr (ACT == UR_ACT_SILU) return p * __builtin_amdgcn_rcpf(1.f + __expf(-p));
     return p;
@@ -65,8 +88,7 @@ template <int ACT, typename F> __device__ __forceinline__ float gn_act_grad(F p,
     if constexpr (ACT == UR_ACT_LEAKYRELU) return p > (F)0 ? 1.f : slope;
     if constexpr (ACT == UR_ACT_HSWISH) return p <= (F)-3 ? 0.f : (p < (F)3 ? (2.f * (float)p + 3.f) * (1.f / 6.f) : 1.f);
     const float q = (float)p;
-    if constexpr (ACT == UR_ACT_GELU)
-        return 0.5f * (1.f + erff(q * 0.70710678118654752f)) + q * 0.3989422804014327f * __expf(-0.5f * q * q);
+    if constexpr (ACT == UR_ACT_GELU) { float e; const float c = gn_phi(q, e); return fmaf(q * 0.3989422804014327f, e, c); }
     if constexpr (ACT == UR_ACT_SILU) {
         const float s = __builtin_amdgcn_rcpf(1.f + __expf(-q));
         return s * (1.f + q * (1.f - s));
@@ -153,21 +175,23 @@ template <int V> struct Affine {
 
 template <typename T, int V, int ACT, bool RES>
 __device__ __forceinline__ Chunk<T, V> fwd_vector(const Affine<V>& k, const Chunk<T, V>& v, const Chunk<T, V>& w, float slope) {
-    Chunk<T, V> o;
+    float z[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         float p = fmaf(v.get(i) - k.m[i], k.a[i], k.b[i]);
         if constexpr (RES) p += w.get(i);
-        o.set(i, gn_act<ACT>(p, slope));
+        z[i] = gn_act<ACT>(p, slope);
     }
+    Chunk<T, V> o;
+    o.put(z);
     return o;
 }
 
-// g = dy * act'(pre) of a vector, d = x - mean_hi.  One branch per vector decides whether any element lies near a kink.
+// g = dy * act'(pre) of a vector, d = x - mean_hi; returns whether an element lies near a kink.  Then the caller corrects
+// the vector with settle().
 template <typename T, int V, int ACT, bool RES>
-__device__ __forceinline__ void bwd_vector(const Affine<V>& k, const Chunk<T, V>& u, const Chunk<T, V>& v, const Chunk<T, V>& w, float slope,
-                                           const double* stats, int g0, const float* __restrict__ gamma, const float* __restrict__ beta,
-                                           int col, int per, float (&g)[V], float (&d)[V]) {
+__device__ __forceinline__ bool bwd_vector(const Affine<V>& k, const Chunk<T, V>& u, const Chunk<T, V>& v, const Chunk<T, V>& w, float slope,
+                                           float (&g)[V], float (&d)[V]) {
     bool near = false;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -177,21 +201,19 @@ __device__ __forceinline__ void bwd_vector(const Affine<V>& k, const Chunk<T, V>
         near |= gn_near_kink<ACT>(p, size);
         g[i] = u.get(i) * gn_act_grad<ACT, float>(p, slope);
     }
-    if constexpr (ACT == UR_ACT_RELU || ACT == UR_ACT_LEAKYRELU || ACT == UR_ACT_RELU6 || ACT == UR_ACT_HSWISH) {
-        if (near) {
+    return near;
+}
+template <typename T, int V, int ACT, bool RES>
+__device__ __forceinline__ void settle(const T* dy, const T* x, const T* res, float slope, const double* stats, int g0,
+                                       const float* __restrict__ gamma, const float* __restrict__ beta, int col, int per, float (&g)[V]) {
 #pragma unroll 1
-            for (int i = 0; i < V; ++i) {
-                const double* st = stats + ((col + i) / per - g0) * 2;
-                const double ga = gamma ? (double)gamma[col + i] : 1.0, be = beta ? (double)beta[col + i] : 0.0;
-                float xv = 0.f, uv = 0.f, wv = 0.f;
+    for (int i = 0; i < V; ++i) {                          // (read again, one by one: few registers)
+        const double* st = stats + ((col + i) / per - g0) * 2;
+        double e = ((double)ur_to_float(x[i]) - st[0]) * st[1] * (gamma ? (double)gamma[col + i] : 1.0) + (beta ? (double)beta[col + i] : 0.0);
+        if constexpr (RES) e += (double)ur_to_float(res[i]);
+        const float exact = ur_to_float(dy[i]) * gn_act_grad<ACT, double>(e, slope);
 #pragma unroll
-                for (int j = 0; j < V; ++j) if (j == i) { xv = v.get(j); uv = u.get(j); if constexpr (RES) wv = w.get(j); }
-                const double e = ((double)xv - st[0]) * st[1] * ga + be + (double)wv;
-                const float r = uv * gn_act_grad<ACT, double>(e, slope);
-#pragma unroll
-                for (int j = 0; j < V; ++j) if (j == i) g[j] = r;
-            }
-        }
+        for (int j = 0; j < V; ++j) g[j] = j == i ? exact : g[j];
     }
 }
 
@@ -321,6 +343,7 @@ _Pragma("unroll")
             if (r < s.hw) {
                 Chunk<T, V> w;
                 if constexpr (RES) w.load(rp + (size_t)r * res_ld);
+                v[j].forget();
                 fwd_vector<T, V, ACT, RES>(k, v[j], w, slope).store(yp + (size_t)r * y_ld);
             }
         }
@@ -364,7 +387,8 @@ _Pragma("unroll")
                 const int r = at.slot + j * at.slots;
                 if (r < s.hw) {
                     if constexpr (RES) w.load(rp + (size_t)r * res_ld);
-                    bwd_vector<T, V, ACT, RES>(k, u[j], v[j], w, slope, st0, g0, gamma, beta, at.col, s.k, g, d);
+                    if (bwd_vector<T, V, ACT, RES>(k, u[j], v[j], w, slope, g, d))
+                        settle<T, V, ACT, RES>(gp + (size_t)r * dy_ld, xp + (size_t)r * ld, RES ? rp + (size_t)r * res_ld : nullptr, slope, st0, g0, gamma, beta, at.col, s.k, g);
 _Pragma("unroll")
                     for (int i = 0; i < V; ++i) { s1[i] += g[i]; s2[i] = fmaf(g[i], d[i], s2[i]); }
                 }
@@ -420,9 +444,14 @@ _Pragma("unroll")
             if (r < s.hw) {
                 Chunk<T, V> o, t;
                 if constexpr (RES) w.load(rp + (size_t)r * res_ld);
-                bwd_vector<T, V, ACT, RES>(k, u[j], v[j], w, slope, st0, g0, gamma, beta, at.col, s.k, g, d);
+                u[j].forget();
+                v[j].forget();
+                if (bwd_vector<T, V, ACT, RES>(k, u[j], v[j], w, slope, g, d))
+                    settle<T, V, ACT, RES>(gp + (size_t)r * dy_ld, xp + (size_t)r * ld, RES ? rp + (size_t)r * res_ld : nullptr, slope, st0, g0, gamma, beta, at.col, s.k, g);
 _Pragma("unroll")
-                for (int i = 0; i < V; ++i) { o.set(i, fmaf(g[i], k.a[i], fmaf(d[i], k2[i], k1[i]))); t.set(i, g[i]); }
+                for (int i = 0; i < V; ++i) d[i] = fmaf(g[i], k.a[i], fmaf(d[i], k2[i], k1[i]));
+                o.put(d);
+                t.put(g);
                 o.store(op + (size_t)r * s.c);
                 if constexpr (RES) { if (qp) t.store(qp + (size_t)r * s.c); }
             }
@@ -455,6 +484,8 @@ __global__ __launch_bounds__(NT) void gn_params_kernel(const double* __restrict_
 // ================================================================== streaming passes
 // Large sizes: two passes over memory with the sums of all workgroups between them.
 constexpr int UNR = 4, SUNR = 8;                           // pixels in flight per thread; in the statistics
+// keeps the scheduler from interleaving the vectors of an unrolled loop, which costs registers and so waves
+#define VECTOR_DONE() __builtin_amdgcn_sched_barrier(0)
 
 // SPAN: channels of a vector that share a group (a power of two that divides both V and k): V / SPAN pairs of sums per thread
 template <typename T, int V, int SPAN>
@@ -570,14 +601,23 @@ __global__ __launch_bounds__(NT) void gn_bwd_reduce_kernel(const T* __restrict__
         const T* gp = dy + (size_t)n * s.hw * dy_ld + at.col;
         const T* xp = x + (size_t)n * s.hw * ld + at.col;
         const T* rp = RES ? res + (size_t)n * s.hw * res_ld + at.col : nullptr;
-        const auto add = [&](const Chunk<T, V>& u, const Chunk<T, V>& v, const Chunk<T, V>& w) {
-            float g[V], d[V];
-            bwd_vector<T, V, ACT, RES>(k, u, v, w, slope, st0, 0, gamma, beta, at.col, s.k, g, d);
+        const auto add = [&](const float (&g)[V], const float (&d)[V]) {
 #pragma unroll
             for (int i = 0; i < V; ++i) { s1[i] += g[i]; s2[i] = fmaf(g[i], d[i], s2[i]); }
         };
+        const auto one = [&](long long r) {
+            Chunk<T, V> u, v, w;
+            float g[V], d[V];
+            u.load(gp + (size_t)r * dy_ld);
+            v.load(xp + (size_t)r * ld);
+            if constexpr (RES) w.load(rp + (size_t)r * res_ld);
+            if (bwd_vector<T, V, ACT, RES>(k, u, v, w, slope, g, d))
+                settle<T, V, ACT, RES>(gp + (size_t)r * dy_ld, xp + (size_t)r * ld, RES ? rp + (size_t)r * res_ld : nullptr, slope, st0, 0, gamma, beta, at.col, s.k, g);
+            add(g, d);
+        };
         at.walk<UNR>(s, [&](long long r) {
             Chunk<T, V> u[UNR], v[UNR], w[UNR];
+            unsigned near = 0;
 #pragma unroll
             for (int j = 0; j < UNR; ++j) {
                 u[j].load(gp + (size_t)(r + j * at.slots) * dy_ld);
@@ -585,14 +625,17 @@ __global__ __launch_bounds__(NT) void gn_bwd_reduce_kernel(const T* __restrict__
                 if constexpr (RES) w[j].load(rp + (size_t)(r + j * at.slots) * res_ld);
             }
 #pragma unroll
-            for (int j = 0; j < UNR; ++j) add(u[j], v[j], w[j]);
-        }, [&](long long r) {
-            Chunk<T, V> u, v, w;
-            u.load(gp + (size_t)r * dy_ld);
-            v.load(xp + (size_t)r * ld);
-            if constexpr (RES) w.load(rp + (size_t)r * res_ld);
-            add(u, v, w);
-        });
+            for (int j = 0; j < UNR; ++j) {
+                float g[V], d[V];
+                const bool skip = bwd_vector<T, V, ACT, RES>(k, u[j], v[j], w[j], slope, g, d);
+                near |= (unsigned)skip << j;
+#pragma unroll
+                for (int i = 0; i < V; ++i) g[i] = skip ? 0.f : g[i];
+                add(g, d);
+                VECTOR_DONE();
+            }
+            for (; near; near &= near - 1) one(r + __builtin_ctz(near) * at.slots);        // rare
+        }, one);
     }
 #pragma unroll
     for (int i = 0; i < V; ++i) { red[2 * i][threadIdx.x] = s1[i]; red[2 * i + 1][threadIdx.x] = s2[i]; }
@@ -684,17 +727,27 @@ __global__ __launch_bounds__(NT) void gn_bwd_apply_kernel(const T* __restrict__ 
     const T* rp = RES ? res + (size_t)n * s.hw * res_ld + at.col : nullptr;
     T* op = dx + (size_t)n * s.hw * s.c + at.col;
     T* qp = RES && dres ? dres + (size_t)n * s.hw * s.c + at.col : nullptr;
-    const auto one = [&](const Chunk<T, V>& u, const Chunk<T, V>& v, const Chunk<T, V>& w, long long row) {
-        float g[V], d[V];
-        bwd_vector<T, V, ACT, RES>(k, u, v, w, slope, st0, 0, gamma, beta, at.col, s.k, g, d);
+    const auto write = [&](float (&g)[V], float (&d)[V], long long row) {
         Chunk<T, V> o, t;
 #pragma unroll
-        for (int i = 0; i < V; ++i) { o.set(i, fmaf(g[i], k.a[i], fmaf(d[i], k2[i], k1[i]))); t.set(i, g[i]); }
+        for (int i = 0; i < V; ++i) d[i] = fmaf(g[i], k.a[i], fmaf(d[i], k2[i], k1[i]));
+        o.put(d);
         o.store(op + (size_t)row * s.c);
-        if constexpr (RES) { if (qp) t.store(qp + (size_t)row * s.c); }
+        if constexpr (RES) { if (qp) { t.put(g); t.store(qp + (size_t)row * s.c); } }
+    };
+    const auto one = [&](long long r) {
+        Chunk<T, V> u, v, w;
+        float g[V], d[V];
+        u.load(gp + (size_t)r * dy_ld);
+        v.load(xp + (size_t)r * ld);
+        if constexpr (RES) w.load(rp + (size_t)r * res_ld);
+        if (bwd_vector<T, V, ACT, RES>(k, u, v, w, slope, g, d))
+            settle<T, V, ACT, RES>(gp + (size_t)r * dy_ld, xp + (size_t)r * ld, RES ? rp + (size_t)r * res_ld : nullptr, slope, st0, 0, gamma, beta, at.col, s.k, g);
+        write(g, d, r);
     };
     at.walk<UNR>(s, [&](long long r) {
         Chunk<T, V> u[UNR], v[UNR], w[UNR];
+        unsigned near = 0;
 #pragma unroll
         for (int j = 0; j < UNR; ++j) {
             u[j].load(gp + (size_t)(r + j * at.slots) * dy_ld);
@@ -702,14 +755,14 @@ __global__ __launch_bounds__(NT) void gn_bwd_apply_kernel(const T* __restrict__ 
             if constexpr (RES) w[j].load(rp + (size_t)(r + j * at.slots) * res_ld);
         }
 #pragma unroll
-        for (int j = 0; j < UNR; ++j) one(u[j], v[j], w[j], r + j * at.slots);
-    }, [&](long long r) {
-        Chunk<T, V> u, v, w;
-        u.load(gp + (size_t)r * dy_ld);
-        v.load(xp + (size_t)r * ld);
-        if constexpr (RES) w.load(rp + (size_t)r * res_ld);
-        one(u, v, w, r);
-    });
+        for (int j = 0; j < UNR; ++j) {
+            float g[V], d[V];
+            near |= (unsigned)bwd_vector<T, V, ACT, RES>(k, u[j], v[j], w[j], slope, g, d) << j;
+            write(g, d, r + j * at.slots);
+            VECTOR_DONE();
+        }
+        for (; near; near &= near - 1) one(r + __builtin_ctz(near) * at.slots);            // rare: written again
+    }, one);
 }
 
 // ------------------------------------------------------------------ host
@@ -768,6 +821,8 @@ Cell make_cell(int dtype, int n, long long hw, int c, int groups, bool vec, int 
 }
 int cell_vectors(const Cell& s, int v) { const int slots = CT / (s.slab / v); return (s.hw + slots - 1) / slots; }
 
+constexpr int FWD_MOST = 16, BWD_MOST = 8;              // vectors (pairs of vectors) per thread of a cell
+
 bool aligned(const void* p, int dtype, long long ld) { return p == nullptr || ((((uintptr_t)p) & 15) == 0 && ld % (dtype == UR_BF16 ? 8 : 4) == 0); }
 
 template <typename T, int V>
@@ -807,7 +862,6 @@ void launch_stats(const void* x, int ld, const Plan& p, int n, double* partial, 
         else if ((k) <= 8) { constexpr int K = 8; __VA_ARGS__; }                           \
         else { constexpr int K = 16; __VA_ARGS__; }                                        \
     } while (0)
-constexpr int FWD_MOST = 16, BWD_MOST = 8;
 
 int check(const char* what, int dtype, int n, long long hw, int c, int groups, int act) {
     UR_REQUIRE(dtype == UR_F32 || dtype == UR_BF16, "%s: bad dtype %d", what, dtype);
