@@ -58,6 +58,7 @@ template <typename T> struct Chunk<T, 1> {
     __device__ __forceinline__ void store(T* p) const { *p = d; }
     __device__ __forceinline__ float get(int) const { return ur_to_float(d); }
     __device__ __forceinline__ void put(const float (&v)[1]) { d = ur_from_float<T>(v[0]); }
+    __device__ __forceinline__ void forget() {}
 };
 
 // ------------------------------------------------------------------ activations
@@ -126,14 +127,23 @@ struct Place {
         col = (blockIdx.z * s.cqb + cg) * V;
         active = slot < slots && col < s.c;
     }
-    // full(r): U pixels r, r + slots, ...; one(r): a single pixel (the end of the image)
-    template <int U, typename Full, typename One>
-    __device__ __forceinline__ void walk(const GnShape& s, const Full& full, const One& one) const {
+    // load(r) and full(r): U pixels r, r + slots, ...; once(): what full and one need besides, while the first loads are on
+    // their way; one(r): a single pixel (the end of the image)
+    template <int U, typename Load, typename Once, typename Full, typename One>
+    __device__ __forceinline__ void walk(const GnShape& s, const Load& load, const Once& once, const Full& full, const One& one) const {
         const long long step = (long long)s.chunks * U * slots;
-        for (long long r = (long long)blockIdx.x * U * slots + slot; r < s.hw; r += step) {
-            if (r + (U - 1) * slots < s.hw) full(r);
-            else for (long long q = r; q < s.hw; q += slots) one(q);
+        long long r = (long long)blockIdx.x * U * slots + slot;
+        bool whole = r + (U - 1) * slots < s.hw;
+        if (whole) load(r);
+        __builtin_amdgcn_sched_barrier(0);
+        once();
+        while (whole) {
+            full(r);
+            r += step;
+            whole = r + (U - 1) * slots < s.hw;
+            if (whole) load(r);
         }
+        for (; r < s.hw; r += slots) one(r);
     }
 };
 
@@ -157,14 +167,22 @@ __device__ __forceinline__ void mean_rstd(double a, double q, double count, floa
     rstd = 1.0 / sqrt(var + (double)eps);
 }
 
+// the group of a channel and of those after it, with one division
+struct GroupOf {
+    int g, left, k;
+    __device__ __forceinline__ GroupOf(int c, int k_) : g(c / k_), left((g + 1) * k_ - c), k(k_) {}
+    __device__ __forceinline__ void next() { if (--left == 0) { ++g; left = k; } }
+};
+
 // the constants of V channels of one image: pre = (x - mean_hi) * a + b.  stats: {mean, rstd} of the groups from g0 on
 template <int V> struct Affine {
     float m[V], a[V], b[V];
     __device__ __forceinline__ void load(const double* stats, int g0, const float* __restrict__ gamma, const float* __restrict__ beta,
                                          int col, int k) {
+        GroupOf at(col, k);
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const double* st = stats + ((col + i) / k - g0) * 2;
+        for (int i = 0; i < V; ++i, at.next()) {
+            const double* st = stats + (at.g - g0) * 2;
             const double ga = gamma ? (double)gamma[col + i] : 1.0, be = beta ? (double)beta[col + i] : 0.0;
             m[i] = (float)st[0];
             a[i] = (float)(st[1] * ga);
@@ -433,8 +451,9 @@ _Pragma("unroll")
     __syncthreads();
     if (!at.active) return;
     float k1[V], k2[V];
+    GroupOf of(at.col, s.k);
 #pragma unroll
-    for (int i = 0; i < V; ++i) { const int h = (at.col + i) / s.k - g0; k1[i] = coef[2 * h]; k2[i] = coef[2 * h + 1]; }
+    for (int i = 0; i < V; ++i, of.next()) { k1[i] = coef[2 * (of.g - g0)]; k2[i] = coef[2 * (of.g - g0) + 1]; }
     T* op = dx + row0 * s.c + at.col;
     T* qp = RES && dres ? dres + row0 * s.c + at.col : nullptr;
     GN_ACT(act, {
@@ -484,8 +503,6 @@ __global__ __launch_bounds__(NT) void gn_params_kernel(const double* __restrict_
 // ================================================================== streaming passes
 // Large sizes: two passes over memory with the sums of all workgroups between them.
 constexpr int UNR = 4, SUNR = 8;                           // pixels in flight per thread; in the statistics
-// keeps the scheduler from interleaving the vectors of an unrolled loop, which costs registers and so waves
-#define VECTOR_DONE() __builtin_amdgcn_sched_barrier(0)
 
 // SPAN: channels of a vector that share a group (a power of two that divides both V and k): V / SPAN pairs of sums per thread
 template <typename T, int V, int SPAN>
@@ -507,13 +524,14 @@ __global__ __launch_bounds__(NT) void gn_stats_kernel(const T* __restrict__ x, i
                 q[i / SPAN] = fma(f, f, q[i / SPAN]);
             }
         };
+        Chunk<T, V> v[SUNR];
         at.walk<SUNR>(s, [&](long long r) {
-            Chunk<T, V> v[SUNR];
 #pragma unroll
             for (int j = 0; j < SUNR; ++j) v[j].load(p + (size_t)(r + j * at.slots) * ld);
+        }, [] {}, [&](long long) {
 #pragma unroll
             for (int j = 0; j < SUNR; ++j) add(v[j]);
-        }, [&](long long r) { Chunk<T, V> v; v.load(p + (size_t)r * ld); add(v); });
+        }, [&](long long r) { Chunk<T, V> e; e.load(p + (size_t)r * ld); add(e); });
     }
 #pragma unroll
     for (int i = 0; i < NA; ++i) { red[2 * i][threadIdx.x] = a[i]; red[2 * i + 1][threadIdx.x] = q[i]; }
@@ -560,17 +578,17 @@ __global__ __launch_bounds__(NT) void gn_fwd_kernel(const T* __restrict__ x, int
     if (!at.active) return;
     const int n = blockIdx.y;
     Affine<V> k;
-    k.load(stats + (size_t)n * s.groups * 2, 0, gamma, beta, at.col, s.k);
     const T* xp = x + (size_t)n * s.hw * ld + at.col;
     const T* rp = RES ? res + (size_t)n * s.hw * res_ld + at.col : nullptr;
     T* yp = y + (size_t)n * s.hw * y_ld + at.col;
+    Chunk<T, V> v[UNR], w[UNR];
     at.walk<UNR>(s, [&](long long r) {
-        Chunk<T, V> v[UNR], w[UNR];
 #pragma unroll
         for (int j = 0; j < UNR; ++j) {
             v[j].load(xp + (size_t)(r + j * at.slots) * ld);
             if constexpr (RES) w[j].load(rp + (size_t)(r + j * at.slots) * res_ld);
         }
+    }, [&] { k.load(stats + (size_t)n * s.groups * 2, 0, gamma, beta, at.col, s.k); }, [&](long long r) {
 #pragma unroll
         for (int j = 0; j < UNR; ++j) fwd_vector<T, V, ACT, RES>(k, v[j], w[j], slope).store(yp + (size_t)(r + j * at.slots) * y_ld);
     }, [&](long long r) {
@@ -597,7 +615,6 @@ __global__ __launch_bounds__(NT) void gn_bwd_reduce_kernel(const T* __restrict__
     for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.f;
     if (at.active) {
         Affine<V> k;
-        k.load(st0, 0, gamma, beta, at.col, s.k);
         const T* gp = dy + (size_t)n * s.hw * dy_ld + at.col;
         const T* xp = x + (size_t)n * s.hw * ld + at.col;
         const T* rp = RES ? res + (size_t)n * s.hw * res_ld + at.col : nullptr;
@@ -615,24 +632,31 @@ __global__ __launch_bounds__(NT) void gn_bwd_reduce_kernel(const T* __restrict__
                 settle<T, V, ACT, RES>(gp + (size_t)r * dy_ld, xp + (size_t)r * ld, RES ? rp + (size_t)r * res_ld : nullptr, slope, st0, 0, gamma, beta, at.col, s.k, g);
             add(g, d);
         };
+        Chunk<T, V> u[UNR], v[UNR], w[UNR];
         at.walk<UNR>(s, [&](long long r) {
-            Chunk<T, V> u[UNR], v[UNR], w[UNR];
-            unsigned near = 0;
 #pragma unroll
             for (int j = 0; j < UNR; ++j) {
                 u[j].load(gp + (size_t)(r + j * at.slots) * dy_ld);
                 v[j].load(xp + (size_t)(r + j * at.slots) * ld);
                 if constexpr (RES) w[j].load(rp + (size_t)(r + j * at.slots) * res_ld);
             }
+        }, [&] {
+            k.load(st0, 0, gamma, beta, at.col, s.k);
+        }, [&](long long r) {
+            unsigned near = 0;
 #pragma unroll
             for (int j = 0; j < UNR; ++j) {
                 float g[V], d[V];
+                u[j].forget();
+                v[j].forget();
                 const bool skip = bwd_vector<T, V, ACT, RES>(k, u[j], v[j], w[j], slope, g, d);
                 near |= (unsigned)skip << j;
 #pragma unroll
                 for (int i = 0; i < V; ++i) g[i] = skip ? 0.f : g[i];
                 add(g, d);
-                VECTOR_DONE();
+#pragma unroll
+                for (int i = 0; i < V; ++i) asm volatile("" : "+v"(s1[i]), "+v"(s2[i]));
+                __builtin_amdgcn_sched_barrier(0);         // vector by vector: interleaved they would cost registers and so waves
             }
             for (; near; near &= near - 1) one(r + __builtin_ctz(near) * at.slots);        // rare
         }, one);
@@ -714,14 +738,7 @@ __global__ __launch_bounds__(NT) void gn_bwd_apply_kernel(const T* __restrict__ 
     if (!at.active) return;
     const double* st0 = stats + (size_t)n * s.groups * 2;
     Affine<V> k;
-    k.load(st0, 0, gamma, beta, at.col, s.k);
     float k1[V], k2[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        const float* q = coef + ((size_t)n * s.groups + (at.col + i) / s.k) * 2;
-        k1[i] = q[0];
-        k2[i] = q[1];
-    }
     const T* gp = dy + (size_t)n * s.hw * dy_ld + at.col;
     const T* xp = x + (size_t)n * s.hw * ld + at.col;
     const T* rp = RES ? res + (size_t)n * s.hw * res_ld + at.col : nullptr;
@@ -745,21 +762,31 @@ __global__ __launch_bounds__(NT) void gn_bwd_apply_kernel(const T* __restrict__ 
             settle<T, V, ACT, RES>(gp + (size_t)r * dy_ld, xp + (size_t)r * ld, RES ? rp + (size_t)r * res_ld : nullptr, slope, st0, 0, gamma, beta, at.col, s.k, g);
         write(g, d, r);
     };
+    Chunk<T, V> u[UNR], v[UNR], w[UNR];
     at.walk<UNR>(s, [&](long long r) {
-        Chunk<T, V> u[UNR], v[UNR], w[UNR];
-        unsigned near = 0;
 #pragma unroll
         for (int j = 0; j < UNR; ++j) {
             u[j].load(gp + (size_t)(r + j * at.slots) * dy_ld);
             v[j].load(xp + (size_t)(r + j * at.slots) * ld);
             if constexpr (RES) w[j].load(rp + (size_t)(r + j * at.slots) * res_ld);
         }
+    }, [&] {
+        k.load(st0, 0, gamma, beta, at.col, s.k);
+    GroupOf of(at.col, s.k);
+#pragma unroll
+    for (int i = 0; i < V; ++i, of.next()) {
+        const float* q = coef + ((size_t)n * s.groups + of.g) * 2;
+        k1[i] = q[0];
+        k2[i] = q[1];
+    }
+    }, [&](long long r) {
+        unsigned near = 0;
 #pragma unroll
         for (int j = 0; j < UNR; ++j) {
             float g[V], d[V];
             near |= (unsigned)bwd_vector<T, V, ACT, RES>(k, u[j], v[j], w[j], slope, g, d) << j;
             write(g, d, r + j * at.slots);
-            VECTOR_DONE();
+            __builtin_amdgcn_sched_barrier(0);             // vector by vector, as above
         }
         for (; near; near &= near - 1) one(r + __builtin_ctz(near) * at.slots);            // rare: written again
     }, one);
@@ -782,15 +809,21 @@ Plan make_plan(int dtype, int n, long long hw, int c, int groups, bool vec) {
     p.s.cqb = cq < NT ? cq : NT;
     p.zs = (cq + p.s.cqb - 1) / p.s.cqb;
     const int slots = NT / p.s.cqb;
-    // Eight workgroups per CU where each still makes three trips (6x64x512x1024 bf16, forward + backward: 663 us at two per
-    // CU, 632 at four, 606 at eight; 6x512x64x128: 174, 172 and, with one and a half trips, 185), trips spread evenly.
-    const long long trips = (hw + (long long)UNR * slots - 1) / ((long long)UNR * slots);
-    long long chunks = 2048 / ((long long)n * p.zs);
-    if (chunks > trips / 3) chunks = trips / 3;
-    if (chunks < 1) chunks = 1;
-    const long long each = (trips + chunks - 1) / chunks;
-    chunks = (trips + each - 1) / each;
-    p.s.chunks = chunks < 1 ? 1 : (int)chunks;
+    // Up to six workgroups per CU, as many as share both the trips of an image and the CUs evenly: 6x64x512x1024 bf16,
+    // forward + backward, takes 584 us with 1,896 workgroups (7.4 per CU), 551 with 1,536; six rather than eight for
+    // 2x64x512x1024, whose forward pass takes 50 us instead of 55.  A small image goes down to one trip per workgroup
+    // (6x512x64x128: 156 us, 165 with three trips; 3x80x77x131: 52 and 63).
+    const long long trips = (hw + (long long)UNR * slots - 1) / ((long long)UNR * slots), per = (long long)n * p.zs;
+    double best = 0.0;
+    for (int w = 6; w >= 1; --w) {
+        long long chunks = 256LL * w / per;
+        if (chunks > trips) chunks = trips;
+        if (chunks < 1) chunks = 1;
+        const long long each = (trips + chunks - 1) / chunks;
+        chunks = (trips + each - 1) / each;
+        const double even = (double)(trips * per) / (double)(each * ((per * chunks + 255) / 256 * 256));
+        if (even > best * 1.02) { best = even; p.s.chunks = (int)chunks; }
+    }
     return p;
 }
 
@@ -802,7 +835,7 @@ Cell make_cell(int dtype, int n, long long hw, int c, int groups, bool vec, int 
     const int v = dtype == UR_BF16 ? 8 : 4, esz = dtype == UR_BF16 ? 2 : 4;
     int base = s.k;
     while (base % v) base += s.k;                          // whole groups and whole vectors; divides c
-    if (base / v > CT) return s;
+    if (base / v > CT / 4) return s;                       // (with a wide slab's sums the backward pass would need more than 64 KB of LDS)
     const int units = c / base;
     const auto fits = [&](int m) {
         const int cqs = m * base / v;
@@ -814,7 +847,7 @@ Cell make_cell(int dtype, int n, long long hw, int c, int groups, bool vec, int 
         --m;
     }
     if (!fits(m) || (m * base * esz < 64 && m < units)) return s;
-    if ((long long)n * ((units + m - 1) / m) > 0x7fffffffLL) return s;
+    if ((long long)n * ((units + m - 1) / m) > 0x7fffffLL) return s;   // a launch has fewer than 2^32 threads
     s.slab = m * base;
     s.slabs = (units + m - 1) / m;
     return s;
@@ -867,7 +900,7 @@ int check(const char* what, int dtype, int n, long long hw, int c, int groups, i
     UR_REQUIRE(dtype == UR_F32 || dtype == UR_BF16, "%s: bad dtype %d", what, dtype);
     UR_REQUIRE(n > 0 && hw > 0 && c > 0 && groups > 0, "%s: non-positive sizes (n %d, pixels %lld, channels %d, groups %d)", what, n, hw, c, groups);
     UR_REQUIRE(c % groups == 0, "%s: %d channels are not divisible by %d groups", what, c, groups);
-    UR_REQUIRE(n < 65535 && hw <= (1LL << 40) && c <= (1 << 20), "%s: sizes beyond the limits (65534 images, 2^40 pixels, 2^20 channels)", what);
+    UR_REQUIRE(n < 65535 && hw <= (1LL << 40) && c <= 16384, "%s: sizes beyond the limits (65534 images, 2^40 pixels, 16384 channels)", what);
     UR_REQUIRE(act >= UR_ACT_NONE && act <= UR_ACT_SILU, "%s: bad activation %d", what, act);
     return UR_OK;
 }
