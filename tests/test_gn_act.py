@@ -177,6 +177,18 @@ def test_to_group_norm_replaces_every_batch_norm_and_keeps_the_parameters():
     assert isinstance(hnn.to_group_norm(torch.nn.BatchNorm2d(6, affine=False), 4), hnn.GroupNorm)
 
 
+def test_to_group_norm_keeps_a_shared_layer_shared():
+    bn = torch.nn.BatchNorm2d(8)
+    inner = torch.nn.Sequential(bn, torch.nn.ReLU(), bn)
+    m = hnn.to_group_norm(torch.nn.Sequential(inner, bn, inner), 4)
+    assert isinstance(m[1], hnn.GroupNorm) and m[0][0] is m[1] and m[0][2] is m[1] and m[2] is m[0]
+
+
+def test_entry_points_refuse_more_channels_than_their_sums_are_laid_out_for():
+    for query in ("ur_gn_fwd_workspace", "ur_gn_bwd_workspace"):
+        assert _lib.query(query, _lib.UR_BF16, 1, 4, 16384, 32) > 0 and _lib.query(query, _lib.UR_BF16, 1, 4, 16392, 8) == 0
+
+
 # ------------------------------------------------------------------------------ values (GPU)
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
@@ -268,6 +280,33 @@ def test_channel_windows_and_other_layouts(c0, wide):
     rest = torch.ones(wide, dtype=torch.bool)
     rest[c0:c0 + 8] = False
     assert (buf[:, rest] == 7).all()                            # what lies beside the window stays
+
+
+@pytest.mark.gpu
+def test_an_output_window_shares_nothing_with_the_inputs():
+    gn = hnn.GroupNorm(4, 8).to(DEV)
+    buf = torch.randn(2, 24, 6, 5, device=DEV).contiguous(memory_format=torch.channels_last)
+    x, y = ops.alias_window(buf, 0, 8), ops.alias_window(buf, 8, 8)
+    want = ops.gn_act(x.clone(memory_format=torch.channels_last), gn)
+    version = y._version
+    with torch.no_grad():
+        assert torch.equal(ops.gn_act(x, gn, out=y), want)      # neighbours in one buffer
+    assert y._version > version
+    for out, residual in ((x, None), (ops.alias_window(buf, 4, 8), None), (y, ops.alias_window(buf, 12, 8)), (ops.alias_window(buf, 7, 8), None)):
+        with pytest.raises(RuntimeError, match="shares elements"):
+            ops.gn_act(x, gn, residual=residual, out=out)
+    first = ops.gn_act(x, gn, out=ops.alias_window(buf, 16, 8))
+    with pytest.raises(RuntimeError, match="belongs to a graph"):
+        ops.gn_act(x, gn, out=first)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(2, 1024, 3, 3, 1), (2, 2048, 3, 3, 1), (1, 4088, 2, 2, 8), (1, 4096, 1, 5, 4096), (3, 72, 90, 70, 8)])
+def test_wide_groups(shape, dtype):
+    """Groups as wide as a cell's sums allow and wider, and the widest slabs."""
+    x, dy, r, gn = make(shape, dtype, 15, residual=True)
+    check(x, dy, r, gn, "silu", run(x, dy, r, gn, "silu"))
 
 
 @pytest.mark.gpu

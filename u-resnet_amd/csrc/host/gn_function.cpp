@@ -9,6 +9,7 @@
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
 
+#include <climits>
 #include <memory>
 #include <stdexcept>
 
@@ -31,7 +32,17 @@ struct Shape {
 int pitch(const at::Tensor& t) {
     if (t.is_contiguous(CL)) return (int)t.size(1);
     const int64_t c = t.size(1), h = t.size(2), w = t.size(3), ld = t.stride(3);
-    return t.stride(1) == 1 && ld >= c && t.stride(2) == w * ld && t.stride(0) == h * w * ld ? (int)ld : 0;
+    return t.stride(1) == 1 && ld >= c && ld <= INT_MAX && t.stride(2) == w * ld && t.stride(0) == h * w * ld ? (int)ld : 0;
+}
+
+// whether two tensors with a pitch share an element; windows over different channels of one buffer do not
+bool overlap(const at::Tensor& a, const at::Tensor& b) {
+    const int64_t pa = pitch(a), pb = pitch(b), c = a.size(1), rows = a.size(0) * a.size(2) * a.size(3), size = (int64_t)a.element_size();
+    const char *p = static_cast<const char*>(a.data_ptr()), *q = static_cast<const char*>(b.data_ptr());
+    if (p + ((rows - 1) * pa + c) * size <= q || q + ((rows - 1) * pb + c) * size <= p) return false;
+    if (pa != pb || (p - q) % size) return true;
+    const int64_t off = (((p - q) / size) % pa + pa) % pa;
+    return off < c || off > pa - c;
 }
 
 void* ptr(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
@@ -108,6 +119,7 @@ at::Tensor forward(const at::Tensor& x, const at::Tensor& gamma, const at::Tenso
     {
         const at::NoGradGuard no_grad;
         if (!z.defined()) z = at::empty(x.sizes(), x.options().memory_format(CL));
+        else if (!z.is_inference()) z.unsafeGetTensorImpl()->bump_version();       // written in place
         stats = at::empty({s.n, groups, 2}, x.options().dtype(at::kDouble));
         const size_t bytes = entry.gn_fwd_workspace(s.dtype, s.n, s.hw, s.c, groups);
         const at::Tensor ws = at::empty({(int64_t)(bytes ? bytes : 16)}, x.options().dtype(at::kByte));
@@ -180,6 +192,11 @@ PyObject* gn_act(PyObject*, PyObject* args) {
     if (out.defined() && (out.dim() != 4 || out.sizes() != x.sizes() || out.device() != x.device() || out.scalar_type() != x.scalar_type() || !pitch(out)))
         return refuse(PyExc_RuntimeError, "`out` must be a channel window with x's shape, dtype and device");
     if (!pitch(x)) return refuse(PyExc_RuntimeError, "x must be channels last or a channel window");
+    if (x.size(0) > INT_MAX) return refuse(PyExc_RuntimeError, std::to_string(x.size(0)) + " images");
+    if (out.defined() && (overlap(out, x) || (residual.defined() && overlap(out, residual))))
+        return refuse(PyExc_RuntimeError, "`out` shares elements with an input");
+    if (out.defined() && out.requires_grad() && at::GradMode::is_enabled())
+        return refuse(PyExc_RuntimeError, "`out` belongs to a graph or is a leaf that requires a gradient");
     at::Tensor z;
     std::string error;
     Py_BEGIN_ALLOW_THREADS

@@ -129,10 +129,18 @@ def to_group_norm(module, num_groups=32):
             gn.weight, gn.bias = module.weight, module.bias
         gn.train(module.training)
         return gn
-    for name, child in list(module.named_children()):
-        new = to_group_norm(child, num_groups)
-        if new is not child:
-            setattr(module, name, new)
+    done = {}                                       # a layer used in several places stays one layer
+
+    def replace(parent):
+        for name, child in list(parent._modules.items()):
+            if child is None:
+                continue
+            if child not in done:
+                done[child] = to_group_norm(child, num_groups) if isinstance(child, tnn.BatchNorm2d) else child
+                replace(child)
+            if done[child] is not child:
+                setattr(parent, name, done[child])
+    replace(module)
     return module
 
 
