@@ -107,6 +107,24 @@ def test_refusals_without_a_gpu():
         train.AdamW([torch.nn.Parameter(torch.zeros(4, dtype=torch.float64))]).state_buffers()
 
 
+def test_parameters_listed_twice_or_sharing_memory_are_refused():
+    import warnings
+    p, q = torch.nn.Parameter(torch.zeros(4)), torch.nn.Parameter(torch.zeros(3))
+    with warnings.catch_warnings():
+        warnings.simplefilter("ignore")
+        with pytest.raises(ValueError, match="twice"):
+            train.AdamW([p, q, p])
+        opt = train.AdamW([q])
+        with pytest.raises(ValueError, match="twice"):
+            opt.add_param_group(dict(params=[p, p]))
+    assert len(opt.param_groups) == 1
+    flat = torch.zeros(10)
+    a, b, c = (torch.nn.Parameter(flat[i:i + 5]) for i in (0, 5, 4))
+    train.AdamW([a, b]).state_buffers()                        # neighbours
+    with pytest.raises(_lib.UResNetHipError, match="share memory"):
+        train.AdamW([a, c]).state_buffers()
+
+
 def test_entry_points_refuse_before_any_launch():
     import ctypes as C
     n = C.c_longlong()
@@ -417,6 +435,16 @@ def test_unaligned_views_channels_last_gradients_and_refused_layouts():
         train.clip_grad_norm_([bad], 1.0)
     with pytest.raises(ValueError, match="twice"):
         train.clip_grad_norm_([cl, cl], 1.0)
+    overlapping = [torch.nn.Parameter(torch.zeros(6, device=DEV)) for _ in range(2)]
+    overlapping[0].grad, overlapping[1].grad = flat_g[:6], flat_g[5:11]
+    with pytest.raises(ValueError, match="overlap"):
+        train.clip_grad_norm_(overlapping, 1.0)
+    turned = torch.nn.Parameter(torch.zeros(30, 7, device=DEV))
+    turned.grad = torch.randn(7, 30, device=DEV).t()           # dense in another order
+    g = turned.grad.cpu()
+    norm, factor = factor_of([g], 0.5)
+    assert abs(train.clip_grad_norm_([turned], 0.5).item() - norm) <= 2 * E24 * norm
+    within(turned.grad, g.double() * factor, 5 * E24 * g.double().abs() * factor, "transposed gradient")
     bad.grad = torch.zeros(4, 4, device=DEV).to_sparse()
     for f in (lambda: train.clip_grad_norm_([bad], 1.0), lambda: train.AdamW([bad]).step()):
         with pytest.raises(_lib.UResNetHipError, match="dense"):

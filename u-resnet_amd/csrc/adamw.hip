@@ -34,6 +34,7 @@ constexpr int CHUNK = U * NT * 4;            // elements per unit of work
 constexpr int MAX_ROWS = 1024;               // tensors per table: the kernels keep its list of first chunks in the LDS
 constexpr int BATCH = 136;                   // rows per table launch: kernel arguments stay under 4 KB
 constexpr int MAX_PARTS = 1024;             // partial sums of the norm
+constexpr long long MAX_CHUNKS = 1LL << 30;  // a chunk's number plus the grid's size stays an int
 constexpr float TOP = 448.f;
 
 typedef __attribute__((ext_vector_type(4))) float fvec4_t;
@@ -409,7 +410,7 @@ int ur_param_table(const long long* params, const long long* grads, const long l
         UR_REQUIRE(sizes[i] >= 0 && sizes[i] <= (1LL << 40), "param_table: a tensor of %lld elements", sizes[i]);
         if (grads[i]) chunks += (sizes[i] + CHUNK - 1) / CHUNK;
     }
-    UR_REQUIRE(chunks > 0 && chunks <= 0x7fffffffLL, "param_table: no gradient with elements, or too many elements");
+    UR_REQUIRE(chunks > 0 && chunks <= MAX_CHUNKS, "param_table: no gradient with elements, or too many elements");
     int first = 0;
     for (int at = 0; at < ntensors; at += BATCH) {
         ListBatch b = {};
@@ -429,7 +430,7 @@ int ur_param_table(const long long* params, const long long* grads, const long l
 }
 
 int ur_grad_sqnorm(const void* table, int ntensors, long long nchunks, double* parts, int* nparts, ur_stream_t s) {
-    UR_REQUIRE(table && ntensors > 0 && ntensors <= MAX_ROWS && nchunks > 0 && nchunks <= 0x7fffffffLL && parts && nparts, "grad_sqnorm: bad arguments");
+    UR_REQUIRE(table && ntensors > 0 && ntensors <= MAX_ROWS && nchunks > 0 && nchunks <= MAX_CHUNKS && parts && nparts, "grad_sqnorm: bad arguments");
     *nparts = norm_parts(nchunks);
     hipLaunchKernelGGL(grad_sqnorm_kernel, dim3(*nparts), dim3(NT), 0, (hipStream_t)s, (const Row*)table, ntensors, (int)nchunks, parts);
     return ur_check_launch("grad_sqnorm");
@@ -437,7 +438,7 @@ int ur_grad_sqnorm(const void* table, int ntensors, long long nchunks, double* p
 
 int ur_grad_clip(const void* table, int ntensors, long long nchunks, const double* parts, int nparts, float max_norm, float* out_norm,
                  ur_stream_t s) {
-    UR_REQUIRE(table && ntensors > 0 && ntensors <= MAX_ROWS && nchunks > 0 && nchunks <= 0x7fffffffLL && parts && nparts > 0, "grad_clip: bad arguments");
+    UR_REQUIRE(table && ntensors > 0 && ntensors <= MAX_ROWS && nchunks > 0 && nchunks <= MAX_CHUNKS && parts && nparts > 0, "grad_clip: bad arguments");
     hipLaunchKernelGGL(grad_scale_kernel, dim3(norm_parts(nchunks)), dim3(NT), 0, (hipStream_t)s, (const Row*)table, ntensors, (int)nchunks,
                        parts, nparts, max_norm, out_norm);
     return ur_check_launch("grad_clip");
@@ -446,7 +447,7 @@ int ur_grad_clip(const void* table, int ntensors, long long nchunks, const doubl
 int ur_adamw_multi(const void* table, int ntensors, long long nchunks, int state_bits, void* exp_avg, void* exp_avg_sq, float* exp_avg_scale,
                    float* exp_avg_sq_scale, double lr, double beta1, double beta2, double eps, double weight_decay, const double* parts,
                    int nparts, float max_norm, float grad_scale, float* out_norm, ur_stream_t s) {
-    UR_REQUIRE(table && ntensors > 0 && ntensors <= MAX_ROWS && nchunks > 0 && nchunks <= 0x7fffffffLL && exp_avg && exp_avg_sq, "adamw_multi: bad arguments");
+    UR_REQUIRE(table && ntensors > 0 && ntensors <= MAX_ROWS && nchunks > 0 && nchunks <= MAX_CHUNKS && exp_avg && exp_avg_sq, "adamw_multi: bad arguments");
     UR_REQUIRE(state_bits == 32 || state_bits == 8, "adamw_multi: state_bits is 32 or 8 (got %d)", state_bits);
     UR_REQUIRE(state_bits == 32 || (exp_avg_scale && exp_avg_sq_scale), "adamw_multi: 8-bit states without scales");
     UR_REQUIRE((((uintptr_t)exp_avg | (uintptr_t)exp_avg_sq) & 15) == 0, "adamw_multi: the state buffers are not 16-byte aligned");

@@ -15,7 +15,7 @@ for s in "${SRCS[@]}"; do
     src="$HERE/$s.hip"
     obj="$OBJ/$s.o"
     stale=0
-    for dep in "$src" "$HERE"/*.h "$HERE/../../include/uresnet_hip.h"; do
+    for dep in "$src" "$HERE/build.sh" "$HERE"/*.h "$HERE/../../include/uresnet_hip.h"; do
         if [ ! -f "$obj" ] || [ "$dep" -nt "$obj" ]; then stale=1; fi
     done
     if [ "$stale" = 1 ]; then
@@ -32,7 +32,7 @@ PYINC="$($PY -c 'import sysconfig; print(sysconfig.get_paths()["include"])')"
 for s in "${HOSTSRC[@]}"; do
     src="$HERE/host/$s.cpp"
     obj="$OBJ/host_$s.o"
-    if [ ! -f "$obj" ] || [ "$src" -nt "$obj" ] || [ "$HERE/host/host.h" -nt "$obj" ] || [ "$HERE/../../include/uresnet_hip.h" -nt "$obj" ]; then
+    if [ ! -f "$obj" ] || [ "$src" -nt "$obj" ] || [ "$HERE/host/host.h" -nt "$obj" ] || [ "$HERE/build.sh" -nt "$obj" ] || [ "$HERE/../../include/uresnet_hip.h" -nt "$obj" ]; then
         ( "${CXX:-g++}" -O2 -std=c++17 -fPIC -Wall -D__HIP_PLATFORM_AMD__=1 -isystem "$TORCH/include" \
             -isystem "$TORCH/include/torch/csrc/api/include" -isystem "${ROCM_PATH:-/opt/rocm}/include" -I"$PYINC" -c "$src" -o "$obj" ) &
         pids+=($!)

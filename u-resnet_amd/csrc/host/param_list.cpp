@@ -4,6 +4,7 @@
 #include "host.h"
 
 #include <algorithm>
+#include <utility>
 #include <vector>
 
 namespace {
@@ -75,16 +76,18 @@ PyObject* clip_rows(PyObject*, PyObject* params) {
         if (!g.defined()) continue;
         if (device < 0) { first = g.device(); device = first.is_cuda() ? first.index() : 0; }
         if (!plain_gpu_f32(g, first)) return fail("clip_grad_norm_: gradients must be dense fp32 tensors on one GPU (got " + told(g) + ")");
-        if (!(g.is_contiguous() || g.is_contiguous(at::MemoryFormat::ChannelsLast))) return fail("clip_grad_norm_: a gradient is not dense");
+        if (!g.is_non_overlapping_and_dense()) return fail("clip_grad_norm_: a gradient is not dense");
         if (!g.numel()) continue;
         gs.push_back((long long)g.data_ptr());
         ns.push_back((long long)g.numel());
     }
-    std::vector<long long> sorted(gs);
+    std::vector<std::pair<long long, long long>> sorted;                       // {begin, end} in bytes
+    for (size_t i = 0; i < gs.size(); ++i) sorted.emplace_back(gs[i], gs[i] + 4 * ns[i]);
     std::sort(sorted.begin(), sorted.end());
-    if (std::adjacent_find(sorted.begin(), sorted.end()) != sorted.end()) {
-        PyErr_SetString(PyExc_ValueError, "clip_grad_norm_: a gradient is listed twice");
-        return nullptr;
-    }
+    for (size_t i = 1; i < sorted.size(); ++i)
+        if (sorted[i].first < sorted[i - 1].second) {
+            PyErr_SetString(PyExc_ValueError, sorted[i] == sorted[i - 1] ? "clip_grad_norm_: a gradient is listed twice" : "clip_grad_norm_: two gradients overlap");
+            return nullptr;
+        }
     return Py_BuildValue("NNni", bytes_of(gs), bytes_of(ns), (Py_ssize_t)gs.size(), device);
 }

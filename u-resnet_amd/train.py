@@ -337,7 +337,7 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     """torch.nn.utils.clip_grad_norm_ for fp32 gradients on one GPU: scales them in place by min(1, max_norm / (norm + 1e-6))
     and returns their norm before that as a 0-dim device tensor.  No host synchronisation (except with error_if_nonfinite,
     which raises before anything is scaled), no staging buffers: it can be captured in a graph.  A norm within the limit
-    leaves the gradients untouched.  Only the 2-norm; gradients must not overlap."""
+    leaves the gradients untouched.  Only the 2-norm; gradients that overlap are refused."""
     if norm_type != 2:
         raise NotImplementedError("clip_grad_norm_: only norm_type=2 is implemented (got %r)" % (norm_type,))
     max_norm = float(max_norm)
@@ -376,6 +376,9 @@ class _MomentPool:
     def __init__(self, group, state):
         self.params, self.bits, self.device = list(group['params']), group['state_bits'], group['params'][0].device
         sizes = [p.numel() for p in self.params]
+        places = sorted((p.data_ptr(), p.data_ptr() + 4 * n) for p, n in zip(self.params, sizes) if n)
+        if any(a[1] > b[0] for a, b in zip(places, places[1:])):
+            raise _lib.UResNetHipError("AdamW: two parameters of a group share memory")
         self.blocks, at = [], 0
         for p, n in zip(self.params, sizes):
             if p.dtype != torch.float32 or not p.is_contiguous() or p.device != self.device:
@@ -454,6 +457,9 @@ class AdamW(torch.optim.Optimizer):
         if not (g['lr'] >= 0 and g['eps'] >= 0 and g['weight_decay'] >= 0 and all(0 <= b < 1 for b in g['betas'])):
             raise ValueError("AdamW: lr, eps and weight_decay must not be negative, betas lie in [0, 1)")
         super().add_param_group(group)
+        if len(set(self.param_groups[-1]['params'])) < len(self.param_groups[-1]['params']):
+            self.param_groups.pop()
+            raise ValueError("AdamW: a parameter is listed twice")
 
     def __setstate__(self, state):             # copied or unpickled: the pools are built again from `state`
         super().__setstate__(state)
