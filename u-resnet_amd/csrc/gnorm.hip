@@ -107,6 +107,9 @@ template <int ACT> __device__ __forceinline__ bool gn_near_kink(float p, float s
     return false;
 }
 
+// a / b for 0 <= a < 2^20: (a + 1/2) / b is at least 1 / (2 b) from an integer, its relative error at most 2^-21
+__device__ __forceinline__ int small_div(int a, int b) { return (int)(((float)a + 0.5f) * __builtin_amdgcn_rcpf((float)b)); }
+
 struct GnShape {
     long long hw;
     int c, groups, k;             // channels, groups, channels per group
@@ -121,8 +124,8 @@ struct Place {
     int slot, slots, cg, col;
     bool active;
     template <int V> __device__ __forceinline__ void set(const GnShape& s) {
-        slots = NT / s.cqb;
-        slot = threadIdx.x / s.cqb;
+        slots = small_div(NT, s.cqb);
+        slot = small_div(threadIdx.x, s.cqb);
         cg = threadIdx.x - slot * s.cqb;
         col = (blockIdx.z * s.cqb + cg) * V;
         active = slot < slots && col < s.c;
@@ -147,16 +150,27 @@ struct Place {
     }
 };
 
-// folds the rows of red[values][slots * cqb] over the slots in halves, always in the same order; result at slot 0
+// Rows of sums in the LDS are padded by eight entries: threads that read one slot of several rows then meet different banks.
+constexpr int PAD = 8;
+
+// adds the rows of red[values][slots * cqb] over the slots, always in the same order; result at slot 0.  Every sum of one row
+// and channel vector is made by up to 16 threads, a strided part of the slots each, and one of them adds their results: two
+// waits whatever the number of slots, and reads that do not depend on each other.
 template <typename F, int N>
-__device__ __forceinline__ void fold_slots(F (*red)[N], int values, int slot, int slots, int cqb) {
+__device__ __forceinline__ void fold_slots(F (*red)[N], int values, int slots, int cqb) {
+    constexpr int THREADS = N - PAD;
     __syncthreads();
-    for (int n = slots; n > 1;) {
-        const int half = (n + 1) >> 1;
-        if (slot + half < n)
-            for (int i = 0; i < values; ++i) red[i][threadIdx.x] += red[i][threadIdx.x + half * cqb];
+    const int outs = values * cqb, parts = min(slots, max(1, min(16, small_div(THREADS, outs))));
+    for (int left = slots, way = parts;; left = way, way = 1) {            // (slots to parts, parts to one)
+        for (int o = threadIdx.x; o < outs * way; o += THREADS) {
+            const int part = small_div(o, outs), q = o - part * outs, i = small_div(q, cqb), cg = q - i * cqb;
+            F s = red[i][part * cqb + cg];                                   // slots part, part + way, ...: no other thread's
+#pragma unroll 4
+            for (int r = part + way; r < left; r += way) s += red[i][r * cqb + cg];
+            red[i][part * cqb + cg] = s;
+        }
         __syncthreads();
-        n = half;
+        if (way == 1) break;
     }
 }
 
@@ -170,23 +184,35 @@ __device__ __forceinline__ void mean_rstd(double a, double q, double count, floa
 // the group of a channel and of those after it, with one division
 struct GroupOf {
     int g, left, k;
-    __device__ __forceinline__ GroupOf(int c, int k_) : g(c / k_), left((g + 1) * k_ - c), k(k_) {}
+    __device__ __forceinline__ GroupOf(int c, int k_) : g(small_div(c, k_)), left((g + 1) * k_ - c), k(k_) {}
     __device__ __forceinline__ void next() { if (--left == 0) { ++g; left = k; } }
 };
 
-// the constants of V channels of one image: pre = (x - mean_hi) * a + b.  stats: {mean, rstd} of the groups from g0 on
-template <int V> struct Affine {
-    float m[V], a[V], b[V];
-    __device__ __forceinline__ void load(const double* stats, int g0, const float* __restrict__ gamma, const float* __restrict__ beta,
-                                         int col, int k) {
+// the constants of V channels of one image: pre = (x - mean_hi) * a + b.  They are fetched first, so that they arrive while
+// the loads of the data are on their way
+template <int V> struct AffineIn {
+    float ga[V], be[V];
+    double mean[V], rstd[V];
+    __device__ __forceinline__ void params(const float* __restrict__ gamma, const float* __restrict__ beta, int col) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) { ga[i] = gamma ? gamma[col + i] : 1.f; be[i] = beta ? beta[col + i] : 0.f; }
+    }
+    // stats: {mean, rstd} of the groups from g0 on
+    __device__ __forceinline__ void groups(const double* stats, int g0, int col, int k) {
         GroupOf at(col, k);
 #pragma unroll
-        for (int i = 0; i < V; ++i, at.next()) {
-            const double* st = stats + (at.g - g0) * 2;
-            const double ga = gamma ? (double)gamma[col + i] : 1.0, be = beta ? (double)beta[col + i] : 0.0;
-            m[i] = (float)st[0];
-            a[i] = (float)(st[1] * ga);
-            b[i] = (float)(be - (st[0] - (double)m[i]) * (st[1] * ga));
+        for (int i = 0; i < V; ++i, at.next()) { mean[i] = stats[(at.g - g0) * 2]; rstd[i] = stats[(at.g - g0) * 2 + 1]; }
+    }
+};
+template <int V> struct Affine {
+    float m[V], a[V], b[V];
+    __device__ __forceinline__ void set(const AffineIn<V>& in) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const double s = in.rstd[i] * (double)in.ga[i];
+            m[i] = (float)in.mean[i];
+            a[i] = (float)s;
+            b[i] = (float)((double)in.be[i] - (in.mean[i] - (double)m[i]) * s);
         }
     }
 };
@@ -263,8 +289,8 @@ struct CellPlace {
         c0 = (blockIdx.x - n * s.slabs) * s.slab;
         sc = min(s.slab, s.c - c0);
         cqs = sc / V;
-        slots = CT / cqs;
-        slot = threadIdx.x / cqs;
+        slots = small_div(CT, cqs);
+        slot = small_div(threadIdx.x, cqs);
         cg = threadIdx.x - slot * cqs;
         col = c0 + cg * V;
         active = slot < slots;
@@ -279,6 +305,9 @@ __global__ __launch_bounds__(CT) void gn_fwd_cell_kernel(const T* __restrict__ x
     CellPlace at;
     at.set<V>(s);
     const size_t row0 = (size_t)at.n * s.hw;
+    AffineIn<V> in;
+    if (at.active) in.params(gamma, beta, at.col);
+    __builtin_amdgcn_sched_barrier(0);
     Chunk<T, V> v[K];
     const T* xp = x + row0 * ld + at.col;
 #pragma unroll
@@ -301,24 +330,27 @@ __global__ __launch_bounds__(CT) void gn_fwd_cell_kernel(const T* __restrict__ x
         }
     }
     // channels of the vector that share a group are added first: span of them (1, 2, 4 or 8)
-    int span = 1;
+    int span = 1, shift = 0;
 #pragma unroll
     for (int w = 1; w < V; w *= 2) {
         if (s.k % (2 * w) == 0) {
 #pragma unroll
             for (int i = 0; i < V; i += 2 * w) { a[i] += a[i + w]; q[i] += q[i + w]; }
             span = 2 * w;
+            ++shift;
         }
     }
     // sums and squares folded together, or one after the other where eight of each per thread would not fit the LDS at once
-    double(*red)[CT] = reinterpret_cast<double(*)[CT]>(cell_lds);
+    double(*red)[CT + PAD] = reinterpret_cast<double(*)[CT + PAD]>(cell_lds);
     const int na = V / span, rows = na > 4 ? na : 2 * na;
-    double* mine = cell_lds + rows * CT;
+    double* mine = cell_lds + rows * (CT + PAD);
     const int gs = at.sc / s.k, g0 = at.c0 / s.k, g = threadIdx.x;         // a slab begins with a group and has at most CT
     const auto group_sum = [&](int first) {
         double t = 0.0;
-        if (g < gs)
-            for (int ch = g * s.k; ch < (g + 1) * s.k; ch += span) t += red[first + (ch % V) / span][ch / V];
+        if (g < gs) {
+#pragma unroll 4
+            for (int ch = g * s.k; ch < (g + 1) * s.k; ch += span) t += red[first + (ch % V >> shift)][ch / V];
+        }
         return t;
     };
     double sa, sq;
@@ -328,7 +360,7 @@ __global__ __launch_bounds__(CT) void gn_fwd_cell_kernel(const T* __restrict__ x
             red[i / span][threadIdx.x] = a[i];
             if (rows > na) red[na + i / span][threadIdx.x] = q[i];
         }
-    fold_slots(red, rows, at.slot, at.slots, at.cqs);
+    fold_slots(red, rows, at.slots, at.cqs);
     sa = group_sum(0);
     if (rows > na) sq = group_sum(na);
     else {
@@ -336,7 +368,7 @@ __global__ __launch_bounds__(CT) void gn_fwd_cell_kernel(const T* __restrict__ x
 #pragma unroll
         for (int i = 0; i < V; ++i)
             if (i % span == 0) red[i / span][threadIdx.x] = q[i];
-        fold_slots(red, rows, at.slot, at.slots, at.cqs);
+        fold_slots(red, rows, at.slots, at.cqs);
         sq = group_sum(0);
     }
     if (g < gs) {
@@ -351,7 +383,8 @@ __global__ __launch_bounds__(CT) void gn_fwd_cell_kernel(const T* __restrict__ x
     __syncthreads();
     if (!at.active) return;
     Affine<V> k;
-    k.load(mine, g0, gamma, beta, at.col, s.k);
+    in.groups(mine, g0, at.col, s.k);
+    k.set(in);
     T* yp = y + row0 * y_ld + at.col;
     const T* rp = RES ? res + row0 * res_ld + at.col : nullptr;
     GN_ACT(act, {
@@ -376,7 +409,7 @@ __global__ __launch_bounds__(CT) void gn_bwd_cell_kernel(const T* __restrict__ d
                                                          T* __restrict__ dx, T* __restrict__ dres, double* __restrict__ sums,
                                                          float* __restrict__ dgamma, float* __restrict__ dbeta, Cell s) {
     extern __shared__ double cell_lds[];
-    float(*red)[CT] = reinterpret_cast<float(*)[CT]>(cell_lds);           // [2 V][CT] floats, then [sc][2] doubles, [gs][2] floats
+    float(*red)[CT + PAD] = reinterpret_cast<float(*)[CT + PAD]>(cell_lds);   // [2 V][CT + PAD] floats, [sc][2] doubles, [gs][2] floats
     CellPlace at;
     at.set<V>(s);
     const size_t row0 = (size_t)at.n * s.hw;
@@ -388,13 +421,16 @@ __global__ __launch_bounds__(CT) void gn_bwd_cell_kernel(const T* __restrict__ d
     const T* gp = dy + row0 * dy_ld + at.col;
     const T* xp = x + row0 * ld + at.col;
     const T* rp = RES ? res + row0 * res_ld + at.col : nullptr;
+    AffineIn<V> in;
+    if (at.active) { in.params(gamma, beta, at.col); in.groups(st0, g0, at.col, s.k); }
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int j = 0; j < K; ++j) {
         const int r = at.slot + j * at.slots;
         if (at.active && r < s.hw) { u[j].load(gp + (size_t)r * dy_ld); v[j].load(xp + (size_t)r * ld); }
     }
     Affine<V> k;
-    if (at.active) k.load(st0, g0, gamma, beta, at.col, s.k);
+    if (at.active) k.set(in);
     float s1[V], s2[V], g[V], d[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.f;
@@ -415,7 +451,7 @@ _Pragma("unroll")
     }
 #pragma unroll
     for (int i = 0; i < V; ++i) { red[2 * i][threadIdx.x] = s1[i]; red[2 * i + 1][threadIdx.x] = s2[i]; }
-    fold_slots(red, 2 * V, at.slot, at.slots, at.cqs);
+    fold_slots(red, 2 * V, at.slots, at.cqs);
     if (at.slot == 0) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
@@ -423,8 +459,9 @@ _Pragma("unroll")
             const double a = red[2 * i][threadIdx.x], b = red[2 * i + 1][threadIdx.x];
             const double q = (b - (st[0] - (double)(float)st[0]) * a) * st[1];         // xhat = (x - mean) * rstd
             const int c = at.col + i;
-            ch_sums[2 * (c - at.c0)] = a;
-            ch_sums[2 * (c - at.c0) + 1] = q;
+            const double ga = gamma ? (double)gamma[c] : 1.0;
+            ch_sums[2 * (c - at.c0)] = ga * a;
+            ch_sums[2 * (c - at.c0) + 1] = ga * q;
             if (sums) {
                 sums[((size_t)at.n * s.c + c) * 2] = a;
                 sums[((size_t)at.n * s.c + c) * 2 + 1] = q;
@@ -439,11 +476,8 @@ _Pragma("unroll")
     const double m = (double)s.hw * s.k;
     for (int h = threadIdx.x; h < gs; h += CT) {
         double p1 = 0.0, p2 = 0.0;
-        for (int c = h * s.k; c < (h + 1) * s.k; ++c) {
-            const double ga = gamma ? (double)gamma[at.c0 + c] : 1.0;
-            p1 += ga * ch_sums[2 * c];
-            p2 += ga * ch_sums[2 * c + 1];
-        }
+#pragma unroll 4
+        for (int c = h * s.k; c < (h + 1) * s.k; ++c) { p1 += ch_sums[2 * c]; p2 += ch_sums[2 * c + 1]; }
         const double mean = st0[2 * h], rstd = st0[2 * h + 1], lo = mean - (double)(float)mean;
         coef[2 * h] = (float)(rstd * (lo * rstd * p2 - p1) / m);
         coef[2 * h + 1] = (float)(-rstd * rstd * p2 / m);
@@ -508,7 +542,7 @@ constexpr int UNR = 4, SUNR = 8;                           // pixels in flight p
 template <typename T, int V, int SPAN>
 __global__ __launch_bounds__(NT) void gn_stats_kernel(const T* __restrict__ x, int ld, GnShape s, double* __restrict__ partial) {
     constexpr int NA = V / SPAN;
-    __shared__ double red[NA * 2][NT];
+    __shared__ double red[NA * 2][NT + PAD];
     Place at;
     at.set<V>(s);
     double a[NA], q[NA];
@@ -535,7 +569,7 @@ __global__ __launch_bounds__(NT) void gn_stats_kernel(const T* __restrict__ x, i
     }
 #pragma unroll
     for (int i = 0; i < NA; ++i) { red[2 * i][threadIdx.x] = a[i]; red[2 * i + 1][threadIdx.x] = q[i]; }
-    fold_slots(red, 2 * NA, at.slot, at.slots, s.cqb);
+    fold_slots(red, 2 * NA, at.slots, s.cqb);
     // channels to groups; groups without a channel in this slab get zeros, so that the slabs' rows can simply be added
     double* out = partial + (((size_t)blockIdx.y * s.chunks + blockIdx.x) * gridDim.z + blockIdx.z) * s.groups * 2;
     const int c_lo = blockIdx.z * s.cqb * V, c_hi = min(s.c, c_lo + s.cqb * V);
@@ -557,6 +591,7 @@ __global__ __launch_bounds__(64) void gn_finalize_kernel(const double* __restric
     const int g = blockIdx.x, n = blockIdx.y, lane = threadIdx.x;
     const double* p = partial + (size_t)n * rows * groups * 2;
     double a = 0.0, q = 0.0;
+#pragma unroll 8
     for (int r = lane; r < rows; r += 64) { a += p[((size_t)r * groups + g) * 2]; q += p[((size_t)r * groups + g) * 2 + 1]; }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) { a += __shfl_xor(a, o, 64); q += __shfl_xor(q, o, 64); }
@@ -577,6 +612,10 @@ __global__ __launch_bounds__(NT) void gn_fwd_kernel(const T* __restrict__ x, int
     at.set<V>(s);
     if (!at.active) return;
     const int n = blockIdx.y;
+    AffineIn<V> in;
+    in.params(gamma, beta, at.col);
+    in.groups(stats + (size_t)n * s.groups * 2, 0, at.col, s.k);
+    __builtin_amdgcn_sched_barrier(0);
     Affine<V> k;
     const T* xp = x + (size_t)n * s.hw * ld + at.col;
     const T* rp = RES ? res + (size_t)n * s.hw * res_ld + at.col : nullptr;
@@ -588,7 +627,7 @@ __global__ __launch_bounds__(NT) void gn_fwd_kernel(const T* __restrict__ x, int
             v[j].load(xp + (size_t)(r + j * at.slots) * ld);
             if constexpr (RES) w[j].load(rp + (size_t)(r + j * at.slots) * res_ld);
         }
-    }, [&] { k.load(stats + (size_t)n * s.groups * 2, 0, gamma, beta, at.col, s.k); }, [&](long long r) {
+    }, [&] { k.set(in); }, [&](long long r) {
 #pragma unroll
         for (int j = 0; j < UNR; ++j) fwd_vector<T, V, ACT, RES>(k, v[j], w[j], slope).store(yp + (size_t)(r + j * at.slots) * y_ld);
     }, [&](long long r) {
@@ -605,7 +644,7 @@ __global__ __launch_bounds__(NT) void gn_bwd_reduce_kernel(const T* __restrict__
                                                            const T* __restrict__ res, int res_ld, const double* __restrict__ stats,
                                                            const float* __restrict__ gamma, const float* __restrict__ beta,
                                                            float slope, GnShape s, float* __restrict__ partial) {
-    __shared__ float red[V * 2][NT];
+    __shared__ float red[V * 2][NT + PAD];
     Place at;
     at.set<V>(s);
     const int n = blockIdx.y;
@@ -614,6 +653,10 @@ __global__ __launch_bounds__(NT) void gn_bwd_reduce_kernel(const T* __restrict__
 #pragma unroll
     for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.f;
     if (at.active) {
+        AffineIn<V> in;
+        in.params(gamma, beta, at.col);
+        in.groups(st0, 0, at.col, s.k);
+        __builtin_amdgcn_sched_barrier(0);
         Affine<V> k;
         const T* gp = dy + (size_t)n * s.hw * dy_ld + at.col;
         const T* xp = x + (size_t)n * s.hw * ld + at.col;
@@ -640,9 +683,7 @@ __global__ __launch_bounds__(NT) void gn_bwd_reduce_kernel(const T* __restrict__
                 v[j].load(xp + (size_t)(r + j * at.slots) * ld);
                 if constexpr (RES) w[j].load(rp + (size_t)(r + j * at.slots) * res_ld);
             }
-        }, [&] {
-            k.load(st0, 0, gamma, beta, at.col, s.k);
-        }, [&](long long r) {
+        }, [&] { k.set(in); }, [&](long long r) {
             unsigned near = 0;
 #pragma unroll
             for (int j = 0; j < UNR; ++j) {
@@ -663,7 +704,7 @@ __global__ __launch_bounds__(NT) void gn_bwd_reduce_kernel(const T* __restrict__
     }
 #pragma unroll
     for (int i = 0; i < V; ++i) { red[2 * i][threadIdx.x] = s1[i]; red[2 * i + 1][threadIdx.x] = s2[i]; }
-    fold_slots(red, 2 * V, at.slot, at.slots, s.cqb);
+    fold_slots(red, 2 * V, at.slots, s.cqb);
     if (at.slot == 0 && at.active) {
         float* out = partial + (((size_t)n * s.chunks + blockIdx.x) * s.c + at.col) * 2;
 #pragma unroll
@@ -671,7 +712,8 @@ __global__ __launch_bounds__(NT) void gn_bwd_reduce_kernel(const T* __restrict__
     }
 }
 
-// The sums of one image's channels and the constants of its groups: a workgroup owns `bundle` groups of image blockIdx.y.
+// The sums of one image's channels and the constants of its groups: a workgroup owns `bundle` groups of image blockIdx.y, one
+// or as many as lie in 32 channels; its waves share the chunks, and the first one does the rest.
 // sums[image][channel] = {S1, S2};  dx = g * a + d * k2 + k1 with coef[image][group] = {k1, k2}
 constexpr int COEF_WAVES = 16;
 __global__ __launch_bounds__(64 * COEF_WAVES) void gn_bwd_coef_kernel(const float* __restrict__ partial, const double* __restrict__ stats,
@@ -680,10 +722,16 @@ __global__ __launch_bounds__(64 * COEF_WAVES) void gn_bwd_coef_kernel(const floa
     __shared__ double red[COEF_WAVES][64][2];
     const int n = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int g_lo = blockIdx.x * bundle, g_hi = min(s.groups, g_lo + bundle), c_lo = g_lo * s.k, c_hi = g_hi * s.k;
-    double* mine = sums + (size_t)n * s.c * 2;
+    double p1 = 0.0, p2 = 0.0;
     for (int c0 = c_lo; c0 < c_hi; c0 += 64) {
         const int c = c0 + lane;
-        double a = 0.0, b = 0.0;
+        double a = 0.0, b = 0.0, ga = 1.0, mean = 0.0, rstd = 0.0;
+        if (wave == 0 && c < c_hi) {
+            const double* st = stats + ((size_t)n * s.groups + c / s.k) * 2;
+            mean = st[0];
+            rstd = st[1];
+            if (gamma) ga = gamma[c];
+        }
         if (c < c_hi) {
             const float2* p = reinterpret_cast<const float2*>(partial) + (size_t)n * s.chunks * s.c + c;
 #pragma unroll 8
@@ -693,29 +741,38 @@ __global__ __launch_bounds__(64 * COEF_WAVES) void gn_bwd_coef_kernel(const floa
         red[wave][lane][1] = b;
         __syncthreads();
         if (wave == 0 && c < c_hi) {
+#pragma unroll
             for (int j = 1; j < COEF_WAVES; ++j) { a += red[j][lane][0]; b += red[j][lane][1]; }
-            const double* st = stats + ((size_t)n * s.groups + c / s.k) * 2;
-            mine[2 * c] = a;
-            mine[2 * c + 1] = (b - (st[0] - (double)(float)st[0]) * a) * st[1];          // xhat = (x - mean) * rstd
+            b = (b - (mean - (double)(float)mean) * a) * rstd;               // xhat = (x - mean) * rstd
+            double* out = sums + ((size_t)n * s.c + c) * 2;
+            out[0] = a;
+            out[1] = b;
+            p1 += ga * a;
+            p2 += ga * b;
         }
         __syncthreads();
     }
-    const double m = (double)s.hw * s.k;
-    for (int g = g_lo + wave; g < g_hi; g += COEF_WAVES) {           // a wave per group
-        double p1 = 0.0, p2 = 0.0;
-        for (int c = g * s.k + lane; c < (g + 1) * s.k; c += 64) {
-            const double ga = gamma ? (double)gamma[c] : 1.0;
-            p1 += ga * mine[2 * c];
-            p2 += ga * mine[2 * c + 1];
-        }
+    if (wave) return;
+    int groups = 1;
+    if (bundle == 1) {
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) { p1 += __shfl_xor(p1, o, 64); p2 += __shfl_xor(p2, o, 64); }
-        if (lane == 0) {
-            const double* st = stats + ((size_t)n * s.groups + g) * 2;
-            const double lo = st[0] - (double)(float)st[0];
-            coef[((size_t)n * s.groups + g) * 2] = (float)(st[1] * (lo * st[1] * p2 - p1) / m);
-            coef[((size_t)n * s.groups + g) * 2 + 1] = (float)(-st[1] * st[1] * p2 / m);
-        }
+    } else {                                                 // lane: channel -> lane: group
+        red[0][lane][0] = p1;
+        red[0][lane][1] = p2;
+        __builtin_amdgcn_wave_barrier();
+        groups = g_hi - g_lo;
+        p1 = p2 = 0.0;
+        if (lane < groups)
+            for (int c = lane * s.k; c < (lane + 1) * s.k; ++c) { p1 += red[0][c][0]; p2 += red[0][c][1]; }
+    }
+    if (lane < groups) {
+        const double m = (double)s.hw * s.k;
+        const double* st = stats + ((size_t)n * s.groups + g_lo + lane) * 2;
+        const double lo = st[0] - (double)(float)st[0];
+        float* out = coef + ((size_t)n * s.groups + g_lo + lane) * 2;
+        out[0] = (float)(st[1] * (lo * st[1] * p2 - p1) / m);
+        out[1] = (float)(-st[1] * st[1] * p2 / m);
     }
 }
 
@@ -737,8 +794,19 @@ __global__ __launch_bounds__(NT) void gn_bwd_apply_kernel(const T* __restrict__ 
     at.set<V>(s);
     if (!at.active) return;
     const double* st0 = stats + (size_t)n * s.groups * 2;
-    Affine<V> k;
+    AffineIn<V> in;
+    in.params(gamma, beta, at.col);
+    in.groups(st0, 0, at.col, s.k);
     float k1[V], k2[V];
+    GroupOf of(at.col, s.k);
+#pragma unroll
+    for (int i = 0; i < V; ++i, of.next()) {
+        const float* q = coef + ((size_t)n * s.groups + of.g) * 2;
+        k1[i] = q[0];
+        k2[i] = q[1];
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    Affine<V> k;
     const T* gp = dy + (size_t)n * s.hw * dy_ld + at.col;
     const T* xp = x + (size_t)n * s.hw * ld + at.col;
     const T* rp = RES ? res + (size_t)n * s.hw * res_ld + at.col : nullptr;
@@ -770,16 +838,7 @@ __global__ __launch_bounds__(NT) void gn_bwd_apply_kernel(const T* __restrict__ 
             v[j].load(xp + (size_t)(r + j * at.slots) * ld);
             if constexpr (RES) w[j].load(rp + (size_t)(r + j * at.slots) * res_ld);
         }
-    }, [&] {
-        k.load(st0, 0, gamma, beta, at.col, s.k);
-    GroupOf of(at.col, s.k);
-#pragma unroll
-    for (int i = 0; i < V; ++i, of.next()) {
-        const float* q = coef + ((size_t)n * s.groups + of.g) * 2;
-        k1[i] = q[0];
-        k2[i] = q[1];
-    }
-    }, [&](long long r) {
+    }, [&] { k.set(in); }, [&](long long r) {
         unsigned near = 0;
 #pragma unroll
         for (int j = 0; j < UNR; ++j) {
@@ -812,7 +871,8 @@ Plan make_plan(int dtype, int n, long long hw, int c, int groups, bool vec) {
     // Up to six workgroups per CU, as many as share both the trips of an image and the CUs evenly: 6x64x512x1024 bf16,
     // forward + backward, takes 584 us with 1,896 workgroups (7.4 per CU), 551 with 1,536; six rather than eight for
     // 2x64x512x1024, whose forward pass takes 50 us instead of 55.  A small image goes down to one trip per workgroup
-    // (6x512x64x128: 156 us, 165 with three trips; 3x80x77x131: 52 and 63).
+    // (3x80x77x131: 52 us, 63 with three trips), but four trips of three workgroups per CU are better than two of six
+    // (6x512x64x128 with residual: 149 us and 153).
     const long long trips = (hw + (long long)UNR * slots - 1) / ((long long)UNR * slots), per = (long long)n * p.zs;
     double best = 0.0;
     for (int w = 6; w >= 1; --w) {
@@ -821,7 +881,9 @@ Plan make_plan(int dtype, int n, long long hw, int c, int groups, bool vec) {
         if (chunks < 1) chunks = 1;
         const long long each = (trips + chunks - 1) / chunks;
         chunks = (trips + each - 1) / each;
-        const double even = (double)(trips * per) / (double)(each * ((per * chunks + 255) / 256 * 256));
+        const long long per_cu = (per * chunks + 255) / 256;
+        double even = (double)(trips * per) / (double)(each * per_cu * 256);
+        if (per_cu > 3 && each < 4) even *= 0.95;
         if (even > best * 1.02) { best = even; p.s.chunks = (int)chunks; }
     }
     return p;
@@ -956,7 +1018,7 @@ int ur_gn_act_fwd(const void* x, int x_ld, const void* residual, int res_ld, con
         GN_VEC_TYPE(dtype, {
             const int span = cell.k % V == 0 ? V : cell.k % 4 == 0 ? 4 : cell.k % 2 == 0 ? 2 : 1;
             const int na = V / span;
-            const size_t lds = sizeof(double) * ((na > 4 ? na : 2 * na) * CT + 2 * (cell.slab / cell.k));
+            const size_t lds = sizeof(double) * ((na > 4 ? na : 2 * na) * (CT + PAD) + 2 * (cell.slab / cell.k));
             const dim3 grid(n * cell.slabs);
             GN_K3(cell_vectors(cell, V), {
                 if (residual) hipLaunchKernelGGL((gn_fwd_cell_kernel<T, V, K, true>), grid, dim3(CT), lds, st, (const T*)x, x_ld, (const T*)residual, res_ld, gamma, beta, eps, act, slope, (T*)y, y_ld, stats, cell);
@@ -996,7 +1058,7 @@ int ur_gn_act_bwd(const void* dy, int dy_ld, const void* x, int x_ld, const void
     const Cell cell = make_cell(dtype, n, hw, c, groups, vec, BWD_MOST);
     if (cell.slabs) {
         GN_VEC_TYPE(dtype, {
-            const size_t lds = sizeof(float) * 2 * V * CT + sizeof(double) * 2 * cell.slab + sizeof(float) * 2 * (cell.slab / cell.k);
+            const size_t lds = sizeof(float) * 2 * V * (CT + PAD) + sizeof(double) * 2 * cell.slab + sizeof(float) * 2 * (cell.slab / cell.k);
             const dim3 grid(n * cell.slabs);
             double* to = n > 1 ? sums : nullptr;
             GN_K2(cell_vectors(cell, V), {
