@@ -195,8 +195,10 @@ def host():
         module = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(module)
         module.set_error_type(UResNetHipError)
-        module.set_entry_points(*(C.cast(getattr(lib, name), C.c_void_p).value for name in
-                                  ("ur_gn_fwd_workspace", "ur_gn_bwd_workspace", "ur_gn_act_fwd", "ur_gn_act_bwd", "ur_last_error")))
+        module.set_entry_points({name: C.cast(getattr(lib, name), C.c_void_p).value for name in
+                                 ("ur_gn_fwd_workspace", "ur_gn_bwd_workspace", "ur_gn_act_fwd", "ur_gn_act_bwd", "ur_param_table_max_rows",
+                                  "ur_param_table_bytes", "ur_param_table", "ur_grad_sqnorm_max_parts", "ur_grad_sqnorm", "ur_grad_clip",
+                                  "ur_adamw_multi", "ur_last_error")})
         _host = module
     return _host
 

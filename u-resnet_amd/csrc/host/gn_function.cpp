@@ -50,10 +50,6 @@ float* fptr(const at::Tensor& t) { return static_cast<float*>(ptr(t)); }
 
 void* stream_of(const at::Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 
-void check(int rc, const char* what) {
-    if (rc) throw std::runtime_error(std::string(what) + " failed: " + entry.last_error());
-}
-
 struct GnBackward : public Node {
     SavedVariable x, gamma, beta, residual;
     at::Tensor stats;

@@ -14,11 +14,19 @@ struct EntryPoints {
     decltype(&ur_gn_bwd_workspace) gn_bwd_workspace;
     decltype(&ur_gn_act_fwd) gn_act_fwd;
     decltype(&ur_gn_act_bwd) gn_act_bwd;
+    decltype(&ur_param_table_max_rows) param_table_max_rows;
+    decltype(&ur_param_table_bytes) param_table_bytes;
+    decltype(&ur_param_table) param_table;
+    decltype(&ur_grad_sqnorm_max_parts) grad_sqnorm_max_parts;
+    decltype(&ur_grad_sqnorm) grad_sqnorm;
+    decltype(&ur_grad_clip) grad_clip;
+    decltype(&ur_adamw_multi) adamw_multi;
     decltype(&ur_last_error) last_error;
 };
 extern EntryPoints entry;
 
 PyObject* fail(const std::string& text);                   // raises the package's error type
-PyObject* adamw_rows(PyObject* self, PyObject* args);
-PyObject* clip_rows(PyObject* self, PyObject* params);
+void check(int status, const char* what);                  // throws with the entry point's message
+PyObject* adamw_step(PyObject* self, PyObject* args);
+PyObject* clip_grads(PyObject* self, PyObject* args);
 PyObject* gn_act(PyObject* self, PyObject* args);

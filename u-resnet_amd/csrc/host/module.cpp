@@ -1,6 +1,8 @@
 #include "host.h"
 
 #include <exception>
+#include <stdexcept>
+#include <type_traits>
 
 EntryPoints entry = {};
 
@@ -15,15 +17,22 @@ PyObject* set_error_type(PyObject*, PyObject* type) {
     Py_RETURN_NONE;
 }
 
-// addresses in the order of EntryPoints
-PyObject* set_entry_points(PyObject*, PyObject* args) {
-    unsigned long long a[5];
-    if (!PyArg_ParseTuple(args, "KKKKK", &a[0], &a[1], &a[2], &a[3], &a[4])) return nullptr;
-    entry.gn_fwd_workspace = reinterpret_cast<decltype(entry.gn_fwd_workspace)>(a[0]);
-    entry.gn_bwd_workspace = reinterpret_cast<decltype(entry.gn_bwd_workspace)>(a[1]);
-    entry.gn_act_fwd = reinterpret_cast<decltype(entry.gn_act_fwd)>(a[2]);
-    entry.gn_act_bwd = reinterpret_cast<decltype(entry.gn_act_bwd)>(a[3]);
-    entry.last_error = reinterpret_cast<decltype(entry.last_error)>(a[4]);
+// entry points by name, as addresses
+PyObject* set_entry_points(PyObject*, PyObject* found) {
+    const auto take = [&](const char* name, auto& to) {
+        PyObject* v = PyDict_GetItemString(found, name);
+        if (!v) { PyErr_Format(PyExc_KeyError, "no entry point %s", name); return false; }
+        to = reinterpret_cast<std::remove_reference_t<decltype(to)>>(PyLong_AsUnsignedLongLong(v));
+        return !PyErr_Occurred();
+    };
+    if (!PyDict_Check(found)) return fail("entry points: a dict is expected");
+    if (!(take("ur_gn_fwd_workspace", entry.gn_fwd_workspace) && take("ur_gn_bwd_workspace", entry.gn_bwd_workspace) &&
+          take("ur_gn_act_fwd", entry.gn_act_fwd) && take("ur_gn_act_bwd", entry.gn_act_bwd) &&
+          take("ur_param_table_max_rows", entry.param_table_max_rows) && take("ur_param_table_bytes", entry.param_table_bytes) &&
+          take("ur_param_table", entry.param_table) && take("ur_grad_sqnorm_max_parts", entry.grad_sqnorm_max_parts) &&
+          take("ur_grad_sqnorm", entry.grad_sqnorm) && take("ur_grad_clip", entry.grad_clip) && take("ur_adamw_multi", entry.adamw_multi) &&
+          take("ur_last_error", entry.last_error)))
+        return nullptr;
     Py_RETURN_NONE;
 }
 
@@ -37,11 +46,11 @@ PyObject* guarded(PyObject* self, PyObject* args) {
     }
 }
 
-PyMethodDef methods[] = {{"adamw_rows", guarded<adamw_rows>, METH_VARARGS, "addresses of parameters and gradients"},
-                         {"clip_rows", guarded<clip_rows>, METH_O, "addresses and sizes of gradients"},
+PyMethodDef methods[] = {{"adamw_step", guarded<adamw_step>, METH_VARARGS, "one AdamW step over parameter groups"},
+                         {"clip_grads", guarded<clip_grads>, METH_VARARGS, "gradients scaled to a norm"},
                          {"gn_act", guarded<gn_act>, METH_VARARGS, "group norm with an activation, with its gradient"},
                          {"set_error_type", set_error_type, METH_O, "exception type for refused tensors"},
-                         {"set_entry_points", set_entry_points, METH_VARARGS, "addresses of the kernel library"},
+                         {"set_entry_points", set_entry_points, METH_O, "addresses of the kernel library"},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
@@ -50,6 +59,10 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, null
 PyObject* fail(const std::string& text) {
     PyErr_SetString(error_type ? error_type : PyExc_RuntimeError, text.c_str());
     return nullptr;
+}
+
+void check(int status, const char* what) {
+    if (status) throw std::runtime_error(std::string(what) + " failed: " + entry.last_error());
 }
 
 PyMODINIT_FUNC PyInit__host(void) { return PyModule_Create(&module); }

@@ -9,7 +9,6 @@
   checkpoints       the dict written at train_UResNetAblitionStudy.py:244-252 (save_checkpoint / load_checkpoint)
 """
 import array
-import ctypes as C
 import operator
 
 import torch
@@ -301,38 +300,6 @@ class SGD(_MultiTensorOptimizer):
         return loss
 
 
-class _ParamList:
-    """Tensors of one launch: addresses and sizes as int64 arrays in host memory (_lib.host()), their table and, where
-    the norm is taken, room for its partial sums in device memory."""
-    PARTS = 1024                                 # ur_grad_sqnorm_max_parts()
-    ROWS = 1024                                  # ur_param_table_max_rows()
-
-    @classmethod
-    def spans(cls, count):
-        """Slices of a list of `count` tensors that fit a table, as byte offsets into its int64 arrays and the first index."""
-        return [(slice(8 * a, 8 * min(a + cls.ROWS, count)), a) for a in range(0, count, cls.ROWS)]
-
-    def __init__(self, params, grads, sizes, device, parts=0):
-        self.params, self.grads, self.sizes, self.count = params, grads, sizes, len(sizes) // 8
-        self.bytes = -(-_lib.query("ur_param_table_bytes", self.count) // 16) * 16
-        self.buf = torch.empty(self.bytes + 8 * parts, dtype=torch.uint8, device=device)
-        self.table = self.buf.data_ptr()
-        self.parts = self.table + self.bytes
-        self.chunks = 0
-
-    def write(self, stream, blocks=None, steps=None, lr=0.0, betas=(0.0, 0.0)):
-        n = C.c_longlong()
-        _lib.call("ur_param_table", self.params, self.grads, self.sizes, blocks, self.count, self.table, self.bytes, steps, lr, betas[0],
-                  betas[1], C.byref(n), stream)
-        self.chunks = n.value
-
-    def sqnorm(self, parts, stream):
-        """Partial sums of the squared gradients at the address `parts`; returns their number."""
-        n = C.c_int()
-        _lib.call("ur_grad_sqnorm", self.table, self.count, self.chunks, parts, C.byref(n), stream)
-        return n.value
-
-
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
     """torch.nn.utils.clip_grad_norm_ for fp32 gradients on one GPU: scales them in place by min(1, max_norm / (norm + 1e-6))
     and returns their norm before that as a 0-dim device tensor.  No host synchronisation (except with error_if_nonfinite,
@@ -343,29 +310,8 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     max_norm = float(max_norm)
     if not max_norm >= 0:
         raise ValueError("clip_grad_norm_: max_norm must not be negative (got %r)" % (max_norm,))
-    grads, sizes, count, index = _lib.host().clip_rows([parameters] if torch.is_tensor(parameters) else list(parameters))
-    if index < 0:
-        return torch.tensor(0.0)
-    device = torch.device("cuda", index)
-    with ops._on(device):
-        if not count:
-            return torch.zeros((), device=device)
-        stream = ops._stream()
-        norm = torch.empty((), device=device)
-        spans = _ParamList.spans(count)
-        lists, nparts = [], 0
-        for span, _ in spans:
-            plist = _ParamList(None, grads[span], sizes[span], device, 0 if lists else _ParamList.PARTS * len(spans))
-            plist.write(stream)
-            lists.append(plist)
-            nparts += plist.sqnorm(lists[0].parts + 8 * nparts, stream)
-        if error_if_nonfinite:
-            total = lists[0].buf[lists[0].bytes:lists[0].bytes + 8 * nparts].view(torch.float64).sum()
-            if not bool(torch.isfinite(total)):
-                raise RuntimeError("clip_grad_norm_: the total norm of the gradients is not finite")
-        for plist in lists:
-            _lib.call("ur_grad_clip", plist.table, plist.count, plist.chunks, lists[0].parts, nparts, max_norm, norm.data_ptr(), stream)
-    return norm
+    norm = _lib.host().clip_grads([parameters] if torch.is_tensor(parameters) else list(parameters), max_norm, bool(error_if_nonfinite))
+    return torch.tensor(0.0) if norm is None else norm
 
 
 class _MomentPool:
@@ -396,6 +342,10 @@ class _MomentPool:
             for k in ('exp_avg', 'exp_avg_sq_root'):
                 self.buffers[k] = torch.zeros(many, dtype=torch.uint8, device=self.device).view(torch.float8_e4m3fn)
                 self.buffers[k + '_scale'] = torch.zeros(at, device=self.device)
+        moments = [buf.data_ptr() for buf in self.buffers.values()]
+        if self.bits == 8:                                     # codes before scales
+            moments = moments[0::2] + moments[1::2]
+        self.places = (self.blocks_there.data_ptr(), self.steps.data_ptr(), self.bits, *(moments + [0, 0])[:4])
         self.waiting = []                                      # parameters without a state: no gradient yet
         for i, p in enumerate(self.params):                    # what the others bring along
             old = state.get(p)
@@ -491,58 +441,17 @@ class AdamW(torch.optim.Optimizer):
                 loss = closure()
         if sum(len(pool.params) - len(pool.waiting) for pool in self._pools.values()) != len(self.state):
             self._pools = {}                                   # `state` was cleared or replaced: built again from it
-        work = []
-        for gi, group in enumerate(self.param_groups):
-            if not group['params']:
-                continue
-            pool, rows = self._pool(gi, group), _lib.host().adamw_rows
-            params, grads, live, uneven = rows(pool.params, pool.sizes, None)
-            held = None
-            if uneven:                                         # copies, until the launches that read them are queued
-                with torch.no_grad():
-                    held = [p.grad if p.grad is None else p.grad.contiguous() for p in pool.params]
-                params, grads, live, _ = rows(pool.params, pool.sizes, held)
-            if pool.waiting:
-                for i in [i for i in pool.waiting if pool.params[i].grad is not None]:
-                    pool.waiting.remove(i)
-                    self.state[pool.params[i]] = pool.views(i)
-            if live and any(grads):
-                work.append((group, pool, params, grads, held))
-        self.grad_norm = None
-        if work:
-            dev = work[0][1].device
-            if any(w[1].device != dev for w in work):
-                raise _lib.UResNetHipError("AdamW: all parameters must be on one GPU")
-            with ops._on(dev):
-                self._launch(work, dev)
+        pools = [(group, self._pool(gi, group)) for gi, group in enumerate(self.param_groups) if group['params']]
+        launched, self.grad_norm = _lib.host().adamw_step(
+            [(pool.params, pool.sizes, *pool.places, float(group['lr']), *group['betas'], group['eps'], group['weight_decay'])
+             for group, pool in pools], self.max_grad_norm, self.grad_scale)
+        for _, pool in pools:
+            for i in [i for i in pool.waiting if pool.params[i].grad is not None]:
+                pool.waiting.remove(i)
+                self.state[pool.params[i]] = pool.views(i)
+        if launched:
             ops.bump_weights_epoch()
         return loss
-
-    def _launch(self, work, dev):
-        stream = ops._stream()
-        clip = self.max_grad_norm is not None
-        lists, parts, nparts, norm = [], None, 0, None
-        work = [(group, pool, params[span], grads[span], pool.sizes[span], at) for group, pool, params, grads, _ in work
-                for span, at in _ParamList.spans(len(pool.params)) if any(grads[span])]
-        for group, pool, params, grads, sizes, at in work:
-            plist = _ParamList(params, grads, sizes, dev, _ParamList.PARTS * len(work) if clip and not lists else 0)
-            plist.write(stream, pool.blocks_there.data_ptr() + 8 * at, pool.steps.data_ptr() + 4 * at, float(group['lr']), group['betas'])
-            lists.append(plist)
-        if clip:
-            norm, parts = torch.empty((), device=dev), lists[0].parts
-            for plist in lists:
-                nparts += plist.sqnorm(parts + 8 * nparts, stream)
-        for (group, pool, *_), plist in zip(work, lists):
-            buf = pool.buffers
-            if pool.bits == 32:
-                state = (buf['exp_avg'].data_ptr(), buf['exp_avg_sq'].data_ptr(), None, None)
-            else:
-                state = (buf['exp_avg'].data_ptr(), buf['exp_avg_sq_root'].data_ptr(), buf['exp_avg_scale'].data_ptr(),
-                         buf['exp_avg_sq_root_scale'].data_ptr())
-            _lib.call("ur_adamw_multi", plist.table, plist.count, plist.chunks, pool.bits, *state, float(group['lr']), group['betas'][0],
-                      group['betas'][1], group['eps'], group['weight_decay'], parts, nparts, float(self.max_grad_norm or 0.0),
-                      float(self.grad_scale), ops._p(norm), stream)
-        self.grad_norm = norm
 
     def state_dict(self):
         sd = super().state_dict()
