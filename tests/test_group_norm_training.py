@@ -65,6 +65,39 @@ def test_fp32_network_matches_the_oracle(oracle, cls):
         assert rel_l2(ops.to_nchw_raw(model(x.to(DEV)), torch.float32).cpu(), ref(x)) < 2e-4
 
 
+@pytest.mark.parametrize("module, cls, oracle_cls, args, kwargs, shape", [
+    ("U_ResNet", "UNet", "UNet", (19, 3, 8), {}, (2, 3, 32, 64)),
+    ("U_ResNet", "UResNetNoResBlock", "UResNetNoResBlock", (19, 3, 8), {}, (2, 3, 32, 64)),
+    ("U_ResNet_CIFAR", "UResNet4_No_SU", "UResNet4_No_SU", (10, 3), {"scale": 3}, (2, 3, 32, 32)),
+    ("U_ResNet_CIFAR", "UResNet3_No_EUCB", "UResNet3_No_EUCB", (10, 3), {"scale": 3}, (2, 3, 32, 32)),
+    ("U_ResNet_CIFAR", "UResNet3_No_UBlock", "UResNet3_No_UBlock", (10, 3), {"scale": 3}, (2, 3, 32, 32)),
+    ("U_ResNet_CIFAR", "E_ResNet", "E_ResNet", (), {}, (2, 3, 32, 32)),
+    ("U_ResNet_MiniImageNet", "U_ResNet", "MiniU_ResNet", (100, 3), {}, (2, 3, 224, 224))])       # the size the class is made for
+def test_other_networks_match_the_oracle(oracle, module, cls, oracle_cls, args, kwargs, shape):
+    """Logits and gradient norms, at the tolerances of the same classes with BatchNorm."""
+    import uresnet_amd
+    torch.manual_seed(0)
+    ref = getattr(oracle, oracle_cls)(*args, **kwargs)
+    model = getattr(getattr(uresnet_amd.modules, module), cls)(*args, **kwargs).set_compute_dtype(torch.float32)
+    model.load_state_dict(ref.state_dict())
+    oracle_group_norm(ref, 8).train()
+    hnn.to_group_norm(model, 8).to(DEV).train()
+    g = torch.Generator().manual_seed(2)
+    x = torch.randn(shape, generator=g)
+    out, ro = model(x.to(DEV)), ref(x)
+    got = out if out.dim() == 2 else ops.to_nchw_raw(out, torch.float32)
+    dy = torch.randn(ro.shape, generator=g)
+    ro.backward(dy)
+    out.backward(dy.to(DEV))
+    assert rel_l2(got.detach().float().cpu(), ro.detach()) < 2e-4
+    want = dict(ref.named_parameters())
+    assert {k for k, p in model.named_parameters() if p.grad is None} == {k for k, p in want.items() if p.grad is None}
+    norms = [(p.grad.double().norm().item(), want[k].grad.double().norm().item()) for k, p in model.named_parameters() if p.grad is not None]
+    floor = 1e-5 * max(n for _, n in norms)
+    errs = sorted(abs(a - b) / b for a, b in norms if b > floor)
+    assert errs[len(errs) // 2] < 1e-4 and errs[-1] < 3e-2, (errs[len(errs) // 2], errs[-1])
+
+
 def test_bf16_network_tracks_fp32(oracle):
     _, a = pair(oracle, "UResNetNewEUCB", torch.float32)
     _, b = pair(oracle, "UResNetNewEUCB", torch.bfloat16)
@@ -138,3 +171,51 @@ def test_clipping_beside_the_other_optimisers(oracle):
     assert abs(results[0][0] - results[1][0]) < 1e-4 * results[1][0] and results[0][0] > 0.5
     for a, b in zip(results[0][1], results[1][1]):
         assert torch.allclose(a, b, rtol=2e-4, atol=0)
+
+
+SCRIPT = r'''
+import os, sys, torch
+import torch.distributed as dist
+sys.path.insert(0, os.environ["UR_ROOT"])
+import uresnet_amd
+from uresnet_amd import nn as hnn, train
+from uresnet_amd.modules.U_ResNet import UResNetNewEUCB
+
+torch.cuda.set_device(0)
+dev = torch.device("cuda", 0)
+dist.init_process_group("nccl", init_method="tcp://127.0.0.1:29543", rank=0, world_size=1, device_id=dev)
+g = torch.Generator().manual_seed(7)
+x = torch.randn(2, 3, 64, 96, generator=g).to(dev)
+y = torch.randint(0, 19, (2, 64, 96), generator=g).to(dev)
+for bits in (32, 8):
+    runs = []
+    for wrapped in (False, True):
+        torch.manual_seed(0)
+        m = hnn.to_group_norm(UResNetNewEUCB(19, 3, 8).set_compute_dtype(torch.float32), 8).to(dev).train()
+        opt = train.AdamW(m.parameters(), lr=1e-3, state_bits=bits, max_grad_norm=1.0)
+        ddp = uresnet_amd.ddp.DataParallel(m, bucket_mb=0.05) if wrapped else None
+        seen = []
+        for _ in range(3):
+            if ddp is None:
+                loss, _ = train.seg_train_step(m, opt, x, y)
+            else:
+                loss, _ = train.seg_train_step(m, opt, x, y, count_hook=ddp.count_hook, grad_hook=ddp.finish)
+            seen += [loss.item(), opt.grad_norm.item()]
+        runs.append(seen)
+        if wrapped:
+            assert {p.grad.data_ptr() % 16 for p in m.parameters() if p.grad is not None} == {0}
+    # the loss is divided by an all-reduced count: equal up to rounding, which the steps then carry on
+    assert all(abs(a - b) <= 1e-3 * abs(a) for a, b in zip(*runs)), runs
+dist.destroy_process_group()
+print("DDP_OK")
+'''
+
+
+def test_one_rank_data_parallel_step_with_group_norm_and_adamw():
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    env = dict(os.environ, UR_ROOT=root, HSA_ENABLE_IPC_MODE_LEGACY="0")
+    r = subprocess.run([sys.executable, "-c", SCRIPT], env=env, capture_output=True, text=True, timeout=240)
+    assert r.returncode == 0 and "DDP_OK" in r.stdout, r.stdout[-2000:] + r.stderr[-4000:]
