@@ -8,7 +8,12 @@
 //   dx = rstd * (gamma * g - P1 - xhat * P2),  dresidual = g
 //
 // Everything is bound by HBM: forward reads x (and the residual) and writes y, backward reads dy, x (and the residual) and
-// writes dx (and the residual's gradient).
+// writes dx (and the residual's gradient).  The sums need all of x (dy and x) before the first result, so what does not fit
+// the registers of one workgroup is read twice: three passes over a tensor forward and five backward instead of two and three.
+// Keeping an image in the registers of many workgroups that exchange their sums was slower (262 and 613 us for the shape
+// below), and so is counting on the last-level cache for the second read: it serves no faster than HBM here.
+// Measured, 6x64x512x1024 bf16 (403 MB a tensor): statistics 64 us (6.3 TB/s), forward 139 (5.8), sums of the backward pass 125
+// (6.4), gradient 198 (6.1); 64x64x32x32 fp32 in cells: forward 11 us, backward 19 + 4.
 //
 // Arithmetic.  The statistics are plain sums of x and x^2 in 64 bits: fp64 vector arithmetic runs at the fp32 rate here, a
 // sum costs four instructions per element against a budget of about thirteen at the HBM rate, and E[x^2] - mean^2 then
@@ -18,6 +23,8 @@
 // values, so one pre-activation on the wrong side of a kink by a rounding would put thousands of elements on the wrong
 // side: within the fp32 error of a kink the backward pass evaluates pre again in 64 bits (rare, one comparison otherwise).
 #include "ur_common.h"
+
+#include <type_traits>
 
 namespace {
 
@@ -130,21 +137,31 @@ struct Place {
         col = (blockIdx.z * s.cqb + cg) * V;
         active = slot < slots && col < s.c;
     }
-    // load(r) and full(r): U pixels r, r + slots, ...; once(): what full and one need besides, while the first loads are on
-    // their way; one(r): a single pixel (the end of the image)
-    template <int U, typename Load, typename Once, typename Full, typename One>
+    // load(h, r) and full(h, r): U pixels r, r + slots, ... into and out of buffer h; once(): what full and one need besides,
+    // while the first loads are on their way; one(r): a single pixel (the end of the image).  BUFFERS 2: a trip is loaded
+    // while the one before it is worked on.
+    template <int U, int BUFFERS, typename Load, typename Once, typename Full, typename One>
     __device__ __forceinline__ void walk(const GnShape& s, const Load& load, const Once& once, const Full& full, const One& one) const {
+        constexpr std::integral_constant<int, 0> first;
+        constexpr std::integral_constant<int, BUFFERS - 1> second;
         const long long step = (long long)s.chunks * U * slots;
         long long r = (long long)blockIdx.x * U * slots + slot;
-        bool whole = r + (U - 1) * slots < s.hw;
-        if (whole) load(r);
+        const auto whole = [&](long long at) { return at + (U - 1) * slots < s.hw; };
+        bool go = whole(r);
+        if (go) load(first, r);
         __builtin_amdgcn_sched_barrier(0);
         once();
-        while (whole) {
-            full(r);
+        const auto trip = [&](auto now, auto next) {
+            go = whole(r + step);
+            if (BUFFERS == 2 && go) load(next, r + step);
+            __builtin_amdgcn_sched_barrier(0);
+            full(now, r);
             r += step;
-            whole = r + (U - 1) * slots < s.hw;
-            if (whole) load(r);
+            if (BUFFERS == 1 && go) load(next, r);
+        };
+        while (go) {
+            trip(first, second);
+            if (BUFFERS == 2 && go) trip(second, first);
         }
         for (; r < s.hw; r += slots) one(r);
     }
@@ -536,7 +553,10 @@ __global__ __launch_bounds__(NT) void gn_params_kernel(const double* __restrict_
 
 // ================================================================== streaming passes
 // Large sizes: two passes over memory with the sums of all workgroups between them.
-constexpr int UNR = 4, SUNR = 8;                           // pixels in flight per thread; in the statistics
+// pixels a thread loads at a time; in the statistics.  The last backward pass loads a trip ahead (6x64x512x1024 bf16 204 -> 198
+// us, 6x512x64x128 with residual 57 -> 54); the forward pass gains nothing by it (139 and 138), and the sums of the first
+// backward pass leave too few registers (125 -> 135).
+constexpr int UNR = 4, SUNR = 8;
 
 // SPAN: channels of a vector that share a group (a power of two that divides both V and k): V / SPAN pairs of sums per thread
 template <typename T, int V, int SPAN>
@@ -559,10 +579,10 @@ __global__ __launch_bounds__(NT) void gn_stats_kernel(const T* __restrict__ x, i
             }
         };
         Chunk<T, V> v[SUNR];
-        at.walk<SUNR>(s, [&](long long r) {
+        at.walk<SUNR, 1>(s, [&](auto, long long r) {
 #pragma unroll
             for (int j = 0; j < SUNR; ++j) v[j].load(p + (size_t)(r + j * at.slots) * ld);
-        }, [] {}, [&](long long) {
+        }, [] {}, [&](auto, long long) {
 #pragma unroll
             for (int j = 0; j < SUNR; ++j) add(v[j]);
         }, [&](long long r) { Chunk<T, V> e; e.load(p + (size_t)r * ld); add(e); });
@@ -621,13 +641,13 @@ __global__ __launch_bounds__(NT) void gn_fwd_kernel(const T* __restrict__ x, int
     const T* rp = RES ? res + (size_t)n * s.hw * res_ld + at.col : nullptr;
     T* yp = y + (size_t)n * s.hw * y_ld + at.col;
     Chunk<T, V> v[UNR], w[UNR];
-    at.walk<UNR>(s, [&](long long r) {
+    at.walk<UNR, 1>(s, [&](auto, long long r) {
 #pragma unroll
         for (int j = 0; j < UNR; ++j) {
             v[j].load(xp + (size_t)(r + j * at.slots) * ld);
             if constexpr (RES) w[j].load(rp + (size_t)(r + j * at.slots) * res_ld);
         }
-    }, [&] { k.set(in); }, [&](long long r) {
+    }, [&] { k.set(in); }, [&](auto, long long r) {
 #pragma unroll
         for (int j = 0; j < UNR; ++j) fwd_vector<T, V, ACT, RES>(k, v[j], w[j], slope).store(yp + (size_t)(r + j * at.slots) * y_ld);
     }, [&](long long r) {
@@ -676,14 +696,14 @@ __global__ __launch_bounds__(NT) void gn_bwd_reduce_kernel(const T* __restrict__
             add(g, d);
         };
         Chunk<T, V> u[UNR], v[UNR], w[UNR];
-        at.walk<UNR>(s, [&](long long r) {
+        at.walk<UNR, 1>(s, [&](auto, long long r) {
 #pragma unroll
             for (int j = 0; j < UNR; ++j) {
                 u[j].load(gp + (size_t)(r + j * at.slots) * dy_ld);
                 v[j].load(xp + (size_t)(r + j * at.slots) * ld);
                 if constexpr (RES) w[j].load(rp + (size_t)(r + j * at.slots) * res_ld);
             }
-        }, [&] { k.set(in); }, [&](long long r) {
+        }, [&] { k.set(in); }, [&](auto, long long r) {
             unsigned near = 0;
 #pragma unroll
             for (int j = 0; j < UNR; ++j) {
@@ -830,20 +850,20 @@ __global__ __launch_bounds__(NT) void gn_bwd_apply_kernel(const T* __restrict__ 
             settle<T, V, ACT, RES>(gp + (size_t)r * dy_ld, xp + (size_t)r * ld, RES ? rp + (size_t)r * res_ld : nullptr, slope, st0, 0, gamma, beta, at.col, s.k, g);
         write(g, d, r);
     };
-    Chunk<T, V> u[UNR], v[UNR], w[UNR];
-    at.walk<UNR>(s, [&](long long r) {
+    Chunk<T, V> u[2][UNR], v[2][UNR], w[2][UNR];
+    at.walk<UNR, 2>(s, [&](auto h, long long r) {
 #pragma unroll
         for (int j = 0; j < UNR; ++j) {
-            u[j].load(gp + (size_t)(r + j * at.slots) * dy_ld);
-            v[j].load(xp + (size_t)(r + j * at.slots) * ld);
-            if constexpr (RES) w[j].load(rp + (size_t)(r + j * at.slots) * res_ld);
+            u[h][j].load(gp + (size_t)(r + j * at.slots) * dy_ld);
+            v[h][j].load(xp + (size_t)(r + j * at.slots) * ld);
+            if constexpr (RES) w[h][j].load(rp + (size_t)(r + j * at.slots) * res_ld);
         }
-    }, [&] { k.set(in); }, [&](long long r) {
+    }, [&] { k.set(in); }, [&](auto h, long long r) {
         unsigned near = 0;
 #pragma unroll
         for (int j = 0; j < UNR; ++j) {
             float g[V], d[V];
-            near |= (unsigned)bwd_vector<T, V, ACT, RES>(k, u[j], v[j], w[j], slope, g, d) << j;
+            near |= (unsigned)bwd_vector<T, V, ACT, RES>(k, u[h][j], v[h][j], w[h][j], slope, g, d) << j;
             write(g, d, r + j * at.slots);
             __builtin_amdgcn_sched_barrier(0);             // vector by vector, as above
         }
