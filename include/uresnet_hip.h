@@ -455,6 +455,7 @@ int ur_seg_metrics_accumulate(const unsigned long long* cm, int classes, const f
  * x, residual, y and dy are NHWC with pixel pitches *_ld (0 = dense), dx and dres dense.  gamma / beta may be NULL (1 / 0).
  * act: UR_ACT_*, slope for UR_ACT_LEAKYRELU.  stats: double[n][groups][2] = {mean, 1 / sqrt(var + eps)}, written by the
  * forward and read by the backward pass.  Backward: any of dx, dres, dgamma, dbeta may be NULL (dres needs residual and dx).
+ * Outputs share nothing with inputs; n <= 65534, c <= 16384.
  * Sums are in a fixed order: the same call gives the same bits.  Workspace bytes: ur_gn_*_workspace (0: bad sizes). */
 size_t ur_gn_fwd_workspace(int dtype, int n, long long hw, int c, int groups);
 size_t ur_gn_bwd_workspace(int dtype, int n, long long hw, int c, int groups);

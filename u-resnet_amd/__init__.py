@@ -2,11 +2,12 @@
 
 Layout
   csrc/        hand-written HIP kernels + the C ABI (include/uresnet_hip.h) -> lib/liburesnet_hip.so
+  csrc/host/   host code against torch's C++ interface -> lib/_host.so
   _lib.py      ctypes binding (fails loudly when the library is missing)
   ops.py       autograd operators over the C ABI (NHWC activations, fp32 parameters)
   nn.py        torch.nn-compatible leaf layers whose forwards call ops
   modules/     the reference's model files, class for class
-  train.py     losses, masks, multi-tensor Adam/SGD, training steps
+  train.py     losses, masks, multi-tensor Adam/AdamW/SGD, gradient clipping, training steps
   ddp.py       one-process-per-GPU data parallelism (bucketed RCCL all-reduce)
 
 The directory name contains a hyphen; import it as `uresnet_amd` (the alias module at the
