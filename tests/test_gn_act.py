@@ -399,6 +399,29 @@ def test_double_backward_and_bad_arguments_are_refused():
 
 
 @pytest.mark.gpu
+def test_saved_tensors_may_come_back_in_another_layout():
+    """Saved-tensor hooks: an offload to the host that returns channels-first tensors (of a channel window as well), and one
+    that returns something else."""
+    x, dy, r, gn = make((2, 8, 6, 5, 4), torch.bfloat16, 16, residual=True)
+    buf = torch.randn(2, 24, 6, 5, device=DEV).to(torch.bfloat16).contiguous(memory_format=torch.channels_last)
+    gn = gn.to(DEV)
+    dyd = dy.to(DEV)
+
+    def grads():
+        a, b = ops.alias_window(buf, 8, 8).requires_grad_(), r.to(DEV).contiguous(memory_format=torch.channels_last).requires_grad_()
+        return torch.autograd.grad(ops.gn_act(a, gn, residual=b), [a, b, gn.weight, gn.bias], dyd)
+    ops.alias_window(buf, 8, 8).copy_(x.to(DEV))
+    want = grads()
+    with torch.autograd.graph.save_on_cpu(pin_memory=True):
+        assert all(torch.equal(p, q) for p, q in zip(grads(), want))
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.clone(memory_format=torch.contiguous_format), lambda t: t):
+        assert all(torch.equal(p, q) for p, q in zip(grads(), want))
+    for change in (lambda t: t.cpu(), lambda t: t.double(), lambda t: t[:1]):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, change), pytest.raises(RuntimeError, match="saved-tensor hook"):
+            grads()
+
+
+@pytest.mark.gpu
 def test_gradients_against_differences():
     """Central differences in the fp32 kernel: truncation h^2 and rounding 2^-24 |y| sqrt(N) / h leave 1e-3 at h = 1e-2."""
     x, dy, r, gn = make((1, 8, 3, 5, 2), torch.float32, 12, residual=True)

@@ -22,7 +22,7 @@ using torch::autograd::variable_list;
 constexpr auto CL = at::MemoryFormat::ChannelsLast;
 
 struct Shape {
-    int x_ld, res_ld, dtype, n, c, groups, act;
+    int dtype, n, c, groups, act;
     long long hw;
     float slope;
 };
@@ -65,6 +65,19 @@ struct GnBackward : public Node {
         stats.reset();
     }
 
+    int layout(at::Tensor& t, at::IntArrayRef sizes, const char* what) const {
+        if (t.device() != stats.device() || t.scalar_type() != (s.dtype == UR_BF16 ? at::kBFloat16 : at::kFloat) || t.sizes() != sizes)
+            throw std::runtime_error(std::string("gn_act: ") + what + " came back from its saved-tensor hook with another type, shape or device");
+        if (const int ld = pitch(t)) return ld;
+        t = t.contiguous(CL);
+        return s.c;
+    }
+    at::Tensor channel_values(const at::Tensor& t) const {
+        if (t.device() != stats.device() || t.scalar_type() != at::kFloat || t.numel() != s.c)
+            throw std::runtime_error("gn_act: a parameter came back from its saved-tensor hook with another type, shape or device");
+        return t.contiguous();
+    }
+
     variable_list apply(variable_list&& grads) override {
         variable_list out(4);
         at::Tensor dy = grads[0];
@@ -75,9 +88,13 @@ struct GnBackward : public Node {
         if (passes_dy && want_res) out[3] = dy;
         const bool want_dres = !passes_dy && want_res;
         if (!(want_x || want_gamma || want_beta || want_dres)) return out;
-        const at::Tensor xs = x.unpack(), gs = gamma.unpack(), bs = beta.unpack(), rs = residual.unpack();
+        at::Tensor xs = x.unpack(), gs = gamma.unpack(), bs = beta.unpack(), rs = residual.unpack();
         if (!stats.defined()) throw std::runtime_error("gn_act: backward through the same graph a second time (retain_graph=True keeps it)");
-        const c10::DeviceGuard guard(xs.device());
+        const c10::DeviceGuard guard(stats.device());
+        // what comes back may be laid out in another way than what was saved (saved-tensor hooks)
+        const int x_ld = layout(xs, dy.sizes(), "x"), res_ld = rs.defined() ? layout(rs, dy.sizes(), "the residual") : 0;
+        for (at::Tensor* p : {&gs, &bs})
+            if (p->defined()) *p = channel_values(*p);
         if (dy.scalar_type() != xs.scalar_type()) dy = dy.to(xs.scalar_type());
         int dy_ld = pitch(dy);
         if (!dy_ld) { dy = dy.contiguous(CL); dy_ld = s.c; }
@@ -88,7 +105,7 @@ struct GnBackward : public Node {
         if (want_beta) out[2] = at::empty({s.c}, xs.options().dtype(at::kFloat));
         const size_t bytes = entry.gn_bwd_workspace(s.dtype, s.n, s.hw, s.c, s.groups);
         const at::Tensor ws = at::empty({(int64_t)bytes}, xs.options().dtype(at::kByte));
-        check(entry.gn_act_bwd(ptr(dy), dy_ld, ptr(xs), s.x_ld, ptr(rs), s.res_ld, fptr(gs), fptr(bs), static_cast<double*>(ptr(stats)),
+        check(entry.gn_act_bwd(ptr(dy), dy_ld, ptr(xs), x_ld, ptr(rs), res_ld, fptr(gs), fptr(bs), static_cast<double*>(ptr(stats)),
                                ptr(out[0]), ptr(dres), fptr(out[1]), fptr(out[2]), s.dtype, s.n, s.hw, s.c, s.groups, s.act, s.slope, ptr(ws),
                                bytes, stream_of(xs)),
               "ur_gn_act_bwd");
@@ -101,8 +118,6 @@ struct GnBackward : public Node {
 at::Tensor forward(const at::Tensor& x, const at::Tensor& gamma, const at::Tensor& beta, const at::Tensor& residual, at::Tensor z, int groups,
                    double eps, int act, double slope) {
     Shape s;
-    s.x_ld = pitch(x);
-    s.res_ld = residual.defined() ? pitch(residual) : 0;
     s.dtype = x.scalar_type() == at::kBFloat16 ? UR_BF16 : UR_F32;
     s.n = (int)x.size(0);
     s.c = (int)x.size(1);
@@ -119,7 +134,7 @@ at::Tensor forward(const at::Tensor& x, const at::Tensor& gamma, const at::Tenso
         stats = at::empty({s.n, groups, 2}, x.options().dtype(at::kDouble));
         const size_t bytes = entry.gn_fwd_workspace(s.dtype, s.n, s.hw, s.c, groups);
         const at::Tensor ws = at::empty({(int64_t)(bytes ? bytes : 16)}, x.options().dtype(at::kByte));
-        check(entry.gn_act_fwd(ptr(x), s.x_ld, ptr(residual), s.res_ld, fptr(gamma), fptr(beta), ptr(z), pitch(z), static_cast<double*>(ptr(stats)),
+        check(entry.gn_act_fwd(ptr(x), pitch(x), ptr(residual), residual.defined() ? pitch(residual) : 0, fptr(gamma), fptr(beta), ptr(z), pitch(z), static_cast<double*>(ptr(stats)),
                                s.dtype, s.n, s.hw, s.c, groups, (float)eps, act, s.slope, ptr(ws), bytes, stream_of(x)),
               "ur_gn_act_fwd");
     }
@@ -132,7 +147,6 @@ at::Tensor forward(const at::Tensor& x, const at::Tensor& gamma, const at::Tenso
         // without an activation nothing depends on the residual's values
         node->passes_dy = residual.defined() && act == UR_ACT_NONE;
         node->residual = SavedVariable(act == UR_ACT_NONE ? at::Tensor() : residual, false);
-        if (act == UR_ACT_NONE) s.res_ld = 0;
         node->stats = stats;
         node->s = s;
         torch::autograd::set_history(z, node);

@@ -116,7 +116,8 @@ def wants_stats(norm):
 
 def to_group_norm(module, num_groups=32):
     """Replace every BatchNorm2d inside `module` by a GroupNorm over the same channels, in place, and return the module (a
-    BatchNorm2d itself: its replacement).  Weight, bias, eps and training mode are kept, running statistics are dropped.
+    BatchNorm2d itself: its replacement).  Weight, bias, eps and training mode are kept, running statistics and hooks are
+    dropped.
     num_groups: the largest number of groups; layers whose channels it does not divide get the largest divisor below it.
     Call it before an optimiser or a data-parallel wrapper takes the parameters."""
     if int(num_groups) < 1:
