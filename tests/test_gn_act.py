@@ -482,6 +482,36 @@ def test_the_same_call_gives_the_same_bits_on_any_stream_and_in_a_replayed_graph
 
 
 @pytest.mark.gpu
+def test_a_captured_backward_pass_beside_a_live_eager_graph_is_refused():
+    x, dy, _, gn = make((2, 16, 9, 5, 4), torch.bfloat16, 17)
+    gn = gn.to(DEV)
+    xd, dyd = (t.to(DEV).contiguous(memory_format=torch.channels_last) for t in (x, dy))
+
+    def step():
+        a = xd.detach().requires_grad_()
+        y = ops.gn_act(a, gn)
+        return torch.autograd.grad(y, [a, gn.weight, gn.bias], dyd)
+    want = [t.clone() for t in step()]
+    alive = ops.gn_act(xd, gn)                                  # holds the accumulators of weight and bias, on the default stream
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="still alive"):
+        with torch.cuda.graph(graph, capture_error_mode="thread_local"):
+            step()
+    torch.cuda.synchronize()
+    alive.backward(dyd)                                         # the eager graph is unharmed
+    assert torch.equal(gn.weight.grad, want[1]) and torch.equal(gn.bias.grad, want[2])
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, capture_error_mode="thread_local"):
+        out = step()
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(out, want))
+
+
+@pytest.mark.gpu
 def test_two_calls_at_once_on_two_streams():
     a = make((2, 64, 96, 80, 32), torch.bfloat16, 15)
     b = make((3, 32, 50, 60, 4), torch.float32, 16)

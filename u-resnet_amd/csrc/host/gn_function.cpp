@@ -4,6 +4,7 @@
 #include <ATen/ATen.h>
 #include <ATen/core/grad_mode.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/utils.h>
@@ -78,11 +79,28 @@ struct GnBackward : public Node {
         return t.contiguous();
     }
 
+    // A captured backward pass cannot hand a gradient on to the default stream, which does not take part in the capture: what
+    // was recorded there eagerly and is still alive (a leaf's accumulator in another, live graph) would end the process
+    void refuse_capture_into_eager_graph(c10::Device device) const {
+        if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+        // by number: the graph's streams carry torch's device type, these HIP's, and so never compare equal
+        const c10::StreamId eager = c10::hip::getDefaultHIPStream(device.index()).id();
+        for (uint32_t i = 0; i < num_outputs(); ++i) {
+            const auto& next = next_edge(i).function;
+            if (!next || !task_should_compute_output(i)) continue;
+            const auto on = next->stream();
+            if (on && on->id() == eager)
+                throw std::runtime_error("gn_act: the captured backward pass reaches a tensor whose graph was recorded outside the capture and "
+                                         "is still alive: drop what an eager forward pass returned before capturing");
+        }
+    }
+
     variable_list apply(variable_list&& grads) override {
         variable_list out(4);
         at::Tensor dy = grads[0];
         if (!dy.defined()) return out;
         if (at::GradMode::is_enabled()) throw std::runtime_error("gn_act: no double backward (create_graph=True)");
+        refuse_capture_into_eager_graph(dy.device());
         const bool want_x = task_should_compute_output(0), want_gamma = task_should_compute_output(1), want_beta = task_should_compute_output(2),
                    want_res = task_should_compute_output(3);
         if (passes_dy && want_res) out[3] = dy;
