@@ -207,13 +207,18 @@ struct GroupOf {
 
 // the constants of V channels of one image: pre = (x - mean_hi) * a + b.  They are fetched first, so that they arrive while
 // the loads of the data are on their way
+// (a module without parameters reads zeros and adds one: a branch around each load would wait for it, sixteen times in turn)
+__device__ const float gn_zeros[8] = {};
 template <int V> struct AffineIn {
-    float ga[V], be[V];
+    float ga[V], be[V], one;
     double mean[V], rstd[V];
     __device__ __forceinline__ void params(const float* __restrict__ gamma, const float* __restrict__ beta, int col) {
+        const float *g = gamma ? gamma + col : gn_zeros, *b = beta ? beta + col : gn_zeros;
+        one = gamma ? 0.f : 1.f;
 #pragma unroll
-        for (int i = 0; i < V; ++i) { ga[i] = gamma ? gamma[col + i] : 1.f; be[i] = beta ? beta[col + i] : 0.f; }
+        for (int i = 0; i < V; ++i) { ga[i] = g[i]; be[i] = b[i]; }
     }
+    __device__ __forceinline__ double weight(int i) const { return (double)(ga[i] + one); }
     // stats: {mean, rstd} of the groups from g0 on
     __device__ __forceinline__ void groups(const double* stats, int g0, int col, int k) {
         GroupOf at(col, k);
@@ -226,7 +231,7 @@ template <int V> struct Affine {
     __device__ __forceinline__ void set(const AffineIn<V>& in) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            const double s = in.rstd[i] * (double)in.ga[i];
+            const double s = in.rstd[i] * in.weight(i);
             m[i] = (float)in.mean[i];
             a[i] = (float)s;
             b[i] = (float)((double)in.be[i] - (in.mean[i] - (double)m[i]) * s);
@@ -476,7 +481,7 @@ _Pragma("unroll")
             const double a = red[2 * i][threadIdx.x], b = red[2 * i + 1][threadIdx.x];
             const double q = (b - (st[0] - (double)(float)st[0]) * a) * st[1];         // xhat = (x - mean) * rstd
             const int c = at.col + i;
-            const double ga = gamma ? (double)gamma[c] : 1.0;
+            const double ga = in.weight(i);
             ch_sums[2 * (c - at.c0)] = ga * a;
             ch_sums[2 * (c - at.c0) + 1] = ga * q;
             if (sums) {
