@@ -305,7 +305,8 @@ struct Cell {
 
 struct CellPlace {
     int n, c0, sc, cqs, slot, slots, cg, col;
-    bool active;
+    bool active;                                           // (the others have a channel vector, too, and load without a branch: a
+                                                           // branch around a load waits for it and for all before it)
     template <int V> __device__ __forceinline__ void set(const Cell& s) {
         n = blockIdx.x / s.slabs;
         c0 = (blockIdx.x - n * s.slabs) * s.slab;
@@ -328,15 +329,12 @@ __global__ __launch_bounds__(CT) void gn_fwd_cell_kernel(const T* __restrict__ x
     at.set<V>(s);
     const size_t row0 = (size_t)at.n * s.hw;
     AffineIn<V> in;
-    if (at.active) in.params(gamma, beta, at.col);
+    in.params(gamma, beta, at.col);
     __builtin_amdgcn_sched_barrier(0);
     Chunk<T, V> v[K];
     const T* xp = x + row0 * ld + at.col;
 #pragma unroll
-    for (int j = 0; j < K; ++j) {
-        const int r = at.slot + j * at.slots;
-        if (at.active && r < s.hw) v[j].load(xp + (size_t)r * ld);
-    }
+    for (int j = 0; j < K; ++j) v[j].load(xp + (size_t)min(at.slot + j * at.slots, s.hw - 1) * ld);
     double a[V], q[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) a[i] = q[i] = 0.0;
@@ -444,15 +442,17 @@ __global__ __launch_bounds__(CT) void gn_bwd_cell_kernel(const T* __restrict__ d
     const T* xp = x + row0 * ld + at.col;
     const T* rp = RES ? res + row0 * res_ld + at.col : nullptr;
     AffineIn<V> in;
-    if (at.active) { in.params(gamma, beta, at.col); in.groups(st0, g0, at.col, s.k); }
+    in.params(gamma, beta, at.col);
+    in.groups(st0, g0, at.col, s.k);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int j = 0; j < K; ++j) {
-        const int r = at.slot + j * at.slots;
-        if (at.active && r < s.hw) { u[j].load(gp + (size_t)r * dy_ld); v[j].load(xp + (size_t)r * ld); }
+        const int r = min(at.slot + j * at.slots, s.hw - 1);
+        u[j].load(gp + (size_t)r * dy_ld);
+        v[j].load(xp + (size_t)r * ld);
     }
     Affine<V> k;
-    if (at.active) k.set(in);
+    k.set(in);
     float s1[V], s2[V], g[V], d[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.f;
