@@ -283,6 +283,19 @@ __device__ __forceinline__ void settle(const T* dy, const T* x, const T* res, fl
     }
 }
 
+// a vector near a kink, from memory again, outside of the unrolled loops (their code would be several times as long)
+template <typename T, int V, int ACT, bool RES>
+__device__ __forceinline__ void again(const Affine<V>& k, long long r, const T* dy, int dy_ld, const T* x, int ld, const T* res, int res_ld, float slope,
+                                      const double* stats, int g0, const float* __restrict__ gamma, const float* __restrict__ beta, int col, int per,
+                                      float (&g)[V], float (&d)[V]) {
+    Chunk<T, V> u, v, w;
+    u.load(dy + (size_t)r * dy_ld);
+    v.load(x + (size_t)r * ld);
+    if constexpr (RES) w.load(res + (size_t)r * res_ld);
+    if (bwd_vector<T, V, ACT, RES>(k, u, v, w, slope, g, d))
+        settle<T, V, ACT, RES>(dy + (size_t)r * dy_ld, x + (size_t)r * ld, RES ? res + (size_t)r * res_ld : nullptr, slope, stats, g0, gamma, beta, col, per, g);
+}
+
 #define GN_ACT(act, ...)                                                              \
     switch (act) {                                                                    \
     case UR_ACT_NONE: { constexpr int ACT = UR_ACT_NONE; __VA_ARGS__; } break;         \
@@ -458,16 +471,22 @@ __global__ __launch_bounds__(CT) void gn_bwd_cell_kernel(const T* __restrict__ d
     for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.f;
     if (at.active) {
         GN_ACT(act, {
+            unsigned near = 0;
 _Pragma("unroll")
             for (int j = 0; j < K; ++j) {
                 const int r = at.slot + j * at.slots;
                 if (r < s.hw) {
                     if constexpr (RES) w.load(rp + (size_t)r * res_ld);
-                    if (bwd_vector<T, V, ACT, RES>(k, u[j], v[j], w, slope, g, d))
-                        settle<T, V, ACT, RES>(gp + (size_t)r * dy_ld, xp + (size_t)r * ld, RES ? rp + (size_t)r * res_ld : nullptr, slope, st0, g0, gamma, beta, at.col, s.k, g);
+                    const bool skip = bwd_vector<T, V, ACT, RES>(k, u[j], v[j], w, slope, g, d);
+                    near |= (unsigned)skip << j;
 _Pragma("unroll")
-                    for (int i = 0; i < V; ++i) { s1[i] += g[i]; s2[i] = fmaf(g[i], d[i], s2[i]); }
+                    for (int i = 0; i < V; ++i) { g[i] = skip ? 0.f : g[i]; s1[i] += g[i]; s2[i] = fmaf(g[i], d[i], s2[i]); }
                 }
+            }
+            for (; near; near &= near - 1) {               // rare
+                again<T, V, ACT, RES>(k, at.slot + __builtin_ctz(near) * at.slots, gp, dy_ld, xp, ld, rp, res_ld, slope, st0, g0, gamma, beta, at.col, s.k, g, d);
+_Pragma("unroll")
+                for (int i = 0; i < V; ++i) { s1[i] += g[i]; s2[i] = fmaf(g[i], d[i], s2[i]); }
             }
         });
     }
@@ -512,24 +531,31 @@ _Pragma("unroll")
     for (int i = 0; i < V; ++i, of.next()) { k1[i] = coef[2 * (of.g - g0)]; k2[i] = coef[2 * (of.g - g0) + 1]; }
     T* op = dx + row0 * s.c + at.col;
     T* qp = RES && dres ? dres + row0 * s.c + at.col : nullptr;
+    const auto write = [&](int r) {
+        Chunk<T, V> o, t;
+#pragma unroll
+        for (int i = 0; i < V; ++i) d[i] = fmaf(g[i], k.a[i], fmaf(d[i], k2[i], k1[i]));
+        o.put(d);
+        o.store(op + (size_t)r * s.c);
+        if constexpr (RES) { if (qp) { t.put(g); t.store(qp + (size_t)r * s.c); } }
+    };
     GN_ACT(act, {
+        unsigned near = 0;
 _Pragma("unroll")
         for (int j = 0; j < K; ++j) {
             const int r = at.slot + j * at.slots;
             if (r < s.hw) {
-                Chunk<T, V> o, t;
                 if constexpr (RES) w.load(rp + (size_t)r * res_ld);
                 u[j].forget();
                 v[j].forget();
-                if (bwd_vector<T, V, ACT, RES>(k, u[j], v[j], w, slope, g, d))
-                    settle<T, V, ACT, RES>(gp + (size_t)r * dy_ld, xp + (size_t)r * ld, RES ? rp + (size_t)r * res_ld : nullptr, slope, st0, g0, gamma, beta, at.col, s.k, g);
-_Pragma("unroll")
-                for (int i = 0; i < V; ++i) d[i] = fmaf(g[i], k.a[i], fmaf(d[i], k2[i], k1[i]));
-                o.put(d);
-                t.put(g);
-                o.store(op + (size_t)r * s.c);
-                if constexpr (RES) { if (qp) t.store(qp + (size_t)r * s.c); }
+                near |= (unsigned)bwd_vector<T, V, ACT, RES>(k, u[j], v[j], w, slope, g, d) << j;
+                write(r);
             }
+        }
+        for (; near; near &= near - 1) {                   // rare: written again
+            const int r = at.slot + __builtin_ctz(near) * at.slots;
+            again<T, V, ACT, RES>(k, r, gp, dy_ld, xp, ld, rp, res_ld, slope, st0, g0, gamma, beta, at.col, s.k, g, d);
+            write(r);
         }
     });
 }
@@ -691,13 +717,8 @@ __global__ __launch_bounds__(NT) void gn_bwd_reduce_kernel(const T* __restrict__
             for (int i = 0; i < V; ++i) { s1[i] += g[i]; s2[i] = fmaf(g[i], d[i], s2[i]); }
         };
         const auto one = [&](long long r) {
-            Chunk<T, V> u, v, w;
             float g[V], d[V];
-            u.load(gp + (size_t)r * dy_ld);
-            v.load(xp + (size_t)r * ld);
-            if constexpr (RES) w.load(rp + (size_t)r * res_ld);
-            if (bwd_vector<T, V, ACT, RES>(k, u, v, w, slope, g, d))
-                settle<T, V, ACT, RES>(gp + (size_t)r * dy_ld, xp + (size_t)r * ld, RES ? rp + (size_t)r * res_ld : nullptr, slope, st0, 0, gamma, beta, at.col, s.k, g);
+            again<T, V, ACT, RES>(k, r, gp, dy_ld, xp, ld, rp, res_ld, slope, st0, 0, gamma, beta, at.col, s.k, g, d);
             add(g, d);
         };
         Chunk<T, V> u[UNR], v[UNR], w[UNR];
@@ -846,13 +867,8 @@ __global__ __launch_bounds__(NT) void gn_bwd_apply_kernel(const T* __restrict__ 
         if constexpr (RES) { if (qp) { t.put(g); t.store(qp + (size_t)row * s.c); } }
     };
     const auto one = [&](long long r) {
-        Chunk<T, V> u, v, w;
         float g[V], d[V];
-        u.load(gp + (size_t)r * dy_ld);
-        v.load(xp + (size_t)r * ld);
-        if constexpr (RES) w.load(rp + (size_t)r * res_ld);
-        if (bwd_vector<T, V, ACT, RES>(k, u, v, w, slope, g, d))
-            settle<T, V, ACT, RES>(gp + (size_t)r * dy_ld, xp + (size_t)r * ld, RES ? rp + (size_t)r * res_ld : nullptr, slope, st0, 0, gamma, beta, at.col, s.k, g);
+        again<T, V, ACT, RES>(k, r, gp, dy_ld, xp, ld, rp, res_ld, slope, st0, 0, gamma, beta, at.col, s.k, g, d);
         write(g, d, r);
     };
     Chunk<T, V> u[2][UNR], v[2][UNR], w[2][UNR];
