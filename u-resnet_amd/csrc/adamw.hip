@@ -6,8 +6,8 @@
 //
 // Bound by HBM: 28 bytes per element with 32-bit moments, 16 + 1/16 with 8-bit ones, 4 more where the norm is taken (the
 // gradients are read twice, the second time partly from the last-level cache).  Measured on the 134 tensors of the
-// segmentation network (32 M elements): norm 23 us (5.6 TB/s), step with 32-bit moments 138 us (6.6 TB/s), with 8-bit ones
-// 88 us (5.9 TB/s); 198 M elements in 8 bits 540 us (5.9 TB/s), where some 75 instructions per element are left of a budget
+// segmentation network (32 M elements): norm 23 us (5.6 TB/s), step with 32-bit moments 136 us (6.7 TB/s), with 8-bit ones
+// 85 us (6.1 TB/s); 198 M elements in 8 bits 540 us (5.9 TB/s), where some 75 instructions per element are left of a budget
 // of about 100 at the HBM rate: the square root is the correctly rounded one (codes depend on it), the quotient of the
 // update is not, and what only NaN, infinity or codes below the normal ones need is behind one branch per wave.
 //
@@ -127,8 +127,13 @@ __device__ __forceinline__ double group_sum(double v) {
 
 __device__ __forceinline__ bool aligned16(const void* a, const void* b) { return (((uintptr_t)a | (uintptr_t)b) & 15) == 0; }
 
-__device__ __forceinline__ fvec4_t ld4(const float* p) { return __builtin_nontemporal_load(reinterpret_cast<const fvec4_t*>(p)); }
-__device__ __forceinline__ void st4(float* p, fvec4_t v) { __builtin_nontemporal_store(v, reinterpret_cast<fvec4_t*>(p)); }
+// Addresses out of a table are global ones, which the compiler cannot know: without these types it takes the flat accesses,
+// whose two wait counters hold up everything else (with that and the loads in one go: 32.5 M elements in 8 bits 87 -> 85 us,
+// in 32 bits 138 -> 136).
+typedef __attribute__((address_space(1))) float gfloat_t;
+typedef __attribute__((address_space(1))) fvec4_t gvec4_t;
+__device__ __forceinline__ fvec4_t ld4(const float* p) { return __builtin_nontemporal_load((const gvec4_t*)p); }
+__device__ __forceinline__ void st4(float* p, fvec4_t v) { __builtin_nontemporal_store(v, (gvec4_t*)p); }
 
 // squares summed in 64 bits (two fp64 instructions per element against the four bytes it is read by)
 __global__ __launch_bounds__(NT) void grad_sqnorm_kernel(const Row* __restrict__ rows, int ntensors, int nchunks, double* __restrict__ parts) {
@@ -137,11 +142,11 @@ __global__ __launch_bounds__(NT) void grad_sqnorm_kernel(const Row* __restrict__
     for (int c = blockIdx.x; c < nchunks; c += gridDim.x) {
         const int t = find(c);
         const long long base = (long long)(c - find.first[t]) * CHUNK, n = rows[t].n;
-        const float* g = rows[t].g;
-        if (aligned16(g, g) && base + CHUNK <= n) {
+        const gfloat_t* g = (const gfloat_t*)rows[t].g;
+        if (aligned16(rows[t].g, rows[t].g) && base + CHUNK <= n) {
             fvec4_t v[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) v[u] = *reinterpret_cast<const fvec4_t*>(g + base + u * (NT * 4) + threadIdx.x * 4);
+            for (int u = 0; u < U; ++u) v[u] = *(const gvec4_t*)(g + base + u * (NT * 4) + threadIdx.x * 4);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
 #pragma unroll
@@ -159,7 +164,13 @@ __global__ __launch_bounds__(NT) void grad_sqnorm_kernel(const Row* __restrict__
 __device__ __forceinline__ float clip_factor(const double* __restrict__ parts, int nparts, float max_norm, float grad_scale,
                                              float* __restrict__ out_norm) {
     double s = 0.0;
-    for (int i = threadIdx.x; i < nparts; i += NT) s += parts[i];
+    for (int at = threadIdx.x; at < nparts; at += 4 * NT) {                  // four loads at a time, in a fixed order
+        double v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = parts[min(at + j * NT, nparts - 1)];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s += at + j * NT < nparts ? v[j] : 0.0;
+    }
     const float norm = (float)(sqrt(group_sum(s)) * (double)fabsf(grad_scale));
     if (out_norm && blockIdx.x == 0 && threadIdx.x == 0) *out_norm = norm;
     float f = max_norm / (norm + 1e-6f);
@@ -185,7 +196,7 @@ __global__ __launch_bounds__(NT) void grad_scale_kernel(const Row* __restrict__ 
 #pragma unroll
             for (int u = 0; u < U; ++u) st4(p + u * (NT * 4), v[u] * f);
         } else {
-            for (long long i = base + threadIdx.x; i < n && i < base + CHUNK; i += NT) g[i] *= f;
+            for (long long i = base + threadIdx.x; i < n && i < base + CHUNK; i += NT) ((gfloat_t*)g)[i] *= f;
         }
     }
 }
@@ -350,6 +361,7 @@ __global__ __launch_bounds__(NT) void adamw_kernel(const Row* __restrict__ rows,
                 g[u] = ld4(row.g + e);
                 st[u].load(m_, v_, ms, vs, at0 + e, b0 + u * (NT * 4 / BLOCK));
             }
+            __builtin_amdgcn_sched_barrier(0);                                // all loads of the chunk before the first wait
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const long long e = e0 + u * (NT * 4);
@@ -371,7 +383,7 @@ __global__ __launch_bounds__(NT) void adamw_kernel(const Row* __restrict__ rows,
                 if (wave0 >= n) break;                                        // (a whole wave: its block does not exist)
                 fvec4_t p = {0.f, 0.f, 0.f, 0.f}, g = p, root;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) if (e + i < n) { p[i] = row.p[e + i]; g[i] = row.g[e + i]; }
+                for (int i = 0; i < 4; ++i) if (e + i < n) { p[i] = ((const gfloat_t*)row.p)[e + i]; g[i] = ((const gfloat_t*)row.g)[e + i]; }
                 State<BITS> st;
                 st.load(m_, v_, ms, vs, at0 + e, row.block + wave0 / BLOCK);
                 st.decode();
@@ -382,7 +394,7 @@ __global__ __launch_bounds__(NT) void adamw_kernel(const Row* __restrict__ rows,
                     p[i] = pi; st.m[i] = mi; st.v[i] = vi; root[i] = ri;
                 }
 #pragma unroll
-                for (int i = 0; i < 4; ++i) if (e + i < n) row.p[e + i] = p[i];
+                for (int i = 0; i < 4; ++i) if (e + i < n) ((gfloat_t*)row.p)[e + i] = p[i];
                 st.store(m_, v_, ms, vs, at0 + e, row.block + wave0 / BLOCK, root, row.step);
             }
         }

@@ -12,8 +12,8 @@
 // the registers of one workgroup is read twice: three passes over a tensor forward and five backward instead of two and three.
 // Keeping an image in the registers of many workgroups that exchange their sums was slower (262 and 613 us for the shape
 // below), and so is counting on the last-level cache for the second read: it serves no faster than HBM here.
-// Measured, 6x64x512x1024 bf16 (403 MB a tensor): statistics 64 us (6.3 TB/s), forward 139 (5.8), sums of the backward pass 125
-// (6.4), gradient 198 (6.1); 64x64x32x32 fp32 in cells: forward 11 us, backward 19 + 4.
+// Measured, 6x64x512x1024 bf16 (403 MB a tensor): statistics 64 us (6.3 TB/s), forward 135 (6.0), sums of the backward pass 122
+// (6.6), gradient 197 (6.1); 64x64x32x32 fp32 in cells: forward 10.5 us, backward 19 + 4.
 //
 // Arithmetic.  The statistics are plain sums of x and x^2 in 64 bits: fp64 vector arithmetic runs at the fp32 rate here, a
 // sum costs four instructions per element against a budget of about thirteen at the HBM rate, and E[x^2] - mean^2 then
@@ -642,8 +642,17 @@ __global__ __launch_bounds__(64) void gn_finalize_kernel(const double* __restric
     const int g = blockIdx.x, n = blockIdx.y, lane = threadIdx.x;
     const double* p = partial + (size_t)n * rows * groups * 2;
     double a = 0.0, q = 0.0;
-#pragma unroll 8
-    for (int r = lane; r < rows; r += 64) { a += p[((size_t)r * groups + g) * 2]; q += p[((size_t)r * groups + g) * 2 + 1]; }
+    for (int r = lane; r < rows; r += 8 * 64) {              // eight loads at a time, the last ones of them possibly idle
+        double v[8][2];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const double* t = p + ((size_t)min(r + 64 * j, rows - 1) * groups + g) * 2;
+            v[j][0] = t[0];
+            v[j][1] = t[1];
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) { const bool in = r + 64 * j < rows; a += in ? v[j][0] : 0.0; q += in ? v[j][1] : 0.0; }
+    }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) { a += __shfl_xor(a, o, 64); q += __shfl_xor(q, o, 64); }
     if (lane == 0) {
@@ -780,8 +789,13 @@ __global__ __launch_bounds__(64 * COEF_WAVES) void gn_bwd_coef_kernel(const floa
         }
         if (c < c_hi) {
             const float2* p = reinterpret_cast<const float2*>(partial) + (size_t)n * s.chunks * s.c + c;
-#pragma unroll 8
-            for (int r = wave; r < s.chunks; r += COEF_WAVES) { const float2 v = p[(size_t)r * s.c]; a += v.x; b += v.y; }
+            for (int r = wave; r < s.chunks; r += 8 * COEF_WAVES) {
+                float2 v[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = p[(size_t)min(r + j * COEF_WAVES, s.chunks - 1) * s.c];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) { const bool in = r + j * COEF_WAVES < s.chunks; a += in ? v[j].x : 0.f; b += in ? v[j].y : 0.f; }
+            }
         }
         red[wave][lane][0] = a;
         red[wave][lane][1] = b;
@@ -910,10 +924,9 @@ Plan make_plan(int dtype, int n, long long hw, int c, int groups, bool vec) {
     p.zs = (cq + p.s.cqb - 1) / p.s.cqb;
     const int slots = NT / p.s.cqb;
     // Up to six workgroups per CU, as many as share both the trips of an image and the CUs evenly: 6x64x512x1024 bf16,
-    // forward + backward, takes 584 us with 1,896 workgroups (7.4 per CU), 551 with 1,536; six rather than eight for
-    // 2x64x512x1024, whose forward pass takes 50 us instead of 55.  A small image goes down to one trip per workgroup
-    // (3x80x77x131: 52 us, 63 with three trips), but four trips of three workgroups per CU are better than two of six
-    // (6x512x64x128 with residual: 149 us and 153).
+    // forward + backward, takes 584 us with 1,896 workgroups (7.4 per CU), 551 with 1,536.  A small image goes down to one
+    // trip per workgroup (3x80x77x131: 52 us, 63 with at least three; 6x512x64x128 with residual: 124 with two trips of six
+    // workgroups per CU, 131 with four of three).
     const long long trips = (hw + (long long)UNR * slots - 1) / ((long long)UNR * slots), per = (long long)n * p.zs;
     double best = 0.0;
     for (int w = 6; w >= 1; --w) {
@@ -922,9 +935,7 @@ Plan make_plan(int dtype, int n, long long hw, int c, int groups, bool vec) {
         if (chunks < 1) chunks = 1;
         const long long each = (trips + chunks - 1) / chunks;
         chunks = (trips + each - 1) / each;
-        const long long per_cu = (per * chunks + 255) / 256;
-        double even = (double)(trips * per) / (double)(each * per_cu * 256);
-        if (per_cu > 3 && each < 4) even *= 0.95;
+        const double even = (double)(trips * per) / (double)(each * ((per * chunks + 255) / 256 * 256));
         if (even > best * 1.02) { best = even; p.s.chunks = (int)chunks; }
     }
     return p;
