@@ -344,10 +344,15 @@ __global__ __launch_bounds__(CT) void gn_fwd_cell_kernel(const T* __restrict__ x
     AffineIn<V> in;
     in.params(gamma, beta, at.col);
     __builtin_amdgcn_sched_barrier(0);
-    Chunk<T, V> v[K];
+    Chunk<T, V> v[K], w[RES ? K : 1];
     const T* xp = x + row0 * ld + at.col;
+    const T* rp = RES ? res + row0 * res_ld + at.col : nullptr;
 #pragma unroll
     for (int j = 0; j < K; ++j) v[j].load(xp + (size_t)min(at.slot + j * at.slots, s.hw - 1) * ld);
+    if constexpr (RES) {
+#pragma unroll
+        for (int j = 0; j < K; ++j) w[j].load(rp + (size_t)min(at.slot + j * at.slots, s.hw - 1) * res_ld);
+    }
     double a[V], q[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) a[i] = q[i] = 0.0;
@@ -419,16 +424,13 @@ __global__ __launch_bounds__(CT) void gn_fwd_cell_kernel(const T* __restrict__ x
     in.groups(mine, g0, at.col, s.k);
     k.set(in);
     T* yp = y + row0 * y_ld + at.col;
-    const T* rp = RES ? res + row0 * res_ld + at.col : nullptr;
     GN_ACT(act, {
 _Pragma("unroll")
         for (int j = 0; j < K; ++j) {
             const int r = at.slot + j * at.slots;
             if (r < s.hw) {
-                Chunk<T, V> w;
-                if constexpr (RES) w.load(rp + (size_t)r * res_ld);
                 v[j].forget();
-                fwd_vector<T, V, ACT, RES>(k, v[j], w, slope).store(yp + (size_t)r * y_ld);
+                fwd_vector<T, V, ACT, RES>(k, v[j], w[RES ? j : 0], slope).store(yp + (size_t)r * y_ld);
             }
         }
     });
@@ -450,7 +452,7 @@ __global__ __launch_bounds__(CT) void gn_bwd_cell_kernel(const T* __restrict__ d
     double* ch_sums = reinterpret_cast<double*>(red + 2 * V);
     float* coef = reinterpret_cast<float*>(ch_sums + 2 * at.sc);
     const double* st0 = stats + ((size_t)at.n * s.groups + g0) * 2;
-    Chunk<T, V> u[K], v[K], w;
+    Chunk<T, V> u[K], v[K], w[RES ? K : 1];
     const T* gp = dy + row0 * dy_ld + at.col;
     const T* xp = x + row0 * ld + at.col;
     const T* rp = RES ? res + row0 * res_ld + at.col : nullptr;
@@ -463,6 +465,7 @@ __global__ __launch_bounds__(CT) void gn_bwd_cell_kernel(const T* __restrict__ d
         const int r = min(at.slot + j * at.slots, s.hw - 1);
         u[j].load(gp + (size_t)r * dy_ld);
         v[j].load(xp + (size_t)r * ld);
+        if constexpr (RES) w[j].load(rp + (size_t)r * res_ld);
     }
     Affine<V> k;
     k.set(in);
@@ -476,8 +479,7 @@ _Pragma("unroll")
             for (int j = 0; j < K; ++j) {
                 const int r = at.slot + j * at.slots;
                 if (r < s.hw) {
-                    if constexpr (RES) w.load(rp + (size_t)r * res_ld);
-                    const bool skip = bwd_vector<T, V, ACT, RES>(k, u[j], v[j], w, slope, g, d);
+                    const bool skip = bwd_vector<T, V, ACT, RES>(k, u[j], v[j], w[RES ? j : 0], slope, g, d);
                     near |= (unsigned)skip << j;
 _Pragma("unroll")
                     for (int i = 0; i < V; ++i) { g[i] = skip ? 0.f : g[i]; s1[i] += g[i]; s2[i] = fmaf(g[i], d[i], s2[i]); }
@@ -545,10 +547,9 @@ _Pragma("unroll")
         for (int j = 0; j < K; ++j) {
             const int r = at.slot + j * at.slots;
             if (r < s.hw) {
-                if constexpr (RES) w.load(rp + (size_t)r * res_ld);
                 u[j].forget();
                 v[j].forget();
-                near |= (unsigned)bwd_vector<T, V, ACT, RES>(k, u[j], v[j], w, slope, g, d) << j;
+                near |= (unsigned)bwd_vector<T, V, ACT, RES>(k, u[j], v[j], w[RES ? j : 0], slope, g, d) << j;
                 write(r);
             }
         }
@@ -566,8 +567,10 @@ __device__ __forceinline__ void sum_images(const double* __restrict__ sums, int 
     __shared__ double red[8][32][2];
     const int ch = threadIdx.x & 31, slot = threadIdx.x >> 5, c = block * 32 + ch;
     double a = 0.0, b = 0.0;
-    if (c < c_all && slot < 8)
+    if (c < c_all && slot < 8) {
+#pragma unroll 4
         for (int n = slot; n < images; n += 8) { const double* p = sums + ((size_t)n * c_all + c) * 2; a += p[0]; b += p[1]; }
+    }
     if (slot < 8) { red[slot][ch][0] = a; red[slot][ch][1] = b; }
     __syncthreads();
     if (slot == 0 && c < c_all) {
