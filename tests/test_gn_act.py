@@ -547,3 +547,36 @@ def test_offsets_beyond_32_bits():
     # another split of the pixels sums in another order (64 bits): one fp32 rounding of the constants, one of the result
     assert torch.allclose(a[-1:].float(), b.float(), rtol=2.0 ** -7, atol=1e-6)
     assert not a[:-1].any()
+
+
+# ------------------------------------------------------------------------------ what a tape node cannot serve
+def refused_transforms(x, gn):
+    """Forward mode (a dual input, weight, residual or output window) and tracing: refused on any device, before the device is
+    looked at."""
+    import torch.autograd.forward_ad as fwd
+    with fwd.dual_level():
+        dual = fwd.make_dual(x, torch.ones_like(x))
+        named = {"weight": fwd.make_dual(gn.weight.detach(), torch.ones_like(gn.weight)), "bias": gn.bias.detach()}
+        for call in (lambda: gn(dual), lambda: ops.gn_act(x, gn, residual=dual), lambda: ops.gn_act(x, gn, out=dual),
+                     lambda: torch.func.functional_call(gn, named, (x,))):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+    with pytest.raises(NotImplementedError, match="torch.jit.trace"):
+        torch.jit.trace(gn, (x,), check_trace=False)
+
+
+def test_forward_mode_and_tracing_are_refused_without_a_gpu():
+    refused_transforms(torch.randn(1, 8, 4, 4).contiguous(memory_format=torch.channels_last), hnn.GroupNorm(4, 8))
+
+
+@pytest.mark.gpu
+def test_forward_mode_tracing_and_function_transforms_are_refused():
+    x, gn = torch.randn(2, 8, 4, 4, device=DEV).contiguous(memory_format=torch.channels_last), hnn.GroupNorm(4, 8).to(DEV)
+    refused_transforms(x, gn)
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda t: gn(t), (x,), (torch.ones_like(x),))
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda t: gn(t).sum())(x)
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda t: gn(t))(x[None])
+    assert torch.isfinite(gn(x)).all()                          # and the operator still works afterwards

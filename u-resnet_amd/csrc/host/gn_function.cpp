@@ -9,6 +9,7 @@
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <climits>
 #include <memory>
@@ -204,6 +205,10 @@ PyObject* gn_act(PyObject*, PyObject* args) {
         PyErr_SetString(type, ("gn_act: " + text).c_str());
         return nullptr;
     };
+    // neither sees what the kernels write through addresses: a tangent would be lost, a recorded call would return fresh memory
+    for (const at::Tensor* p : t)
+        if (p->defined() && p->_fw_grad(0).defined()) return refuse(PyExc_NotImplementedError, "no forward-mode gradient (an input carries a tangent)");
+    if (torch::jit::tracer::isTracing()) return refuse(PyExc_NotImplementedError, "cannot be recorded by torch.jit.trace");
     if (!x.defined() || x.dim() != 4) return refuse(PyExc_ValueError, "expected a 4-D NCHW tensor" + (x.defined() ? ", got shape " + shape_of(x) : ""));
     if (act < UR_ACT_NONE || act > UR_ACT_SILU) return refuse(PyExc_ValueError, "unknown activation code " + std::to_string(act));
     if (!x.is_cuda()) return fail("u-resnet_amd operators run on the GPU only (got a " + x.device().str() + " tensor); there is no CPU fallback");

@@ -1036,7 +1036,8 @@ def gn_act(x, gn, residual=None, act=_lib.ACT_RELU, slope=0.0, out=None):
     converted first); residual: x's shape and dtype.  out: optional channel window (alias_window) to write the result into.
     Training and evaluation are the same computation.  A group of one value normalises to zero.  Gradients flow to x, the
     module's weight and bias and the residual, once: a backward pass with create_graph=True is refused, and so is a captured one
-    while the result of an eager forward pass on the default stream still holds the same leaves.
+    while the result of an eager forward pass on the default stream still holds the same leaves.  Forward-mode gradients and
+    torch.jit.trace are refused.
 
     The tape node lives in the host module (csrc/host/gn_function.cpp): it saves x, the residual (where an activation needs
     the sum) and the fp64 {mean, rstd} of every image and group, and recomputes the pre-activation from them."""
