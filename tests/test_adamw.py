@@ -585,3 +585,40 @@ def test_a_closure_and_weight_images():
         return loss
     assert opt.step(closure).item() == 10.0
     assert ops._weights_epoch == epoch + 1 and torch.allclose(p, torch.full_like(p, 0.9))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_graph_from_before_the_step_is_refused_after_it(bits):
+    """The step rewrites what the graph saved: as with any in-place change, autograd has to see it."""
+    from uresnet_amd import nn as hnn
+    gn = hnn.GroupNorm(4, 8).to(DEV)
+    other = torch.nn.Parameter(torch.ones(5, device=DEV))                  # without a gradient: not written
+    opt = train.AdamW(list(gn.parameters()) + [other], lr=0.5, state_bits=bits)
+    x = torch.randn(2, 8, 4, 4, device=DEV).contiguous(memory_format=torch.channels_last).requires_grad_()
+    y = ops.gn_act(x, gn)
+    (y ** 2).sum().backward(retain_graph=True)
+    versions = [t._version for t in (gn.weight, gn.bias, other)]
+    opt.step()
+    assert [t._version for t in (gn.weight, gn.bias, other)] == [versions[0] + 1, versions[1] + 1, versions[2]]
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        (y ** 2).sum().backward()
+    opt.zero_grad()
+    (ops.gn_act(x, gn) ** 2).sum().backward()                              # a new graph is what such a loop needs
+    opt.step()
+    with torch.inference_mode():
+        p = torch.nn.Parameter(torch.ones(3, device=DEV))                  # has no version
+        p.grad = torch.ones(3, device=DEV)
+        train.AdamW([p], lr=0.1, state_bits=bits).step()
+        assert (p < 1).all()
+
+
+@pytest.mark.gpu
+def test_clipped_gradients_count_as_written():
+    p = torch.nn.Parameter(torch.zeros(7, device=DEV))
+    p.grad = torch.full((7,), 3.0, device=DEV)
+    w = torch.ones(7, device=DEV, requires_grad=True)
+    y = (p.grad * w).sum()                                                 # saves the gradient
+    train.clip_grad_norm_([p], 1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()

@@ -76,6 +76,12 @@ struct Group {
     double lr, beta1, beta2, eps, wd;
 };
 
+// The kernels write through addresses: without a count autograd would hand a graph that saved these tensors their new values.
+void count_writes(const std::vector<at::Tensor>& written) {
+    for (const at::Tensor& t : written)
+        if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 at::Tensor scalar_on(c10::Device device) { return at::empty({}, at::TensorOptions().dtype(at::kFloat).device(device)); }
 
 }  // namespace
@@ -91,7 +97,7 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
     const double max_norm = clip ? PyFloat_AsDouble(limit) : 0.0;
     if (PyErr_Occurred()) return nullptr;
     std::vector<Group> groups((size_t)PyList_GET_SIZE(list));
-    std::vector<at::Tensor> held;                              // contiguous copies of gradients, until the launches are queued
+    std::vector<at::Tensor> held, written;                     // contiguous copies of gradients, until the launches are queued
     c10::Device device(c10::kCPU);
     bool live = false;
     for (size_t k = 0; k < groups.size(); ++k) {
@@ -126,6 +132,7 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
             }
             q.params[i] = (long long)p.data_ptr();
             q.grads[i] = (long long)g.data_ptr();
+            written.push_back(std::move(p));
         }
         q.spans = spans_of(q.grads, q.sizes);
     }
@@ -165,6 +172,7 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
         error = *e.what() ? e.what() : "AdamW failed";
     }
     Py_END_ALLOW_THREADS
+    count_writes(written);
     if (!error.empty()) return fail(error);
     if (!clip) return Py_BuildValue("OO", Py_True, Py_None);
     return Py_BuildValue("ON", Py_True, THPVariable_Wrap(norm));
@@ -177,6 +185,7 @@ PyObject* clip_grads(PyObject*, PyObject* args) {
     int raise;
     if (!PyArg_ParseTuple(args, "O!dp", &PyList_Type, &params, &max_norm, &raise)) return nullptr;
     std::vector<long long> gs, ns;
+    std::vector<at::Tensor> written;
     bool live = false;
     c10::Device device(c10::kCPU);
     for (Py_ssize_t i = 0; i < PyList_GET_SIZE(params); ++i) {
@@ -191,6 +200,7 @@ PyObject* clip_grads(PyObject*, PyObject* args) {
         if (!g.numel()) continue;
         gs.push_back((long long)g.data_ptr());
         ns.push_back((long long)g.numel());
+        written.push_back(g);
     }
     if (!live) Py_RETURN_NONE;
     std::vector<std::pair<long long, long long>> sorted;       // {begin, end} in bytes
@@ -238,5 +248,6 @@ PyObject* clip_grads(PyObject*, PyObject* args) {
     }
     Py_END_ALLOW_THREADS
     if (!error.empty()) return fail(error);
+    count_writes(written);
     return THPVariable_Wrap(norm);
 }
