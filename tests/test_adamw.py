@@ -216,6 +216,82 @@ def test_eight_bit_checkpoints_round_trip_through_a_file(tmp_path):
     assert torch.equal(other.state[ps[5]]["exp_avg"].float(), state[5]["exp_avg"].float()) and int(other.state[ps[5]]["step"]) == 7
 
 
+def made_up_state(ps, bits, step=7.0):
+    state = {}
+    for i, p in enumerate(ps):
+        n, g = p.numel(), torch.Generator().manual_seed(i)
+        m, v = torch.randn(n, generator=g), torch.rand(n, generator=g)
+        if bits == 32:
+            state[i] = {"exp_avg": m.view(p.shape), "exp_avg_sq": v.view(p.shape)}
+        else:
+            (q, s), (r, u) = quantise(m.double()), quantise(v.double(), torch.arange(n), 3)
+            state[i] = {"exp_avg": q.to(torch.float8_e4m3fn).view(p.shape), "exp_avg_scale": s.float(),
+                        "exp_avg_sq_root": r.to(torch.float8_e4m3fn).view(p.shape), "exp_avg_sq_root_scale": u.float()}
+        state[i]["step"] = torch.tensor(step)
+    return state
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_loading_keeps_every_group_key_and_runs_the_hooks(bits):
+    """A scheduler continues from a loaded state (its initial_lr travels in the groups); registered hooks run, those before the
+    load may change what is loaded, those after it see the loaded moments."""
+    ps = [torch.nn.Parameter(v) for v in tensors(40, SIZES[:5])]
+    opt = train.AdamW(ps, lr=0.5, state_bits=bits)
+    torch.optim.lr_scheduler.StepLR(opt, 3)
+    opt.param_groups[0]["note"] = "kept"
+    sd = {**opt.state_dict(), "state": made_up_state(ps, bits)}
+    other = train.AdamW(ps, state_bits=bits)
+    seen = []
+
+    def before(o, d):
+        seen.append("before")
+        d["param_groups"][0]["eps"] = 1e-6
+        return {**d}
+
+    def after(o):
+        seen.append(o.state[ps[3]]["exp_avg"].float().clone())
+    other.register_load_state_dict_pre_hook(before)
+    other.register_load_state_dict_post_hook(after)
+    other.load_state_dict(sd)
+    group = other.param_groups[0]
+    assert group["note"] == "kept" and group["lr"] == 0.5 and group["eps"] == 1e-6 and group["state_bits"] == bits
+    sched = torch.optim.lr_scheduler.StepLR(other, 3, last_epoch=2)
+    assert sched.get_last_lr()[0] == pytest.approx(0.05)
+    assert seen[0] == "before" and torch.equal(seen[1], sd["state"][3]["exp_avg"].float()) and len(seen) == 2
+    for i, p in enumerate(ps):
+        for k, v in other.state[p].items():
+            assert torch.equal(v.float(), sd["state"][i][k].float()), k
+    other.load_state_dict(sd)                                  # nothing of the first load is left behind
+    assert len(seen) == 4
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_state_that_does_not_fit_leaves_the_optimiser_as_it_was(bits):
+    ps = [torch.nn.Parameter(v) for v in tensors(41, SIZES[:5])]
+    opt = train.AdamW(ps, lr=0.25, state_bits=bits)
+    opt.load_state_dict({**opt.state_dict(), "state": made_up_state(ps, bits)})
+    want = {k: v.float().clone() for k, v in opt.state_buffers().items()}
+    for key in ("exp_avg", "exp_avg_sq") if bits == 32 else ("exp_avg", "exp_avg_scale", "exp_avg_sq_root", "exp_avg_sq_root_scale"):
+        bad = {**opt.state_dict(), "state": made_up_state(ps, bits, 9.0)}
+        bad["param_groups"][0]["lr"] = 1.0
+        bad["state"][4][key] = torch.cat([bad["state"][4][key].flatten().float()] * 2)
+        with pytest.raises(ValueError, match=key):
+            opt.load_state_dict(bad)
+        state, group = opt.state, opt.param_groups[0]
+        assert group["lr"] == 0.25 and all(int(state[p]["step"]) == 7 for p in ps)
+        assert all(torch.equal(v.float(), want[k]) for k, v in opt.state_buffers().items())
+        assert state[ps[4]]["exp_avg"].untyped_storage().data_ptr() == opt.state_buffers()["exp_avg"].untyped_storage().data_ptr()
+
+    def fails(o):
+        raise OSError("a hook that fails")
+    handle = opt.register_load_state_dict_post_hook(fails)
+    with pytest.raises(OSError):
+        opt.load_state_dict({**opt.state_dict(), "state": made_up_state(ps, bits, 9.0)})
+    handle.remove()
+    assert int(opt.state[ps[0]]["step"]) == 7 and opt.step() is None
+    assert all(torch.equal(v.float(), want[k]) for k, v in opt.state_buffers().items())
+
+
 def test_dither_is_uniform_over_places_and_steps():
     """Mean and correlation of 2^16 draws against their standard errors (4 of them)."""
     n = 1 << 16

@@ -374,6 +374,13 @@ class _MomentPool:
         return out
 
 
+class _Loaded:
+    """A parameter's loaded state on its way through torch.optim.Optimizer.load_state_dict, which would cast 8-bit codes."""
+
+    def __init__(self, entry):
+        self.entry = entry
+
+
 class AdamW(torch.optim.Optimizer):
     """torch.optim.AdamW semantics (decoupled weight decay, no amsgrad) over all tensors of a group in one launch.
 
@@ -413,6 +420,9 @@ class AdamW(torch.optim.Optimizer):
 
     def __setstate__(self, state):             # copied or unpickled: the pools are built again from `state`
         super().__setstate__(state)
+        for p, entry in self.state.items():
+            if isinstance(entry, _Loaded):
+                self.state[p] = entry.entry
         self._pools = {}
         for k, v in (('max_grad_norm', None), ('grad_scale', 1.0), ('grad_norm', None)):
             self.__dict__.setdefault(k, v)
@@ -468,34 +478,46 @@ class AdamW(torch.optim.Optimizer):
                 g.setdefault(k, v)
         return sd
 
-    def load_state_dict(self, state_dict):
+    def _checked(self, state_dict):
+        """What load_state_dict takes over, looked through as a whole: this group's state_bits, the other keys as saved."""
         groups, saved = self.param_groups, state_dict['param_groups']
         if [len(g['params']) for g in groups] != [len(g['params']) for g in saved]:
             raise ValueError("AdamW: the loaded state has other parameter groups")
-        state = {}
+        state, taken = {}, []
         for group, old in zip(groups, saved):
             if old.get('amsgrad') or old.get('maximize') or old.get('decoupled_weight_decay') is False:
                 raise NotImplementedError("AdamW: amsgrad, maximize and coupled weight decay states cannot be loaded")
             bits = old.get('state_bits', group['state_bits'])
-            names = {'exp_avg', 'exp_avg_sq'} if bits == 32 else {'exp_avg', 'exp_avg_scale', 'exp_avg_sq_root', 'exp_avg_sq_root_scale'}
+            names = ('exp_avg', 'exp_avg_sq') if bits == 32 else ('exp_avg', 'exp_avg_scale', 'exp_avg_sq_root', 'exp_avg_sq_root_scale')
             for p, k in zip(group['params'], old['params']):
                 entry = state_dict['state'].get(k)
                 if not entry:
                     continue
-                if not names | {'step'} <= set(entry) or bits != group['state_bits']:
+                if not {*names, 'step'} <= set(entry) or bits != group['state_bits']:
                     raise ValueError("AdamW: the loaded moments are not %d-bit ones" % group['state_bits'])
-                if entry['exp_avg'].numel() != p.numel():
-                    raise ValueError("AdamW: loaded moments of shape %s for a parameter of shape %s"
-                                     % (tuple(entry['exp_avg'].shape), tuple(p.shape)))
-                state[p] = {**{n: entry[n] for n in names}, 'step': torch.as_tensor(entry['step']).round().to(torch.int32)}
-        for group, old in zip(groups, saved):
-            group.update({k: old[k] for k in ('lr', 'betas', 'eps', 'weight_decay') if k in old})
-        self.state.clear()
-        self.state.update(state)
-        self._pools = {}
-        for gi, group in enumerate(groups):
-            if group['params']:
-                self._pool(gi, group)
+                for n in names:
+                    if entry[n].numel() != (-(-p.numel() // _MomentPool.BLOCK) if n.endswith('_scale') else p.numel()):
+                        raise ValueError("AdamW: a loaded %s of shape %s for a parameter of shape %s" % (n, tuple(entry[n].shape), tuple(p.shape)))
+                state[k] = _Loaded({**{n: entry[n] for n in names}, 'step': torch.as_tensor(entry['step']).reshape(()).round().to(torch.int32)})
+            taken.append({**{k: v for k, v in group.items() if k != 'params'}, **old, 'state_bits': group['state_bits']})
+            taken[-1]['lr'] = float(taken[-1]['lr'])
+        return {**state_dict, 'state': state, 'param_groups': taken}
+
+    def load_state_dict(self, state_dict):
+        """Takes over the moments and every key of the groups but state_bits (a scheduler's `initial_lr` among them).  A state
+        that does not fit is refused and leaves the optimiser as it was."""
+        before = self.state, self.param_groups, self._pools
+        last = self.register_load_state_dict_pre_hook(AdamW._checked)        # sees what the other hooks made of it
+        try:
+            super().load_state_dict(state_dict)
+            for gi, group in enumerate(self.param_groups):
+                if group['params']:
+                    self._pool(gi, group)
+        except BaseException:
+            self.state, self.param_groups, self._pools = before
+            raise
+        finally:
+            last.remove()
 
 
 class GraphedStep:
