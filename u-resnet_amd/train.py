@@ -498,7 +498,7 @@ class AdamW(torch.optim.Optimizer):
                 for n in names:
                     if entry[n].numel() != (-(-p.numel() // _MomentPool.BLOCK) if n.endswith('_scale') else p.numel()):
                         raise ValueError("AdamW: a loaded %s of shape %s for a parameter of shape %s" % (n, tuple(entry[n].shape), tuple(p.shape)))
-                state[k] = _Loaded({**{n: entry[n] for n in names}, 'step': torch.as_tensor(entry['step']).reshape(()).round().to(torch.int32)})
+                state[k] = _Loaded({**{n: entry[n] for n in names}, 'step': torch.as_tensor(entry['step']).round().to(torch.int32)})
             taken.append({**{k: v for k, v in group.items() if k != 'params'}, **old, 'state_bits': group['state_bits']})
             taken[-1]['lr'] = float(taken[-1]['lr'])
         return {**state_dict, 'state': state, 'param_groups': taken}
