@@ -292,6 +292,35 @@ def test_a_state_that_does_not_fit_leaves_the_optimiser_as_it_was(bits):
     assert all(torch.equal(v.float(), want[k]) for k, v in opt.state_buffers().items())
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_what_a_caller_puts_into_the_state_counts(bits):
+    """Entries emptied or replaced between steps, tensors replaced inside an entry, entries of the caller's own."""
+    ps = [torch.nn.Parameter(v) for v in tensors(42, SIZES[:5])]
+    opt = train.AdamW(ps, state_bits=bits)
+    opt.load_state_dict({**opt.state_dict(), "state": made_up_state(ps, bits)})
+    want = {i: {k: v.float().clone() for k, v in opt.state[p].items()} for i, p in enumerate(ps)}
+    opt.state[ps[0]] = {}
+    opt.state[ps[2]]["exp_avg"] = torch.full(ps[2].shape, 2.0)
+    opt.state[ps[3]] = {**opt.state[ps[3]], "step": torch.tensor(3.0), "mine": "kept"}
+    opt.state[ps[4]]["exp_avg"].zero_()                        # in place, as ever
+    sd = opt.state_dict()["state"]
+    assert sd[0] == {} and [float(sd[i]["step"]) for i in (1, 2, 3, 4)] == [7, 7, 3, 7]
+    opt.step()                                                 # no gradients: only what the optimiser holds is looked at
+    flat, at = opt.state_buffers()["exp_avg"].float(), 0
+    for i, p in enumerate(ps):
+        n = p.numel()
+        expected = {0: torch.zeros(n), 2: torch.full((n,), 2.0), 4: torch.zeros(n)}.get(i, want[i]["exp_avg"].flatten())
+        assert torch.equal(flat[at:at + n], expected), i
+        at += -(-n // 256) * 256
+    assert not opt.state[ps[0]] and opt.state[ps[3]]["mine"] == "kept" and int(opt.state[ps[3]]["step"]) == 3
+    pool = opt._pools[0]
+    opt.step()
+    assert opt._pools[0] is pool and 0 in pool.waiting         # nothing changed since: nothing is built again
+    del opt.state[ps[1]]
+    opt.step()
+    assert not opt.state_buffers()["exp_avg"].float()[256:256 + 3].any() and sorted(opt._pools[0].waiting) == [0, 1]
+
+
 def test_dither_is_uniform_over_places_and_steps():
     """Mean and correlation of 2^16 draws against their standard errors (4 of them)."""
     n = 1 << 16

@@ -28,5 +28,6 @@ extern EntryPoints entry;
 PyObject* fail(const std::string& text);                   // raises the package's error type
 void check(int status, const char* what);                  // throws with the entry point's message
 PyObject* adamw_step(PyObject* self, PyObject* args);
+PyObject* holds(PyObject* self, PyObject* args);
 PyObject* clip_grads(PyObject* self, PyObject* args);
 PyObject* gn_act(PyObject* self, PyObject* args);

@@ -47,6 +47,7 @@ PyObject* guarded(PyObject* self, PyObject* args) {
 }
 
 PyMethodDef methods[] = {{"adamw_step", guarded<adamw_step>, METH_VARARGS, "one AdamW step over parameter groups"},
+                         {"holds", guarded<holds>, METH_VARARGS, "whether a dict of dicts still holds the same objects"},
                          {"clip_grads", guarded<clip_grads>, METH_VARARGS, "gradients scaled to a norm"},
                          {"gn_act", guarded<gn_act>, METH_VARARGS, "group norm with an activation, with its gradient"},
                          {"set_error_type", set_error_type, METH_O, "exception type for refused tensors"},

@@ -178,6 +178,22 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
     return Py_BuildValue("ON", Py_True, THPVariable_Wrap(norm));
 }
 
+// holds(state, entries, contents): whether the values of the dict `state` are the dicts `entries` and their values, one after the
+// other, the objects of the list `contents`
+PyObject* holds(PyObject*, PyObject* args) {
+    PyObject *state, *entries, *contents;
+    if (!PyArg_ParseTuple(args, "O!O!O!", &PyDict_Type, &state, &PyList_Type, &entries, &PyList_Type, &contents)) return nullptr;
+    if (PyDict_Size(state) != PyList_GET_SIZE(entries)) Py_RETURN_FALSE;
+    Py_ssize_t at = 0, i = 0, k = 0;
+    for (PyObject *key, *entry; PyDict_Next(state, &at, &key, &entry); ++i) {
+        if (entry != PyList_GET_ITEM(entries, i) || !PyDict_Check(entry)) Py_RETURN_FALSE;
+        Py_ssize_t in = 0;
+        for (PyObject *name, *value; PyDict_Next(entry, &in, &name, &value); ++k)
+            if (k >= PyList_GET_SIZE(contents) || value != PyList_GET_ITEM(contents, k)) Py_RETURN_FALSE;
+    }
+    return PyBool_FromLong(k == PyList_GET_SIZE(contents));
+}
+
 // clip_grads(parameters, max_norm, whether to raise on a norm that is not finite) -> norm, None without gradients
 PyObject* clip_grads(PyObject*, PyObject* args) {
     PyObject* params;

@@ -9,6 +9,7 @@
   checkpoints       the dict written at train_UResNetAblitionStudy.py:244-252 (save_checkpoint / load_checkpoint)
 """
 import array
+import itertools
 import operator
 
 import torch
@@ -355,7 +356,7 @@ class _MomentPool:
                 new = self.views(i)
                 for k, v in new.items():
                     v.copy_(torch.as_tensor(old[k]).reshape(v.shape))
-                state[p] = new
+                state[p] = {**old, **new}
 
     def holds(self, group):
         ps = group['params']
@@ -398,6 +399,7 @@ class AdamW(torch.optim.Optimizer):
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, max_grad_norm=None):
         self._pools = {}                       # group index -> _MomentPool
+        self._held = [], []                    # the entries of `state` and what is in them, as the last step left them
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits))
         if max_grad_norm is not None and not float(max_grad_norm) > 0:
             raise ValueError("AdamW: max_grad_norm must be positive (got %r)" % (max_grad_norm,))
@@ -424,6 +426,7 @@ class AdamW(torch.optim.Optimizer):
             if isinstance(entry, _Loaded):
                 self.state[p] = entry.entry
         self._pools = {}
+        self._held = [], []
         for k, v in (('max_grad_norm', None), ('grad_scale', 1.0), ('grad_norm', None)):
             self.__dict__.setdefault(k, v)
 
@@ -437,11 +440,22 @@ class AdamW(torch.optim.Optimizer):
             if dev.type == 'cuda' and torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("AdamW: run at least one eager step before capturing")
             pool = self._pools[gi] = _MomentPool(group, self.state)
+            self._held = self._contents()
         return pool
+
+    def _contents(self):
+        entries = list(self.state.values())
+        return entries, list(itertools.chain.from_iterable(map(dict.values, entries)))
+
+    def _look_at_state(self):
+        """What was cleared or replaced in `state` since the last step counts: the pools are then built again from it."""
+        if not _lib.host().holds(self.state, *self._held):
+            self._pools = {}
 
     def state_buffers(self, group=0):
         """The moments of a parameter group as flat tensors, parameters in order, each at a multiple of 256 elements (32 bits:
         exp_avg, exp_avg_sq; 8 bits: exp_avg, exp_avg_sq_root and a scale per 256 elements).  The optimiser's own buffers."""
+        self._look_at_state()
         return dict(self._pool(group, self.param_groups[group]).buffers)
 
     def step(self, closure=None):
@@ -449,21 +463,23 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        if sum(len(pool.params) - len(pool.waiting) for pool in self._pools.values()) != len(self.state):
-            self._pools = {}                                   # `state` was cleared or replaced: built again from it
+        self._look_at_state()
         pools = [(group, self._pool(gi, group)) for gi, group in enumerate(self.param_groups) if group['params']]
         launched, self.grad_norm = _lib.host().adamw_step(
             [(pool.params, pool.sizes, *pool.places, float(group['lr']), *group['betas'], group['eps'], group['weight_decay'])
              for group, pool in pools], self.max_grad_norm, self.grad_scale)
-        for _, pool in pools:
-            for i in [i for i in pool.waiting if pool.params[i].grad is not None]:
-                pool.waiting.remove(i)
-                self.state[pool.params[i]] = pool.views(i)
+        new = [(pool, i) for _, pool in pools for i in pool.waiting if pool.params[i].grad is not None]
+        for pool, i in new:
+            pool.waiting.remove(i)
+            self.state[pool.params[i]] = pool.views(i)
+        if new:
+            self._held = self._contents()
         if launched:
             ops.bump_weights_epoch()
         return loss
 
     def state_dict(self):
+        self._look_at_state()
         sd = super().state_dict()
         host = {gi: pool.steps.cpu() for gi, pool in self._pools.items()}          # one device read per group
         order = [(gi, i) for gi, group in enumerate(self.param_groups) for i in range(len(group['params']))]
@@ -471,7 +487,7 @@ class AdamW(torch.optim.Optimizer):
         def step_of(k, v):
             gi, i = order[k]
             return float(host[gi][i]) if gi in host and self._pools[gi].holds(self.param_groups[gi]) else float(v['step'])
-        sd['state'] = {k: {**v, 'step': torch.tensor(step_of(k, v))} for k, v in sd['state'].items()}
+        sd['state'] = {k: {**v, 'step': torch.tensor(step_of(k, v))} if v else v for k, v in sd['state'].items()}
         for g in sd['param_groups']:                 # torch.optim.AdamW's remaining group keys, at their defaults
             for k, v in (('amsgrad', False), ('maximize', False), ('foreach', None), ('capturable', False),
                          ('differentiable', False), ('fused', None), ('decoupled_weight_decay', True)):
@@ -506,7 +522,7 @@ class AdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict):
         """Takes over the moments and every key of the groups but state_bits (a scheduler's `initial_lr` among them).  A state
         that does not fit is refused and leaves the optimiser as it was."""
-        before = self.state, self.param_groups, self._pools
+        before = self.state, self.param_groups, self._pools, self._held
         last = self.register_load_state_dict_pre_hook(AdamW._checked)        # sees what the other hooks made of it
         try:
             super().load_state_dict(state_dict)
@@ -514,7 +530,7 @@ class AdamW(torch.optim.Optimizer):
                 if group['params']:
                     self._pool(gi, group)
         except BaseException:
-            self.state, self.param_groups, self._pools = before
+            self.state, self.param_groups, self._pools, self._held = before
             raise
         finally:
             last.remove()
