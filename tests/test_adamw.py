@@ -727,3 +727,39 @@ def test_clipped_gradients_count_as_written():
     train.clip_grad_norm_([p], 1.0)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.backward()
+
+
+@pytest.mark.gpu
+def test_a_root_above_zero_keeps_a_code_above_zero():
+    """b2 = 0: the root is |g|.  Twelve decades inside every block: what is far below the lowest code (2^-9 of the scale) gets
+    that code, only exact zeros get 0."""
+    gen = torch.Generator().manual_seed(50)
+    g = 10 ** (-12 * torch.rand(16, 256, generator=gen)) * torch.randn(16, 256, generator=gen).sign()
+    g[:, 7], g[:, 0] = 0.0, 1.0
+    p = torch.nn.Parameter(torch.zeros(g.numel(), device=DEV))
+    opt = train.AdamW([p], lr=0.0, betas=(0.0, 0.0), state_bits=8)
+    p.grad = g.flatten().to(DEV)
+    for _ in range(3):
+        opt.step()
+        codes = opt.state_buffers()["exp_avg_sq_root"].float().cpu().view(16, 256)
+        assert (codes[g == 0] == 0).all() and (codes[g != 0] >= 2.0 ** -9).all()
+        below = (g != 0) & (g.abs() * 448 < 2.0 ** -9)
+        assert below.sum() > 1000 and (codes[below] == 2.0 ** -9).all()
+
+
+@pytest.mark.gpu
+def test_eight_bit_steps_with_six_decades_inside_a_block_stay_bounded():
+    """(1 - b1) / sqrt(1 - b2) = 3.2 lr bounds a step in 32 bits; a code more or less among the lowest ones is a factor of two
+    for m and for the root: four times that."""
+    gen = torch.Generator(device=DEV).manual_seed(51)
+    n = 256 * 64
+    size = 10 ** (-6 * torch.rand(n, generator=gen, device=DEV))
+    p = torch.nn.Parameter(torch.zeros(n, device=DEV))
+    opt = train.AdamW([p], lr=1.0, weight_decay=0.0, state_bits=8)
+    largest = torch.zeros((), device=DEV)
+    for _ in range(300):
+        p.grad = size * torch.randn(n, generator=gen, device=DEV)
+        before = p.detach().clone()
+        opt.step()
+        largest = torch.maximum(largest, (p.detach() - before).abs().max())
+    assert largest.item() < 4 * 3.2

@@ -20,7 +20,8 @@
 // 256 elements that maps the block's largest value to the largest code, 448.  m is rounded to the nearest code: it moves by
 // a tenth of itself per step, more than half a code step (3 to 6 %).  r moves by at most 0.05 % per step when the gradients
 // get smaller, so nearest rounding would pin it for good; it is rounded up with the probability of its fraction instead,
-// so that its expectation follows the recurrence.  The 20 random bits per element come from a hash of the element's place
+// so that its expectation follows the recurrence.  A root above zero never gets the code 0: the next update would divide m by
+// eps (hundreds of lr where the gradients of a block span six decades).  The 20 random bits per element come from a hash of the element's place
 // in the state and the step count: the same step gives the same bits, and nothing is kept between calls.  The step itself
 // uses m and v before they are rounded.
 #include "ur_common.h"
@@ -321,7 +322,10 @@ template <> struct State<8> {
         if (__any(low)) {
             q = 0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) q |= (r[i] < LOWEST_NORMAL ? encode_up_low(r[i], d[i]) : encode_up(r[i], d[i])) << (8 * i);
+            for (int i = 0; i < 4; ++i) {
+                const unsigned code = r[i] < LOWEST_NORMAL ? encode_up_low(r[i], d[i]) : encode_up(r[i], d[i]);
+                q |= (root[i] > 0.f ? max(code, 1u) : code) << (8 * i);
+            }
         }
         unsigned qm_new = encode4(y);
         if (!all_finite) {                                                    // an infinite or NaN value becomes the NaN code and stays alone
