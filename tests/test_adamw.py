@@ -763,3 +763,26 @@ def test_eight_bit_steps_with_six_decades_inside_a_block_stay_bounded():
         opt.step()
         largest = torch.maximum(largest, (p.detach() - before).abs().max())
     assert largest.item() < 4 * 3.2
+
+
+@pytest.mark.gpu
+def test_weights_without_a_gradient_come_to_rest_in_eight_bits():
+    """Half of every block stops getting gradients.  Its first moment falls by at least one code per step while the scale does
+    not fall (a tenth is more than half a step between normal codes, and lower ones are rounded down): the 127 codes are
+    passed in at most 127 steps, then the weights stay where they are."""
+    gen = torch.Generator(device=DEV).manual_seed(52)
+    n, lr = 256 * 16, 1e-2
+    live = (torch.arange(n, device=DEV) % 2).float()
+    g = torch.randn(n, generator=gen, device=DEV)
+    g[1::256] = 4.0                                            # the largest of its block, and constant: the scale only grows
+    p = torch.nn.Parameter(torch.zeros(n, device=DEV))
+    opt = train.AdamW([p], lr=lr, betas=(0.9, 0.95), weight_decay=0.0, state_bits=8)
+    for t in range(20 + 127):
+        p.grad = (g if t < 20 else g * live).clamp(-4, 4)
+        opt.step()
+    dead = live == 0
+    assert not opt.state_buffers()["exp_avg"].float()[dead].any() and opt.state_buffers()["exp_avg"].float()[~dead].any()
+    rest = p.detach().clone()
+    for _ in range(800):                                       # the roots fall to their lowest code
+        opt.step()
+    assert torch.equal(p.detach()[dead], rest[dead]) and (opt.state_buffers()["exp_avg_sq_root"].float()[dead] == 2.0 ** -9).all()

@@ -18,7 +18,9 @@
 //
 // 8-bit moments.  m and r = sqrt(v) are stored as e4m3 codes (3 mantissa bits, exponents over 2^17) with one fp32 scale per
 // 256 elements that maps the block's largest value to the largest code, 448.  m is rounded to the nearest code: it moves by
-// a tenth of itself per step, more than half a code step (3 to 6 %).  r moves by at most 0.05 % per step when the gradients
+// a tenth of itself per step, more than half a code step (3 to 6 %).  Below the normal codes, whose steps are larger than that,
+// a falling m is rounded towards zero: to the nearest, the m of a weight without a gradient would stop at four steps and the
+// weight drift for good.  r moves by at most 0.05 % per step when the gradients
 // get smaller, so nearest rounding would pin it for good; it is rounded up with the probability of its fraction instead,
 // so that its expectation follows the recurrence.  A root above zero never gets the code 0: the next update would divide m by
 // eps (hundreds of lr where the gradients of a block span six decades).  The 20 random bits per element come from a hash of the element's place
@@ -315,14 +317,16 @@ template <> struct State<8> {
         for (int i = 0; i < 4; ++i) {
             y[i] = m[i] * im;                                                 // at most a rounding above 448, which is its nearest code
             r[i] = fminf(root[i] * ir, TOP);
-            low |= r[i] < LOWEST_NORMAL;
+            low |= fminf(r[i], fabsf(y[i])) < LOWEST_NORMAL;
             d[i] = dither(h0 + i * HASH_PLACE);
             q |= encode_up(r[i], d[i]) << (8 * i);
         }
         if (__any(low)) {
             q = 0;
+            const fvec4_t before = decode4(qm) * sm;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
+                if (fabsf(y[i]) < LOWEST_NORMAL && fabsf(m[i]) < fabsf(before[i])) y[i] = truncf(y[i] * 512.f) * (1.f / 512.f);
                 const unsigned code = r[i] < LOWEST_NORMAL ? encode_up_low(r[i], d[i]) : encode_up(r[i], d[i]);
                 q |= (root[i] > 0.f ? max(code, 1u) : code) << (8 * i);
             }
