@@ -497,7 +497,7 @@ int ur_sgd_multi(const void* const* ptrs, const long long* sizes, int ntensors, 
  *   3. ur_adamw_multi makes the step.  nparts > 0: gradients are scaled by min(1, max_norm / (norm + 1e-6)), norm over all
  *      `nparts` sums, and out_norm (may be NULL) gets the norm before clipping.  grad_scale multiplies every gradient first.
  *      Moments lie in buffers of blocks of 256 elements: state_bits 32: fp32; 8: e4m3 codes of m and of sqrt(v) and an
- *      fp32 scale per block.
+ *      fp32 scale per block (beta1 at most 17/18).
  *   or ur_grad_clip scales the gradients in place.
  * Parameters and gradients are dense fp32; tensors of a list must not overlap. */
 int ur_param_table_max_rows(void); /* tensors per table; longer lists take several */

@@ -292,6 +292,29 @@ def test_a_state_that_does_not_fit_leaves_the_optimiser_as_it_was(bits):
     assert all(torch.equal(v.float(), want[k]) for k, v in opt.state_buffers().items())
 
 
+def test_eight_bit_moments_need_a_first_beta_that_lets_them_fall():
+    """A falling m leaves every code that nearest rounding could keep it on only if 9/8 * b1 < 17/16."""
+    values = (1 + torch.arange(8) / 8).double()
+    for b1, moves in ((17 / 18 - 1e-6, True), (0.9, True), (0.95, False)):
+        rounded = (values * b1 * 16).float().to(torch.float8_e4m3fn).double() / 16
+        assert bool((rounded < values).all()) is moves
+    p = torch.nn.Parameter(torch.zeros(4))
+    with pytest.raises(ValueError, match="17/18"):
+        train.AdamW([p], betas=(0.95, 0.999), state_bits=8)
+    train.AdamW([p], betas=(0.95, 0.999))
+    opt = train.AdamW([p], betas=(17 / 18, 0.999), state_bits=8)
+    sd = opt.state_dict()
+    sd["param_groups"][0]["betas"] = (0.99, 0.999)
+    with pytest.raises(ValueError, match="17/18"):
+        opt.load_state_dict(sd)
+    assert opt.param_groups[0]["betas"][0] == 17 / 18
+    opt.param_groups[0]["betas"] = (0.95, 0.999)               # as a scheduler that cycles the momentum sets it
+    with pytest.raises(_lib.UResNetHipError, match="17/18"):
+        opt.step()
+    with pytest.raises(_lib.UResNetHipError, match="17/18"):
+        _lib.call("ur_adamw_multi", 16, 1, 1, 8, 16, 16, 16, 16, 1e-3, 0.95, 0.999, 1e-8, 0.0, None, 0, 1.0, 1.0, None, None)
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 def test_what_a_caller_puts_into_the_state_counts(bits):
     """Entries emptied or replaced between steps, tensors replaced inside an entry, entries of the caller's own."""
@@ -786,3 +809,32 @@ def test_weights_without_a_gradient_come_to_rest_in_eight_bits():
     for _ in range(800):                                       # the roots fall to their lowest code
         opt.step()
     assert torch.equal(p.detach()[dead], rest[dead]) and (opt.state_buffers()["exp_avg_sq_root"].float()[dead] == 2.0 ** -9).all()
+
+
+@pytest.mark.gpu
+def test_eight_bit_moments_over_some_hundred_steps():
+    """Against the recurrences in 64 bits.  The root's rounding adds a variance of f (1 - f) s^2 per step, f the fraction of the
+    code step s by which it moves: to first order |change| s.  The change is (1 - b2) / 2 |g^2 / v - 1|, 0.97 (1 - b2) / 2 on
+    average for Gaussian gradients, s is 0.090 on average (1/8 of the power of two below), and what is there decays by b2 per
+    step: 0.97 * 0.090 / 4 = 0.0218 remains, 14.8 % rms.  m's nearest rounding adds s^2 / 12 per step, kept for 1 / (1 - b1^2):
+    5.5 % rms, together 15.8 % for the update.  A third more is allowed for the higher orders."""
+    gen = torch.Generator(device=DEV).manual_seed(53)
+    n, steps = 256 * 256, 400
+    p = torch.nn.Parameter(torch.zeros(n, device=DEV))
+    opt = train.AdamW([p], lr=1.0, weight_decay=0.0, state_bits=8)
+    m, v = torch.zeros(2, n, dtype=torch.float64, device=DEV)
+    for t in range(1, steps + 1):
+        g = 1e-3 * torch.randn(n, generator=gen, device=DEV)
+        m, v = 0.9 * m + 0.1 * g.double(), 0.999 * v + 0.001 * g.double() ** 2
+        before = p.detach().clone()
+        p.grad = g
+        opt.step()
+    want = m / (1 - 0.9 ** steps) / ((v / (1 - 0.999 ** steps)).sqrt() + 1e-8)
+    off = (before - p.detach()).double() - want
+    assert (off.square().mean() / want.square().mean()).sqrt().item() < 0.158 * 4 / 3
+    st = opt.state_buffers()
+    root = dequantise(st["exp_avg_sq_root"].float().cpu(), st["exp_avg_sq_root_scale"].cpu()) / v.sqrt().cpu() - 1
+    assert root.square().mean().sqrt().item() < 0.148 * 4 / 3
+    # The rounding keeps r on average and so adds its variance to v = r^2: 0.97 * 0.090 * (1 - b2) / 2 of v per step, which decays
+    # by 1 - b2 of itself: 0.0437 = 2 * 0.148^2 above.  The same third more on a root, its square here.
+    assert 0 < ((root + 1) ** 2).mean().item() - 1 < 2 * (0.148 * 4 / 3) ** 2

@@ -18,14 +18,15 @@
 //
 // 8-bit moments.  m and r = sqrt(v) are stored as e4m3 codes (3 mantissa bits, exponents over 2^17) with one fp32 scale per
 // 256 elements that maps the block's largest value to the largest code, 448.  m is rounded to the nearest code: it moves by
-// a tenth of itself per step, more than half a code step (3 to 6 %).  Below the normal codes, whose steps are larger than that,
-// a falling m is rounded towards zero: to the nearest, the m of a weight without a gradient would stop at four steps and the
-// weight drift for good.  r moves by at most 0.05 % per step when the gradients
-// get smaller, so nearest rounding would pin it for good; it is rounded up with the probability of its fraction instead,
-// so that its expectation follows the recurrence.  A root above zero never gets the code 0: the next update would divide m by
-// eps (hundreds of lr where the gradients of a block span six decades).  The 20 random bits per element come from a hash of the element's place
-// in the state and the step count: the same step gives the same bits, and nothing is kept between calls.  The step itself
-// uses m and v before they are rounded.
+// a tenth of itself per step, more than half a code step (3 to 6 %).  Below the normal codes, whose steps are larger than
+// that, a falling m is rounded towards zero: to the nearest, the m of a weight without a gradient would stop at four steps
+// and the weight drift for good.  That takes b1 <= 17/18: nearest rounding moves a falling m off every code only if b1 *
+// 9/8 is below 17/16, so larger b1 are refused.  r moves by at most 0.05 % per step when the gradients get smaller, so
+// nearest rounding would pin it for good; it is rounded up with the probability of its fraction instead, so that a rounding
+// keeps its expectation (v = r^2 gains the variance: 4 to 5 % at b2 = 0.999).  A root above zero never gets the code 0: the
+// next update would divide m by eps (hundreds of lr where the gradients of a block span six decades).  The 20 random bits
+// per element come from a hash of the element's place in the state and the step count: the same step gives the same bits,
+// and nothing is kept between calls.  The step itself uses m and v before they are rounded.
 #include "ur_common.h"
 
 namespace {
@@ -39,6 +40,7 @@ constexpr int BATCH = 136;                   // rows per table launch: kernel ar
 constexpr int MAX_PARTS = 1024;             // partial sums of the norm
 constexpr long long MAX_CHUNKS = 1LL << 30;  // a chunk's number plus the grid's size stays an int
 constexpr float TOP = 448.f;
+constexpr double BETA1_MOST_8 = 17.0 / 18.0; // largest b1 for 8-bit moments
 
 typedef __attribute__((ext_vector_type(4))) float fvec4_t;
 typedef __attribute__((ext_vector_type(2))) float fvec2_t;
@@ -470,6 +472,7 @@ int ur_adamw_multi(const void* table, int ntensors, long long nchunks, int state
     UR_REQUIRE(table && ntensors > 0 && ntensors <= MAX_ROWS && nchunks > 0 && nchunks <= MAX_CHUNKS && exp_avg && exp_avg_sq, "adamw_multi: bad arguments");
     UR_REQUIRE(state_bits == 32 || state_bits == 8, "adamw_multi: state_bits is 32 or 8 (got %d)", state_bits);
     UR_REQUIRE(state_bits == 32 || (exp_avg_scale && exp_avg_sq_scale), "adamw_multi: 8-bit states without scales");
+    UR_REQUIRE(state_bits == 32 || beta1 <= BETA1_MOST_8, "adamw_multi: 8-bit moments need beta1 <= 17/18 (got %g)", beta1);
     UR_REQUIRE((((uintptr_t)exp_avg | (uintptr_t)exp_avg_sq) & 15) == 0, "adamw_multi: the state buffers are not 16-byte aligned");
     UR_REQUIRE(nparts == 0 || (nparts > 0 && parts), "adamw_multi: bad partial sums");
     const Hyper h = {(float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)eps, (float)(1.0 - lr * weight_decay)};

@@ -106,6 +106,7 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
         if (!PyArg_ParseTuple(PyList_GET_ITEM(list, (Py_ssize_t)k), "O!SKKiKKKKddddd", &PyList_Type, &params, &sizes, &q.blocks, &q.steps, &q.bits,
                               &q.m, &q.v, &q.ms, &q.vs, &q.lr, &q.beta1, &q.beta2, &q.eps, &q.wd))
             return nullptr;
+        if (q.bits == 8 && q.beta1 > 17.0 / 18.0) return fail("AdamW: 8-bit moments need betas[0] <= 17/18 (got " + std::to_string(q.beta1) + ")");
         const Py_ssize_t n = PyList_GET_SIZE(params);
         if (PyBytes_GET_SIZE(sizes) != (Py_ssize_t)(n * sizeof(long long))) return fail("AdamW: lists of different lengths");
         const long long* want = reinterpret_cast<const long long*>(PyBytes_AS_STRING(sizes));
