@@ -838,3 +838,20 @@ def test_eight_bit_moments_over_some_hundred_steps():
     # The rounding keeps r on average and so adds its variance to v = r^2: 0.97 * 0.090 * (1 - b2) / 2 of v per step, which decays
     # by 1 - b2 of itself: 0.0437 = 2 * 0.148^2 above.  The same third more on a root, its square here.
     assert 0 < ((root + 1) ** 2).mean().item() - 1 < 2 * (0.148 * 4 / 3) ** 2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_nan_norm_leaves_the_state_between_the_tensors_zero(bits):
+    sizes = [(300,), (5,), (2049,)]
+    ps = params_on_gpu([torch.ones(s) for s in sizes], tensors(54, sizes))
+    ps[1].grad[2] = float("nan")
+    opt = train.AdamW(ps, state_bits=bits, max_grad_norm=1.0)
+    for _ in range(2):
+        opt.step()
+    assert opt.grad_norm.isnan() and all(p.isnan().all() for p in ps)
+    for k, buf in opt.state_buffers().items():
+        if not k.endswith("scale"):
+            buf = buf.float().cpu()
+            for lo, hi in ((300, 512), (512 + 5, 768), (768 + 2049, buf.numel())):
+                assert (buf[lo:hi] == 0).all(), (k, lo)

@@ -398,9 +398,9 @@ __global__ __launch_bounds__(NT) void adamw_kernel(const Row* __restrict__ rows,
                 st.load(m_, v_, ms, vs, at0 + e, row.block + wave0 / BLOCK);
                 st.decode();
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int i = 0; i < 4; ++i) {                                 // (behind the end zero also under a NaN factor)
                     float pi = p[i], mi = st.m[i], vi = st.v[i], ri;
-                    adamw_one(pi, g[i] * factor, mi, vi, ri, h, row.step_size, row.bc2_rsqrt);
+                    adamw_one(pi, e + i < n ? g[i] * factor : 0.f, mi, vi, ri, h, row.step_size, row.bc2_rsqrt);
                     p[i] = pi; st.m[i] = mi; st.v[i] = vi; root[i] = ri;
                 }
 #pragma unroll

@@ -400,7 +400,8 @@ class AdamW(torch.optim.Optimizer):
     Step counts live on the device and nothing is staged on the host: after one eager step a step can be captured in a graph
     and replayed (learning rate and the other constants are then those of the capture).  state_dict() has torch.optim.AdamW's
     layout with 32-bit moments and loads into it; 8-bit moments load into 8-bit groups only.  Checkpoints hold `exp_avg` and
-    `exp_avg_sq_root` as float8_e4m3fn beside their `_scale`s.  An infinite or NaN gradient makes its own element NaN only."""
+    `exp_avg_sq_root` as float8_e4m3fn beside their `_scale`s.  An infinite or NaN gradient makes its own element NaN only
+    (with max_grad_norm all of them, as its norm is the factor's)."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, max_grad_norm=None):
         self._pools = {}                       # group index -> _MomentPool
