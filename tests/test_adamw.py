@@ -855,3 +855,17 @@ def test_a_nan_norm_leaves_the_state_between_the_tensors_zero(bits):
             buf = buf.float().cpu()
             for lo, hi in ((300, 512), (512 + 5, 768), (768 + 2049, buf.numel())):
                 assert (buf[lo:hi] == 0).all(), (k, lo)
+
+
+@pytest.mark.gpu
+def test_a_norm_beyond_fp32_is_not_finite():
+    """Finite gradients whose norm is no fp32 number: infinity, as in torch (and gradients scaled to zero), or an error."""
+    p = torch.nn.Parameter(torch.zeros(3, device=DEV))
+    p.grad = torch.full((3,), 3e38, device=DEV)
+    with pytest.raises(RuntimeError, match="not finite"):
+        train.clip_grad_norm_([p], 1.0, error_if_nonfinite=True)
+    assert (p.grad == 3e38).all()
+    assert train.clip_grad_norm_([p], 1.0).isinf() and (p.grad == 0).all()
+    p.grad = torch.full((3,), 1.9e38, device=DEV)              # 3.3e38: still one
+    norm = train.clip_grad_norm_([p], 1.0, error_if_nonfinite=True)
+    assert abs(norm.item() - 1.9e38 * 3 ** 0.5) <= 4 * E24 * norm.item()

@@ -254,7 +254,7 @@ PyObject* clip_grads(PyObject*, PyObject* args) {
                 const int64_t at = (reinterpret_cast<char*>(mem.parts) - static_cast<char*>(mem.buf.data_ptr())) / 8;
                 const at::NoGradGuard no_grad;
                 const double total = mem.buf.narrow(0, 8 * at, 8 * (int64_t)nparts).view(at::kDouble).sum().item<double>();
-                if (!std::isfinite(total)) error = "clip_grad_norm_: the total norm of the gradients is not finite";
+                if (!std::isfinite((float)std::sqrt(total))) error = "clip_grad_norm_: the total norm of the gradients is not finite";
             }
             if (error.empty())
                 for (const Span* s : spans)
