@@ -580,3 +580,44 @@ def test_forward_mode_tracing_and_function_transforms_are_refused():
     with pytest.raises(RuntimeError):
         torch.func.vmap(lambda t: gn(t))(x[None])
     assert torch.isfinite(gn(x)).all()                          # and the operator still works afterwards
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["relu", "leakyrelu", "relu6"])
+@pytest.mark.parametrize("residual", [False, True])
+def test_zero_weights_beside_a_rectified_residual(residual, act):
+    """pre = r exactly, 0 for half of the elements: the slope of the activation at 0, in both forms of the kernels."""
+    for shape, dtype in (((2, 32, 9, 11, 8), torch.float32), ((3, 72, 90, 70, 8), torch.bfloat16)):
+        x, dy, r, gn = make(shape, dtype, 18, residual=residual)
+        with torch.no_grad():
+            gn.weight.zero_()
+            gn.bias.zero_()
+        if residual:
+            r = r.relu()
+        check(x, dy, r, gn, act, run(x, dy, r, gn, act))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape, dtype", [((2, 64, 512, 512, 32), torch.bfloat16), ((64, 64, 64, 64, 8), torch.float32)])
+def test_zero_weights_take_the_time_of_any_others(shape, dtype):
+    """The same passes over the same bytes; half as much again is allowed for the clock."""
+    x, dy, r, gn = make(shape, dtype, 19, residual=True)
+    cl = lambda t: t.to(DEV).contiguous(memory_format=torch.channels_last)      # noqa: E731
+    x, dy, r = cl(x).requires_grad_(), cl(dy), cl(r.relu()).requires_grad_()
+    outs = []
+    for zero in (False, True):
+        norm = hnn.GroupNorm(shape[4], shape[1]).to(DEV)
+        with torch.no_grad():
+            norm.weight.copy_(0 * gn.weight if zero else gn.weight)
+            norm.bias.copy_(0 * gn.bias if zero else gn.bias)
+        outs.append((ops.gn_act(x, norm, residual=r), norm))
+    best = [float("inf")] * 2
+    for _ in range(25):
+        for i, (y, norm) in enumerate(outs):
+            start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            start.record()
+            torch.autograd.grad(y, [x, r, norm.weight, norm.bias], dy, retain_graph=True)
+            end.record()
+            end.synchronize()
+            best[i] = min(best[i], start.elapsed_time(end))
+    assert best[1] < 1.5 * best[0], best
