@@ -621,3 +621,122 @@ def test_zero_weights_take_the_time_of_any_others(shape, dtype):
             end.synchronize()
             best[i] = min(best[i], start.elapsed_time(end))
     assert best[1] < 1.5 * best[0], best
+
+
+# ------------------------------------------------------------------------------ every pixel counts once
+def trips_per_workgroup(shape, dtype, vec):
+    """What the launch plan of the streaming passes gives a workgroup: trips of 4 vectors per thread, 256 threads."""
+    n, c, h, w, _ = shape
+    v = (8 if dtype == torch.bfloat16 else 4) if vec else 1
+    cq = -(-c // v)
+    cqb = min(cq, 256)
+    slots, zs = 256 // cqb, -(-cq // cqb)
+    trips, per = -(-h * w // (4 * slots)), n * zs
+    best, plan = 0.0, None
+    for k in range(6, 0, -1):
+        chunks = max(1, min(256 * k // per, trips))
+        each = -(-trips // chunks)
+        chunks = -(-trips // each)
+        even = trips * per / (each * (-(-per * chunks // 256) * 256))
+        if even > best * 1.02:
+            best, plan = even, each
+    return plan, h * w % (4 * slots)
+
+
+def whole_numbers(shape, dtype, seed, act, residual, kink):
+    """Inputs whose sums are whole numbers below 2^24 in every fp32 accumulator: x of mean exactly 0 in every channel, in random
+    pixel order, dy and the residual small.  A pixel left out or counted twice shows.  kink: biases that put one value of x
+    within 1e-8 of it."""
+    n, c, h, w, groups = shape
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    hw, rand = h * w, lambda lo, hi, *s: torch.randint(lo, hi, s, generator=g, device=DEV, dtype=torch.int8).to(dtype)     # noqa: E731
+    half = rand(-6, 7, n, hw // 2, c)
+    order = torch.randperm(hw, generator=g, device=DEV)
+    x = torch.cat([half, -half, half.new_zeros(n, hw % 2, c)], 1)[:, order].view(n, h, w, c).permute(0, 3, 1, 2)
+    dy = rand(-3, 4, n, h, w, c).permute(0, 3, 1, 2)
+    r = rand(-4, 5, n, h, w, c).permute(0, 3, 1, 2) if residual else None
+    gn = hnn.GroupNorm(groups, c).to(DEV)
+    with torch.no_grad():
+        gn.weight.copy_(1 + 0.3 * torch.randn(c, generator=g, device=DEV))
+        gn.bias.copy_(0.3 * torch.randn(c, generator=g, device=DEV))
+        if kink:
+            var = x[0].double().square().reshape(groups, -1).mean(1)
+            gn.bias.copy_(-2 * (var + gn.eps).rsqrt().repeat_interleave(c // groups) * gn.weight)
+    return x, dy, r, gn
+
+
+def check_whole_numbers(shape, dtype, act, residual, kink=False, seed=20):
+    x, dy, r, gn = whole_numbers(shape, dtype, seed, act, residual, kink)
+    n, c, h, w, groups = shape
+    xd, rd = x.detach().requires_grad_(), None if r is None else r.detach().requires_grad_()
+    y = ops.gn_act(xd, gn, residual=rd, act=ACTS[act], slope=0.25)
+    got = torch.autograd.grad(y, [xd, gn.weight, gn.bias] + ([] if r is None else [rd]), dy)
+
+    # in 64 bits on the GPU: [n][pixels][groups][channels of a group]
+    def split(t):
+        return t.detach().permute(0, 2, 3, 1).reshape(n, h * w, groups, -1).double()
+    ga, be = (t.detach().double().view(groups, -1) for t in (gn.weight, gn.bias))
+    xs, m = split(x), h * w * (c // groups)
+    assert xs.sum((1, 3)).abs().max() == 0
+    rstd = (xs.square().sum((1, 3), keepdim=True) / m + gn.eps).rsqrt()
+    pre = xs * rstd * ga + be
+    size = (xs * rstd * ga).abs() + be.abs()
+    if r is not None:
+        pre, size = pre + split(r), size + split(r).abs()
+    slope = {"none": torch.ones_like(pre), "relu": (pre > 0).double(), "leakyrelu": torch.where(pre > 0, 1.0, 0.25).double()}[act]
+    gs = split(dy) * slope
+    s1, s2 = gs.sum(1), (gs * xs).sum(1)                               # exact
+    p1, p2 = (s1 * ga).sum(2) / m, (s2 * ga).sum(2) / m
+    p1, p2 = p1.view(n, 1, groups, 1), p2.view(n, 1, groups, 1) * rstd
+    dx = rstd * (ga * gs - p1 - xs * rstd * p2)
+    size_dx = rstd * ((ga * gs).abs() + p1.abs() + (xs * rstd * p2).abs())
+    half = HALF[dtype]
+
+    def close(a, want, tol, what):
+        off = (split(a) if a.dim() == 4 else a.detach().double().view(groups, -1)) - want
+        assert (off.abs() <= tol).all(), "%s: off by %.3g" % (what, off.abs().max().item())
+    # one rounding each of A, B (mean exactly 0: B is the bias), the product with the sum and the residual's sum: 4 of 2^-24
+    close(y, pre * torch.where(pre > 0, 1.0, {"none": 1.0, "relu": 0.0, "leakyrelu": 0.25}[act]), half * pre.abs() + 6 * E24 * size, "y")
+    # A, the two constants of a group (one rounding each after exact sums), two sums
+    close(got[0], dx, half * dx.abs() + 6 * E24 * size_dx, "dx")
+    # whole numbers times rstd (64 bits), rounded once
+    want = (s2 * rstd[:, 0]).sum(0)
+    close(got[1], want, E24 * want.abs() * 1.01 + 1e-12 * (s2.abs() * rstd[:, 0]).sum(0), "dgamma")
+    close(got[2], s1.sum(0), E24 * s1.sum(0).abs(), "dbeta")
+    if r is not None:
+        close(got[3], gs, torch.zeros(()), "dres") if act != "none" else close(got[3], split(dy), torch.zeros(()), "dres")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", SHAPES + [(2, 1024, 3, 3, 1), (1, 4088, 2, 2, 8), (3, 72, 90, 70, 8), (64, 64, 32, 32, 8), (5, 60, 41, 47, 20)])
+def test_every_pixel_counts_once(shape, dtype):
+    for act, residual in (("none", False), ("relu", True)):
+        check_whole_numbers(shape, dtype, act, residual)
+
+
+LONG = [  # shape, dtype, vectors, trips per workgroup
+    ((6, 64, 181, 361, 32), torch.bfloat16, True, 2),
+    ((1, 64, 523, 1031, 32), torch.bfloat16, True, 17),
+    ((2, 512, 113, 181, 32), torch.bfloat16, True, 2),
+    ((1, 256, 409, 479, 8), torch.bfloat16, True, 4),
+    ((3, 40, 331, 499, 5), torch.bfloat16, True, 2),
+    ((1, 64, 421, 691, 8), torch.float32, True, 3),
+    ((2, 96, 173, 397, 32), torch.float32, True, 7),
+    ((1, 60, 277, 307, 20), torch.bfloat16, False, 7),
+    ((2, 3, 557, 1021, 3), torch.float32, False, 7),
+    ((4, 300, 53, 61, 300), torch.bfloat16, False, 13),
+]
+
+
+def test_long_shapes_take_several_trips_and_leave_a_remainder():
+    for shape, dtype, vec, trips in LONG:
+        got, rest = trips_per_workgroup(shape, dtype, vec)
+        assert got == trips and rest, (shape, got, rest)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act, residual, kink", [("none", False, False), ("relu", False, True), ("relu", True, False), ("leakyrelu", True, True)])
+@pytest.mark.parametrize("shape, dtype, vec, trips", LONG)
+def test_every_pixel_counts_once_over_several_trips(shape, dtype, vec, trips, act, residual, kink):
+    check_whole_numbers(shape, dtype, act, residual, kink)
