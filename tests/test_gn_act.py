@@ -740,3 +740,23 @@ def test_long_shapes_take_several_trips_and_leave_a_remainder():
 @pytest.mark.parametrize("shape, dtype, vec, trips", LONG)
 def test_every_pixel_counts_once_over_several_trips(shape, dtype, vec, trips, act, residual, kink):
     check_whole_numbers(shape, dtype, act, residual, kink)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act, low, high", [("relu", 0.0, None), ("relu6", 0.0, 6.0), ("hswish", -3.0, None)])
+@pytest.mark.parametrize("shape, dtype", [((2, 32, 9, 11, 8), torch.float32), ((3, 72, 90, 70, 8), torch.bfloat16), ((2, 5, 6, 7, 5), torch.float32)])
+def test_infinite_gradients_where_the_slope_is_zero_count_for_nothing(shape, dtype, act, low, high):
+    """As the gradient of a square root behind a ReLU is: infinite exactly where nothing passes."""
+    x, dy, r, gn = make(shape, dtype, 21, residual=True)
+    r = (4 * r.float()).to(dtype)
+    n, c, h, w, groups = shape
+    xs = x.double().reshape(n, groups, -1)
+    xhat = ((xs - xs.mean(2, keepdim=True)) * (xs.var(2, unbiased=False, keepdim=True) + gn.eps).rsqrt()).view(n, c, h, w)
+    pre = xhat * gn.weight.detach().double().view(c, 1, 1) + gn.bias.detach().double().view(c, 1, 1) + r.double()
+    closed = (pre < low - 1e-3) | (pre > high + 1e-3) if high is not None else pre < low - 1e-3
+    bad = dy.clone()
+    bad[closed] = float("inf")
+    bad[closed & (r > 1)] = float("nan")
+    want = run(x, torch.where(closed, torch.zeros_like(dy), dy), r, gn, act)
+    got = run(x, bad, r, gn, act)
+    assert closed.any() and all(torch.equal(got[k], want[k]) for k in want)

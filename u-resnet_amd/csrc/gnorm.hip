@@ -90,18 +90,19 @@ template <int ACT> __device__ __forceinline__ float gn_act(float p, float slope)
     if constexpr (ACT == UR_ACT_SILU) return p * __builtin_amdgcn_rcpf(1.f + __expf(-p));
     return p;
 }
-template <int ACT, typename F> __device__ __forceinline__ float gn_act_grad(F p, float slope) {
-    if constexpr (ACT == UR_ACT_RELU) return p <= (F)0 ? 0.f : 1.f;
-    if constexpr (ACT == UR_ACT_RELU6) return (p > (F)0 && p < (F)6) ? 1.f : 0.f;
-    if constexpr (ACT == UR_ACT_LEAKYRELU) return p > (F)0 ? 1.f : slope;
-    if constexpr (ACT == UR_ACT_HSWISH) return p <= (F)-3 ? 0.f : (p < (F)3 ? (2.f * (float)p + 3.f) * (1.f / 6.f) : 1.f);
+// dy * act'(p).  Where the slope is 0 dy is left out, not multiplied: infinite or NaN there, it counts for nothing
+template <int ACT, typename F> __device__ __forceinline__ float gn_act_grad(float dy, F p, float slope) {
+    if constexpr (ACT == UR_ACT_RELU) return p <= (F)0 ? 0.f : dy;
+    if constexpr (ACT == UR_ACT_RELU6) return (p > (F)0 && p < (F)6) ? dy : 0.f;
+    if constexpr (ACT == UR_ACT_LEAKYRELU) return p > (F)0 ? dy : dy * slope;
+    if constexpr (ACT == UR_ACT_HSWISH) return p <= (F)-3 ? 0.f : (p < (F)3 ? dy * ((2.f * (float)p + 3.f) * (1.f / 6.f)) : dy);
     const float q = (float)p;
-    if constexpr (ACT == UR_ACT_GELU) { float e; const float c = gn_phi(q, e); return fmaf(q * 0.3989422804014327f, e, c); }
+    if constexpr (ACT == UR_ACT_GELU) { float e; const float c = gn_phi(q, e); return dy * fmaf(q * 0.3989422804014327f, e, c); }
     if constexpr (ACT == UR_ACT_SILU) {
         const float s = __builtin_amdgcn_rcpf(1.f + __expf(-q));
-        return s * (1.f + q * (1.f - s));
+        return dy * (s * (1.f + q * (1.f - s)));
     }
-    return 1.f;
+    return dy;
 }
 // whether p is so close to a kink of the activation's derivative that its fp32 value may be on the wrong side.  Near a kink
 // at t: d * A = t - B - r up to the result, and d, A, B, the products and the sums each carry at most 2^-24 relative to
@@ -268,7 +269,7 @@ __device__ __forceinline__ bool bwd_vector(const Affine<V>& k, const Chunk<T, V>
         float p = fmaf(d[i], k.a[i], k.b[i]), size = fabsf(k.b[i]);
         if constexpr (RES) { p += w.get(i); size += fabsf(w.get(i)); }
         near |= gn_near_kink<ACT>(p, size);
-        g[i] = u.get(i) * gn_act_grad<ACT, float>(p, slope);
+        g[i] = gn_act_grad<ACT, float>(u.get(i), p, slope);
     }
     return near;
 }
@@ -280,7 +281,7 @@ __device__ __forceinline__ void settle(const T* dy, const T* x, const T* res, fl
         const double* st = stats + ((col + i) / per - g0) * 2;
         double e = ((double)ur_to_float(x[i]) - st[0]) * st[1] * (gamma ? (double)gamma[col + i] : 1.0) + (beta ? (double)beta[col + i] : 0.0);
         if constexpr (RES) e += (double)ur_to_float(res[i]);
-        const float exact = ur_to_float(dy[i]) * gn_act_grad<ACT, double>(e, slope);
+        const float exact = gn_act_grad<ACT, double>(ur_to_float(dy[i]), e, slope);
 #pragma unroll
         for (int j = 0; j < V; ++j) g[j] = j == i ? exact : g[j];
     }
