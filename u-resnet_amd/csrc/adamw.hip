@@ -6,10 +6,12 @@
 //
 // Bound by HBM: 28 bytes per element with 32-bit moments, 16 + 1/16 with 8-bit ones, 4 more where the norm is taken (the
 // gradients are read twice, the second time partly from the last-level cache).  Measured on the 134 tensors of the
-// segmentation network (32 M elements): norm 23 us (5.6 TB/s), step with 32-bit moments 136 us (6.7 TB/s), with 8-bit ones
-// 85 us (6.1 TB/s); 198 M elements in 8 bits 540 us (5.9 TB/s), where some 75 instructions per element are left of a budget
-// of about 100 at the HBM rate: the square root is the correctly rounded one (codes depend on it), the quotient of the
-// update is not, and what only NaN, infinity or codes below the normal ones need is behind one branch per wave.
+// segmentation network (32 M elements): norm 23 us (5.6 TB/s), step with 32-bit moments 137 us (6.6 TB/s), with 8-bit ones
+// 87 us (6.0 TB/s); a whole step of 198 M elements in 8 bits 540 us (5.9 TB/s; its kernel 534 to 590 under the profiler), where
+// some 75 instructions per element are left of a budget of about 100 at the HBM rate: the square root is the correctly rounded
+// one (codes depend on it), the quotient of the update is not, and what only NaN, infinity or codes below the normal ones need
+// is behind one branch per wave.  The scales are reciprocals and products where the definition divides: a code next to a border
+// between two can differ from the definition's.
 //
 // Work list.  The host hands over the tensors by value (as kernel arguments); param_table_kernel writes them as a table in
 // the caller's workspace, advances the step counts and derives the bias corrections.  No staging buffer and no copy from
@@ -476,8 +478,9 @@ int ur_adamw_multi(const void* table, int ntensors, long long nchunks, int state
     UR_REQUIRE((((uintptr_t)exp_avg | (uintptr_t)exp_avg_sq) & 15) == 0, "adamw_multi: the state buffers are not 16-byte aligned");
     UR_REQUIRE(nparts == 0 || (nparts > 0 && parts), "adamw_multi: bad partial sums");
     const Hyper h = {(float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)eps, (float)(1.0 - lr * weight_decay)};
-    // A workgroup per chunk streams best (32 M elements in 32 bits 135 us, 147 at 2048 workgroups; 198 M in 8 bits 583 and 656);
-    // with clipping every workgroup adds up the partial sums first, which 8192 of them repay (8 bits 88 us, one per chunk 95).
+    // A workgroup per chunk streams best (32 M elements in 32 bits 135 us, 147 at 2048 workgroups; 198 M in 8 bits 583 and 656
+    // before the accesses became global ones); with clipping every workgroup adds up the partial sums first, which 8192 of them
+    // repay (8 bits 87 us, one per chunk 94).
     const long long most = nparts ? 8192 : 65536;
     const int grid = (int)(nchunks < most ? nchunks : most);
     if (state_bits == 32)

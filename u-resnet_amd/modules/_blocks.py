@@ -41,7 +41,8 @@ def act_layer(act, inplace=False, neg_slope=0.2, n_prelu=1):
 
 
 def _cba(seq, x, i, out=None, pool=False, out_stats=False):
-    """Run seq[i] (conv), seq[i+1] (BN), seq[i+2] (activation) fused when the activation is ReLU.  `out`: optional
+    """Run seq[i] (conv), seq[i+1] (BN), seq[i+2] (activation) fused when the activation is ReLU (behind a GroupNorm: any
+    of _GN_ACT_CODES).  `out`: optional
     channel window for the result (honoured on the fused path only; callers compare data_ptr()).  pool: the caller
     max-pools the result next, out_stats: the caller normalises it with another BatchNorm next (ops.bn_act)."""
     conv, bn, act = seq[i], seq[i + 1], seq[i + 2]
