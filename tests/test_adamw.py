@@ -869,3 +869,25 @@ def test_a_norm_beyond_fp32_is_not_finite():
     p.grad = torch.full((3,), 1.9e38, device=DEV)              # 3.3e38: still one
     norm = train.clip_grad_norm_([p], 1.0, error_if_nonfinite=True)
     assert abs(norm.item() - 1.9e38 * 3 ** 0.5) <= 4 * E24 * norm.item()
+
+
+@pytest.mark.gpu
+def test_parameters_that_come_to_share_memory_are_refused():
+    """Tied by hand after the first step: both would be written by one launch."""
+    a, b, c = (torch.nn.Parameter(torch.ones(40, device=DEV)) for _ in range(3))
+    opt = train.AdamW([a, b, c], lr=0.1)
+    for p in (a, b, c):
+        p.grad = torch.ones(40, device=DEV)
+    opt.step()
+    whole = torch.ones(60, device=DEV)
+    for first, second in ((whole[:40], whole[:40]), (whole[20:], whole[:40])):
+        a.data, c.data = first, second
+        with pytest.raises(_lib.UResNetHipError, match="share memory"):
+            opt.step()
+        assert (whole == 1).all() and int(opt.state[a]["step"]) == 1
+    c.grad = None                                              # not written: no race
+    opt.step()
+    assert (whole[20:] < 1).all() and (whole[:20] == 1).all()
+    a.data, c.data, c.grad = whole[:30], whole[30:], torch.ones(30, device=DEV)
+    with pytest.raises(_lib.UResNetHipError, match="size"):
+        opt.step()

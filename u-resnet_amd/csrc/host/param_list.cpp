@@ -68,6 +68,16 @@ struct Memory {
     }
 };
 
+// Bytes [begin, end) of each tensor of four-byte elements at `addresses`, in order; empty and absent ones left out.
+std::vector<std::pair<long long, long long>> ranges(const std::vector<long long>& addresses, const std::vector<long long>& sizes) {
+    std::vector<std::pair<long long, long long>> out;
+    out.reserve(addresses.size());
+    for (size_t i = 0; i < addresses.size(); ++i)
+        if (addresses[i] && sizes[i]) out.emplace_back(addresses[i], addresses[i] + 4 * sizes[i]);
+    std::sort(out.begin(), out.end());
+    return out;
+}
+
 struct Group {
     std::vector<long long> params, grads, sizes;
     std::vector<Span> spans;
@@ -135,6 +145,9 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
             q.grads[i] = (long long)g.data_ptr();
             written.push_back(std::move(p));
         }
+        const auto places = ranges(q.params, q.sizes);         // one launch writes them all: shared memory would be a race
+        for (size_t i = 1; i < places.size(); ++i)
+            if (places[i].first < places[i - 1].second) return fail("AdamW: two parameters of a group share memory");
         q.spans = spans_of(q.grads, q.sizes);
     }
     std::vector<Span*> spans;
@@ -220,9 +233,7 @@ PyObject* clip_grads(PyObject*, PyObject* args) {
         written.push_back(g);
     }
     if (!live) Py_RETURN_NONE;
-    std::vector<std::pair<long long, long long>> sorted;       // {begin, end} in bytes
-    for (size_t i = 0; i < gs.size(); ++i) sorted.emplace_back(gs[i], gs[i] + 4 * ns[i]);
-    std::sort(sorted.begin(), sorted.end());
+    const auto sorted = ranges(gs, ns);
     for (size_t i = 1; i < sorted.size(); ++i)
         if (sorted[i].first < sorted[i - 1].second) {
             PyErr_SetString(PyExc_ValueError, sorted[i] == sorted[i - 1] ? "clip_grad_norm_: a gradient is listed twice" : "clip_grad_norm_: two gradients overlap");

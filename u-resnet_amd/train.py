@@ -383,7 +383,8 @@ class _Loaded:
 
 
 class AdamW(torch.optim.Optimizer):
-    """torch.optim.AdamW semantics (decoupled weight decay, no amsgrad) over all tensors of a group in one launch.
+    """torch.optim.AdamW semantics (decoupled weight decay, no amsgrad) over all tensors of a group in one launch.  A group's moments
+    are allocated together, also those of parameters that never get a gradient.
 
     state_bits (also per group): 32, or 8 -- both moments as e4m3 codes with one fp32 scale per 256 elements, 2 bytes per
     element instead of 8.  The second moment is held by its root and rounded in proportion (a rounding keeps the root's
