@@ -760,3 +760,37 @@ def test_infinite_gradients_where_the_slope_is_zero_count_for_nothing(shape, dty
     want = run(x, torch.where(closed, torch.zeros_like(dy), dy), r, gn, act)
     got = run(x, bad, r, gn, act)
     assert closed.any() and all(torch.equal(got[k], want[k]) for k in want)
+
+
+@pytest.mark.gpu
+def test_activation_checkpointing_and_errors_of_saved_tensor_hooks():
+    """Checkpointing without reentry ends its recomputation by an exception out of the hook that packs the last saved tensor."""
+    from torch.utils.checkpoint import checkpoint
+    x, dy, r, gn = make((2, 16, 9, 5, 4), torch.bfloat16, 22, residual=True)
+    gn, cl = gn.to(DEV), lambda t: t.to(DEV).contiguous(memory_format=torch.channels_last)      # noqa: E731
+    second = hnn.GroupNorm(2, 16).to(DEV)
+    xd, rd, dyd = cl(x).requires_grad_(), cl(r).requires_grad_(), cl(dy)
+
+    def last(a, b):
+        return ops.gn_act(a, gn, residual=b)
+
+    def inside(a, b):
+        return ops.gn_act(ops.gn_act(a, gn, residual=b, act=ACTS["silu"]), second).float() * 2
+    for f, norms in ((last, [gn]), (inside, [gn, second])):
+        wrt = [xd, rd] + [p for m in norms for p in m.parameters()]
+        want = torch.autograd.grad(f(xd, rd), wrt, dyd.to(f(xd, rd).dtype))
+        for early_stop in (True, False):
+            with torch.utils.checkpoint.set_checkpoint_early_stop(early_stop):
+                y = checkpoint(f, xd, rd, use_reentrant=False)
+                assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, wrt, dyd.to(y.dtype)), want))
+
+    def fails(t):
+        raise KeyError("the hook's own")
+    with torch.autograd.graph.saved_tensors_hooks(fails, lambda t: t), pytest.raises(KeyError, match="the hook's own"):
+        ops.gn_act(xd, gn)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, fails):
+        y = ops.gn_act(xd, gn)
+    with pytest.raises(KeyError, match="the hook's own"):
+        y.sum().backward()
+    with pytest.raises(_lib.UResNetHipError, match="limits"):      # errors of the entry points as before
+        ops.gn_act(torch.zeros(1, 16392, 1, 1, device=DEV), hnn.GroupNorm(1, 16392).to(DEV))

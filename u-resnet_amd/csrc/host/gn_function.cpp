@@ -6,10 +6,12 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
+#include <torch/csrc/utils/pybind.h>
 
 #include <climits>
 #include <memory>
@@ -231,15 +233,12 @@ PyObject* gn_act(PyObject*, PyObject* args) {
     if (out.defined() && out.requires_grad() && at::GradMode::is_enabled())
         return refuse(PyExc_RuntimeError, "`out` belongs to a graph or is a leaf that requires a gradient");
     at::Tensor z;
-    std::string error;
-    Py_BEGIN_ALLOW_THREADS
     try {
+        pybind11::gil_scoped_release no_gil;
         z = forward(x, gamma, beta, residual, out, groups, eps, act, slope);
-    } catch (const std::exception& e) {
-        error = e.what();
-        if (error.empty()) error = "gn_act failed";
+    } catch (python_error& e) {                                // a saved-tensor hook's own (activation checkpointing stops by one)
+        e.restore();
+        return PyErr_Occurred() ? nullptr : fail("gn_act: a saved-tensor hook failed");
     }
-    Py_END_ALLOW_THREADS
-    if (!error.empty()) return fail(error);
     return THPVariable_Wrap(z);
 }
