@@ -891,3 +891,29 @@ def test_parameters_that_come_to_share_memory_are_refused():
     a.data, c.data, c.grad = whole[:30], whole[30:], torch.ones(30, device=DEV)
     with pytest.raises(_lib.UResNetHipError, match="size"):
         opt.step()
+
+
+@pytest.mark.gpu
+def test_running_out_of_memory_raises_as_in_torch():
+    """What a program catches to go on with smaller batches; afterwards the calls work."""
+    from uresnet_amd import nn as hnn
+    gn = hnn.GroupNorm(4, 64).to(DEV)
+    x = torch.randn(8, 64, 256, 256, device=DEV).contiguous(memory_format=torch.channels_last)          # 134 MB
+    p = torch.nn.Parameter(torch.zeros(4096, 4096, device=DEV))
+    p.grad = torch.ones(4096, 8192, device=DEV)[:, ::2]                                                # has to be copied: 67 MB
+    opt = train.AdamW([p], lr=0.1, weight_decay=0.0)
+    opt.state_buffers()
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    total = torch.cuda.get_device_properties(0).total_memory
+    try:
+        torch.cuda.set_per_process_memory_fraction((torch.cuda.memory_reserved() + (8 << 20)) / total)
+        for call in (lambda: gn(x), opt.step):
+            with pytest.raises(torch.OutOfMemoryError):
+                call()
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+    version = p._version
+    assert torch.isfinite(gn(x)).all()
+    opt.step()
+    assert (p < 0).all() and p._version == version + 1 and int(opt.state[p]["step"]) == 1

@@ -6,7 +6,6 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
-#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
@@ -233,12 +232,9 @@ PyObject* gn_act(PyObject*, PyObject* args) {
     if (out.defined() && out.requires_grad() && at::GradMode::is_enabled())
         return refuse(PyExc_RuntimeError, "`out` belongs to a graph or is a leaf that requires a gradient");
     at::Tensor z;
-    try {
-        pybind11::gil_scoped_release no_gil;
+    {
+        const pybind11::gil_scoped_release no_gil;
         z = forward(x, gamma, beta, residual, out, groups, eps, act, slope);
-    } catch (python_error& e) {                                // a saved-tensor hook's own (activation checkpointing stops by one)
-        e.restore();
-        return PyErr_Occurred() ? nullptr : fail("gn_act: a saved-tensor hook failed");
     }
     return THPVariable_Wrap(z);
 }

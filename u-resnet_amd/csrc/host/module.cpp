@@ -1,5 +1,8 @@
 #include "host.h"
 
+#include <c10/util/Exception.h>
+#include <torch/csrc/Exceptions.h>
+
 #include <exception>
 #include <stdexcept>
 #include <type_traits>
@@ -36,11 +39,22 @@ PyObject* set_entry_points(PyObject*, PyObject* found) {
     Py_RETURN_NONE;
 }
 
-// C++ exceptions become Python ones
+// C++ exceptions become Python ones: Python's own (out of a saved-tensor hook; activation checkpointing stops by one) and torch's
+// for memory as they are, others the package's
 template <PyObject* (*F)(PyObject*, PyObject*)>
 PyObject* guarded(PyObject* self, PyObject* args) {
     try {
         return F(self, args);
+    } catch (python_error& e) {
+        e.restore();
+        return PyErr_Occurred() ? nullptr : fail("a Python callback failed");
+    } catch (const c10::OutOfMemoryError& e) {
+        PyObject* torch = PyImport_ImportModule("torch");
+        PyObject* type = torch ? PyObject_GetAttrString(torch, "OutOfMemoryError") : nullptr;
+        if (type) PyErr_SetString(type, e.what_without_backtrace());
+        Py_XDECREF(type);
+        Py_XDECREF(torch);
+        return nullptr;
     } catch (const std::exception& e) {
         return fail(e.what());
     }

@@ -6,6 +6,7 @@
 #include <ATen/core/grad_mode.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/utils/pybind.h>
 
 #include <algorithm>
 #include <cmath>
@@ -92,6 +93,12 @@ void count_writes(const std::vector<at::Tensor>& written) {
         if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
+struct Written {                                               // counted when it goes, also by an exception
+    const std::vector<at::Tensor>& tensors;
+    explicit Written(const std::vector<at::Tensor>& t) : tensors(t) {}
+    ~Written() { count_writes(tensors); }
+};
+
 at::Tensor scalar_on(c10::Device device) { return at::empty({}, at::TensorOptions().dtype(at::kFloat).device(device)); }
 
 }  // namespace
@@ -155,13 +162,13 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
         for (Span& s : q.spans) spans.push_back(&s);
     if (spans.empty()) return Py_BuildValue("OO", Py_False, Py_None);
     at::Tensor norm;
-    std::string error;
-    Py_BEGIN_ALLOW_THREADS
-    try {
+    {
+        const pybind11::gil_scoped_release no_gil;
         const c10::DeviceGuard guard(device);
         void* stream = c10::hip::getCurrentHIPStream(device.index()).stream();
         const Memory mem(spans, clip, device);
         if (clip) norm = scalar_on(device);
+        const Written count(written);
         for (Group& q : groups)
             for (Span& s : q.spans)
                 check(entry.param_table(&q.params[s.at], &q.grads[s.at], &q.sizes[s.at], reinterpret_cast<const long long*>(q.blocks) + s.at, s.count,
@@ -182,12 +189,7 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
                                         clip ? mem.parts : nullptr, nparts, (float)max_norm, (float)grad_scale,
                                         clip ? norm.data_ptr<float>() : nullptr, stream),
                       "ur_adamw_multi");
-    } catch (const std::exception& e) {
-        error = *e.what() ? e.what() : "AdamW failed";
     }
-    Py_END_ALLOW_THREADS
-    count_writes(written);
-    if (!error.empty()) return fail(error);
     if (!clip) return Py_BuildValue("OO", Py_True, Py_None);
     return Py_BuildValue("ON", Py_True, THPVariable_Wrap(norm));
 }
@@ -244,8 +246,8 @@ PyObject* clip_grads(PyObject*, PyObject* args) {
     for (Span& s : list) spans.push_back(&s);
     at::Tensor norm;
     std::string error;
-    Py_BEGIN_ALLOW_THREADS
-    try {
+    {
+        const pybind11::gil_scoped_release no_gil;
         const c10::DeviceGuard guard(device);
         norm = scalar_on(device);
         if (spans.empty()) norm.zero_();
@@ -271,10 +273,7 @@ PyObject* clip_grads(PyObject*, PyObject* args) {
                 for (const Span* s : spans)
                     check(entry.grad_clip(s->table, s->count, s->chunks, mem.parts, nparts, (float)max_norm, norm.data_ptr<float>(), stream), "ur_grad_clip");
         }
-    } catch (const std::exception& e) {
-        error = *e.what() ? e.what() : "clip_grad_norm_ failed";
     }
-    Py_END_ALLOW_THREADS
     if (!error.empty()) return fail(error);
     count_writes(written);
     return THPVariable_Wrap(norm);
